@@ -1,0 +1,284 @@
+"""Cases of the channels-last operators: 8-bit activation checkpoints, group norm with an activation, and the weight gradient of a
+dense (1 x 1) layer from a checkpoint.
+
+The 8-bit format: a row's channels in blocks of 32 (the last one may be shorter), one power-of-two scale 2^e a block,
+e = k - 6 for a largest magnitude m 2^k (1 <= m < 2), one more where 64 m >= 127.5, held in [-126, 121]; q = x / 2^e rounded to the nearest
+integer (ties to even) within +-127.  Scales are powers of two, so q is a function of x alone: no second rounding.  A block with an
+infinity or NaN is NaN as a whole.  Storage: q int8 [rows, 32 blocks] padded with zeros, codes uint8 [rows, blocks] = e + 127 (255: NaN)."""
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+EPS = 1e-5
+SQRT2 = math.sqrt(2.0)
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def listed():
+    return [
+        # a 1x1 layer's input of the 64 x 256 maps at batch 16, kept for the backward pass and read back
+        {"name": "pack_bf16_16x64x256_c128", "op": "pack", "dtype": "bf16", "rows": 262144, "ch": 128},
+        # odd everything: a ragged batch of fp32 rows whose last block is short
+        {"name": "pack_fp32_rows10007_c250", "op": "pack", "dtype": "fp32", "rows": 10007, "ch": 250},
+        # one sample of the 8 x 32 maps: a single image is generated, latency counts
+        {"name": "norm_infer_bf16_1x8x32_c256", "op": "norm", "mode": "infer", "dtype": "bf16", "n": 1, "s": 256, "ch": 256, "groups": 32, "act": "silu", "affine": "channel", "sink": False},
+        # the generator's widest maps, a batch of images generated, styles as per-sample scales
+        {"name": "norm_infer_bf16_16x64x256_c128", "op": "norm", "mode": "infer", "dtype": "bf16", "n": 16, "s": 16384, "ch": 128, "groups": 32, "act": "lrelu", "affine": "sample", "sink": False},
+        # the forward pass of a block in training: the output's own 8-bit checkpoint comes from the same launch (the next layer keeps it)
+        {"name": "norm_sink_bf16_16x32x128_c128", "op": "norm", "mode": "infer", "dtype": "bf16", "n": 16, "s": 4096, "ch": 128, "groups": 16, "act": "silu", "affine": "channel", "sink": True},
+        # a training step at full precision, the input kept as it is
+        {"name": "norm_train_fp32_4x32x128_c128", "op": "norm", "mode": "train", "dtype": "fp32", "n": 4, "s": 4096, "ch": 128, "groups": 32, "act": "lrelu", "affine": "channel", "sink": False},
+        # the largest training step: bf16, 8-bit checkpoint, batch 32 of the 64 x 256 maps
+        {"name": "norm_train8_bf16_32x64x256_c128", "op": "norm", "mode": "train8", "dtype": "bf16", "n": 32, "s": 16384, "ch": 128, "groups": 32, "act": "silu", "affine": "channel", "sink": False},
+        # odd: positions, channels and channels a group that no vector width divides, per-sample scales, fp16
+        {"name": "norm_train8_fp16_3x33x65_c120", "op": "norm", "mode": "train8", "dtype": "fp16", "n": 3, "s": 2145, "ch": 120, "groups": 8, "act": "lrelu", "affine": "sample", "sink": False},
+        # a mapping-network-sized layer: few rows
+        {"name": "wgrad_bf16_r512_512x512", "op": "wgrad", "dtype": "bf16", "rows": 512, "cin": 512, "cout": 512},
+        # the largest: a 1x1 layer of 512 channels over 262144 positions
+        {"name": "wgrad_bf16_r262144_512x512", "op": "wgrad", "dtype": "bf16", "rows": 262144, "cin": 512, "cout": 512},
+        # gradients in fp32 (the exact configuration): 32 x 128 maps at batch 4
+        {"name": "wgrad_fp32_r16384_256x256", "op": "wgrad", "dtype": "fp32", "rows": 16384, "cin": 256, "cout": 256},
+        # ragged rows and channels, fp16
+        {"name": "wgrad_fp16_r4099_200x72", "op": "wgrad", "dtype": "fp16", "rows": 4099, "cin": 200, "cout": 72},
+    ]
+
+
+def _log(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["pack", "norm", "norm", "wgrad"])
+    dtype = rng.choice(["bf16", "fp16", "fp32"])
+    if op == "pack":
+        ch = _log(rng, 1, 1024)
+        return {"op": op, "dtype": dtype, "rows": _log(rng, 1, max(1, min(300000, 33554432 // ch))), "ch": ch}
+    if op == "wgrad":
+        cin, cout = _log(rng, 1, 1024), _log(rng, 1, 1024)
+        most = min(262144, 262144 * 512 * 512 // (4 * max(cin, 64) * max(cout, 64)), 200000000 // (cin + 2 * cout))
+        return {"op": op, "dtype": dtype, "rows": _log(rng, 1, most), "cin": cin, "cout": cout}
+    mode = rng.choice(["infer", "train", "train8"])
+    groups = rng.choice([1, 2, 3, 4, 8, 16, 32])
+    ch = groups * _log(rng, 1, max(1, 1024 // groups))
+    n = _log(rng, 1, 32)
+    s = _log(rng, 1, max(1, min(16384, 33554432 // (n * ch))))
+    if mode != "infer":  # a group of a few values only has hardly a gradient: x moves, the normalised values stay
+        s = max(s, -(-16 * groups // ch))
+    # the output's own checkpoint is drawn for 16-bit types: in fp32 the last bit of y decides roundings to 8 bits, which is no error of either side
+    sink = mode == "infer" and dtype != "fp32" and rng.random() < 0.5
+    return {"op": op, "mode": mode, "dtype": dtype, "n": n, "s": s, "ch": ch, "groups": groups, "act": rng.choice(["linear", "lrelu", "silu"]),
+            "affine": rng.choice(["channel", "sample"]), "sink": sink}
+
+
+def _values(g, rows, ch):
+    """What activations look like: channels of their own spread and offset, now and then a far value."""
+    spread = torch.exp(0.7 * torch.randn(ch, generator=g, device=DEV))
+    x = (torch.randn(rows, ch, generator=g, device=DEV) + 0.5 * torch.randn(ch, generator=g, device=DEV)) * spread
+    far = torch.rand(rows, ch, generator=g, device=DEV) < 1e-4
+    return torch.where(far, 8 * x, x)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    t = DTYPES[case["dtype"]]
+    if case["op"] == "pack":
+        return dict(case, x=_values(g, case["rows"], case["ch"]).to(t))
+    if case["op"] == "wgrad":
+        q, e = _pack(_values(g, case["rows"], case["cin"]).to(t))
+        return dict(case, q=q, e=e, dy=torch.randn(case["rows"], case["cout"], generator=g, device=DEV).to(t), coef=1 / math.sqrt(case["cin"]))
+    n, s, ch = case["n"], case["s"], case["ch"]
+    x = _values(g, n * s, ch).reshape(n, s, ch).to(t)
+    shape = (ch,) if case["affine"] == "channel" else (n, ch)
+    gamma = 1 + 0.3 * torch.randn(shape, generator=g, device=DEV)
+    beta = 0.3 * torch.randn(shape, generator=g, device=DEV)
+    st = dict(case, x=x, gamma=gamma, beta=beta)
+    if case["mode"] != "infer":
+        st["dy"] = torch.randn(n, s, ch, generator=g, device=DEV).to(t)
+        st["leaves"] = [v.requires_grad_() for v in (x, gamma, beta)]
+    return st
+
+
+# ---- the plain forms
+
+def _pow2(e):
+    """2^e in 32 bits from its bits, e in [-126, 127]."""
+    return ((e.int() + 127) << 23).view(torch.float32)
+
+
+def _pack(x):
+    rows, ch = x.shape
+    nb = (ch + 31) // 32
+    v = torch.nn.functional.pad(x.float(), (0, nb * 32 - ch)).reshape(rows, nb, 32)
+    amax = v.abs().amax(dim=2)
+    m, k = torch.frexp(amax)                       # amax = m 2^k, 0.5 <= m < 1
+    e = torch.where(amax > 0, k - 7 + (m >= 127.5 / 128).int(), -126).clamp(-126, 121)
+    fine = torch.isfinite(v).all(dim=2)
+    q = (v * _pow2(-e)[:, :, None]).round().clamp(-127, 127)
+    q = torch.where(fine[:, :, None], q, 0)
+    return q.to(torch.int8).reshape(rows, nb * 32), torch.where(fine, e + 127, 255).to(torch.uint8)
+
+
+def _unpack(q, e, ch):
+    rows, nb = e.shape
+    scale = torch.where(e == 255, float("nan"), _pow2(e.int() - 127))
+    return (q.float().reshape(rows, nb, 32) * scale[:, :, None]).reshape(rows, nb * 32)[:, :ch]
+
+
+def _plain_norm(st):
+    x, dtype, mode, act, groups = st["x"].detach(), st["x"].dtype, st["mode"], st["act"], st["groups"]
+    n, s, ch = x.shape
+    per = (lambda v: v.detach().reshape(-1, 1, ch))
+    gamma, beta = per(st["gamma"]), per(st["beta"])
+    spread = (lambda v: v.repeat_interleave(ch // groups, dim=1)[:, None, :])  # [n, groups] -> [n, 1, ch]
+    xf = x.float().reshape(n, s, groups, ch // groups)
+    # 64 bits where the mean decides roundings to 8 bits or the side of the activation's kink a value is on
+    wide = mode == "train8" or (mode == "train" and act == "lrelu")
+    xs = xf.double() if wide else xf
+    mean = xs.mean(dim=(1, 3))
+    var = (xs - mean[:, None, :, None]).square().mean(dim=(1, 3))
+    rstd = (var + EPS).rsqrt()
+    d = xf.reshape(n, s, ch) - spread(mean.float())
+    xh = d * spread(rstd.float())
+    z = gamma * xh + beta
+    y = (z if act == "linear" else SQRT2 * torch.where(z > 0, z, 0.2 * z) if act == "lrelu" else z * torch.sigmoid(z)).to(dtype)
+    if mode == "infer":
+        if not st["sink"]:
+            return y
+        q, e = _pack(y.reshape(n * s, ch))
+        return y, _unpack(q, e, ch).to(dtype).reshape(n, s, ch)
+    if mode == "train8":
+        q, e = _pack(d.reshape(n * s, ch))
+        d = _unpack(q, e, ch).reshape(n, s, ch)
+        xh = d * spread(rstd.float())
+        z = gamma * xh + beta
+    dz = st["dy"].float()
+    if act == "lrelu":
+        z64 = (d.double() if mode == "train8" else x.double() - spread(mean)) * spread(rstd) * gamma.double() + beta.double()
+        dz = dz * torch.where(z64 > 0, SQRT2, 0.2 * SQRT2).float()
+    elif act == "silu":
+        sg = torch.sigmoid(z)
+        dz = dz * (sg * (1 + z * (1 - sg)))
+    over = (lambda v: v.reshape(n, s, groups, ch // groups).sum(dim=(1, 3)) / (s * (ch // groups)))
+    dx = spread(rstd.float()) * (gamma * dz - spread(over(gamma * dz)) - xh * spread(over(gamma * dz * xh)))
+    dims = 1 if st["affine"] == "sample" else (0, 1)
+    return y, dx.to(dtype), (dz * xh).sum(dim=dims), dz.sum(dim=dims)
+
+
+def _plain(st):
+    if st["op"] == "pack":
+        q, e = _pack(st["x"])
+        return _unpack(q, e, st["ch"]).to(st["x"].dtype)
+    if st["op"] == "wgrad":
+        x, dy = _unpack(st["q"], st["e"], st["cin"]), st["dy"].float()
+        return st["coef"] * (x.t() @ dy), dy.sum(dim=0)
+    return _plain_norm(st)
+
+
+# ---- the framework's calls
+
+def _own(st):
+    from textboxgan_amd import ops_cl
+    if st["op"] == "pack":
+        return ops_cl.act8_unpack(ops_cl.act8_pack(st["x"]))
+    if st["op"] == "wgrad":
+        a = ops_cl.Act8(st["q"], st["e"], (st["rows"], st["cin"]), st["dy"].dtype)
+        return ops_cl.act8_wgrad(a, st["dy"], coef=st["coef"])
+    call = (lambda **kw: ops_cl.group_norm_act(st["x"], st["gamma"], st["beta"], st["groups"], act=st["act"], eps=EPS, **kw))
+    if st["mode"] == "infer":
+        if not st["sink"]:
+            return call()
+        y, y8 = call(sink=True)
+        return y, ops_cl.act8_unpack(y8)
+    y = call(save="act8" if st["mode"] == "train8" else "input")
+    return (y.detach(), *torch.autograd.grad(y, st["leaves"], st["dy"]))
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return _plain(state)
+
+
+def work(case):
+    es = 4 if case["dtype"] == "fp32" else 2
+    if case["op"] == "pack":  # x read, the checkpoint written and read, the values written
+        el = case["rows"] * case["ch"]
+        return {"bytes": el * (2 * es + 2 * 33 / 32), "flops": 4 * el}
+    if case["op"] == "wgrad":
+        r, k, c = case["rows"], case["cin"], case["cout"]
+        return {"bytes": r * k * 33 / 32 + r * c * es + 4 * k * c + 4 * c, "flops": 2 * r * k * c}
+    el = case["n"] * case["s"] * case["ch"]
+    if case["mode"] == "infer":  # x read, y written; with a sink the checkpoint written and read, its values written
+        return {"bytes": el * (2 * es + (2 * 33 / 32 + es if case["sink"] else 0)), "flops": 8 * el}
+    # forward: x read, y (and the checkpoint) written; backward: dy and x (or the checkpoint) read, dx written
+    return {"bytes": el * (2 * es + 2 * es + (es if case["mode"] == "train" else 2 * 33 / 32)), "flops": 30 * el}
+
+
+# ---- the definitions in 64 bits
+
+def _two_to(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def _exact_round_trip(x):
+    """The values the 8-bit format keeps of x [rows, ch] (float64, already holding what the format is given)."""
+    rows, ch = x.shape
+    blocks = torch.split(x, 32, dim=1)
+    out = []
+    for b in blocks:
+        big = b.abs().max(dim=1, keepdim=True).values
+        e = torch.floor(torch.log2(big.clamp(min=2.0 ** -140))) - 6
+        e = e + (big * _two_to(-e) >= 128).double() - (big * _two_to(-e) < 64).double()  # the logarithm's own rounding, put right
+        e = (e + (big * _two_to(-e) >= 127.5).double()).clamp(-126, 121)
+        out.append(torch.clamp(torch.round(b * _two_to(-e)), -127, 127) * _two_to(e))
+    return torch.cat(out, dim=1)
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    if case["op"] == "pack":
+        return _exact_round_trip(st["x"].double())
+    if case["op"] == "wgrad":
+        q, codes = st["q"].double(), st["e"].double()
+        x = torch.cat([b * _two_to(codes[:, i:i + 1] - 127) for i, b in enumerate(torch.split(q, 32, dim=1))], dim=1)[:, :case["cin"]]
+        dy = st["dy"].double()
+        return case["cin"] ** -0.5 * torch.matmul(x.t(), dy), dy.sum(dim=0)
+    n, s, ch, groups, act = case["n"], case["s"], case["ch"], case["groups"], case["act"]
+    x = st["x"].detach().double()
+    gam, bet = (v.detach().double().expand(n, ch).reshape(n, 1, groups, -1) for v in (st["gamma"], st["beta"]))
+    xg = x.reshape(n, s, groups, -1)
+    mean = xg.sum(dim=(1, 3), keepdim=True) / (s * ch // groups)
+    sd = torch.sqrt(((xg - mean) ** 2).sum(dim=(1, 3), keepdim=True) / (s * ch // groups) + EPS)
+
+    def f(z):
+        if act == "silu":
+            return z / (1 + torch.exp(-z))
+        return z if act == "linear" else SQRT2 * torch.maximum(z, 0.2 * z)
+
+    def slope(z):
+        if act == "silu":
+            u = torch.exp(-z)
+            return (1 + u + z * u) / (1 + u) ** 2
+        return torch.ones_like(z) if act == "linear" else SQRT2 * (0.2 + 0.8 * (z > 0).double())
+
+    y = f((xg - mean) / sd * gam + bet).reshape(n, s, ch)
+    if case["mode"] == "infer":
+        # the checkpoint is of y as rounded to its type: no value in 64 bits stands for it
+        return (y, None) if case["sink"] else y
+    if case["mode"] == "train8":  # the format is given x - mean in 32 bits, both of them 32-bit numbers
+        c = (st["x"].detach().float().reshape(n, s, groups, -1) - mean.float()).double()
+        hat = _exact_round_trip(c.reshape(n * s, ch)).reshape(n, s, groups, -1) / sd
+    else:
+        hat = (xg - mean) / sd
+    t = st["dy"].double().reshape(n, s, groups, -1) * slope(hat * gam + bet)
+    u = t * gam
+    mu = (lambda v: v.sum(dim=(1, 3), keepdim=True) / (s * ch // groups))
+    dx = ((u - mu(u) - hat * mu(u * hat)) / sd).reshape(n, s, ch)
+    dg, db = (t * hat).sum(dim=1).reshape(n, ch), t.sum(dim=1).reshape(n, ch)
+    if case["affine"] == "channel":
+        dg, db = dg.sum(dim=0), db.sum(dim=0)
+    return y, dx, dg, db
