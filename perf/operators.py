@@ -4,7 +4,10 @@ dense (1 x 1) layer from a checkpoint.
 The 8-bit format: a row's channels in blocks of 32 (the last one may be shorter), one power-of-two scale 2^e a block,
 e = k - 6 for a largest magnitude m 2^k (1 <= m < 2), one more where 64 m >= 127.5, held in [-126, 121]; q = x / 2^e rounded to the nearest
 integer (ties to even) within +-127.  Scales are powers of two, so q is a function of x alone: no second rounding.  A block with an
-infinity or NaN is NaN as a whole.  Storage: q int8 [rows, 32 blocks] padded with zeros, codes uint8 [rows, blocks] = e + 127 (255: NaN)."""
+infinity or NaN is NaN as a whole.  Storage: q int8 [rows, 32 blocks] padded with zeros, codes uint8 [rows, blocks] = e + 127 (255: NaN).
+
+What a group norm with LeakyReLU keeps of x - mean is moved by one step towards the value where rounding has put it on the other side of the
+activation's kink, so that the backward pass takes the slope that the value had."""
 import math
 
 import torch
@@ -152,7 +155,13 @@ def _plain_norm(st):
         return y, _unpack(q, e, ch).to(dtype).reshape(n, s, ch)
     if mode == "train8":
         q, e = _pack(d.reshape(n * s, ch))
-        d = _unpack(q, e, ch).reshape(n, s, ch)
+        kept = _unpack(q, e, ch).reshape(n, s, ch)
+        if act == "lrelu":
+            above = (lambda v: v.double() * (spread(rstd) * gamma.double()) + beta.double() > 0)
+            step = torch.where(above(d) != above(kept), torch.sign(d - kept), 0).reshape(n * s, ch)
+            q[:, :ch] = (q[:, :ch].float() + step).clamp(-127, 127).to(torch.int8)
+            kept = _unpack(q, e, ch).reshape(n, s, ch)
+        d = kept
         xh = d * spread(rstd.float())
         z = gamma * xh + beta
     dz = st["dy"].float()
@@ -224,8 +233,9 @@ def _two_to(e):
     return ((e.long() + 1023) << 52).view(torch.float64)
 
 
-def _exact_round_trip(x):
-    """The values the 8-bit format keeps of x [rows, ch] (float64, already holding what the format is given)."""
+def _exact_round_trip(x, scale=None, shift=None):
+    """The values the 8-bit format keeps of x [rows, ch] (float64, already holding what the format is given); with `scale` and `shift` [rows, ch]
+    on the side of the kink scale v + shift = 0 that x is on, if a step can reach it."""
     rows, ch = x.shape
     blocks = torch.split(x, 32, dim=1)
     out = []
@@ -234,7 +244,13 @@ def _exact_round_trip(x):
         e = torch.floor(torch.log2(big.clamp(min=2.0 ** -140))) - 6
         e = e + (big * _two_to(-e) >= 128).double() - (big * _two_to(-e) < 64).double()  # the logarithm's own rounding, put right
         e = (e + (big * _two_to(-e) >= 127.5).double()).clamp(-126, 121)
-        out.append(torch.clamp(torch.round(b * _two_to(-e)), -127, 127) * _two_to(e))
+        k = torch.clamp(torch.round(b * _two_to(-e)), -127, 127)
+        if scale is not None:
+            a, c = scale[:, :b.shape[1]], shift[:, :b.shape[1]]
+            scale, shift = scale[:, 32:], shift[:, 32:]
+            crossed = (a * b + c > 0) ^ (a * (k * _two_to(e)) + c > 0)
+            k = torch.clamp(k + crossed * ((b > k * _two_to(e)).double() * 2 - 1), -127, 127)
+        out.append(k * _two_to(e))
     return torch.cat(out, dim=1)
 
 
@@ -271,7 +287,8 @@ def exact(case, seed):
         return (y, None) if case["sink"] else y
     if case["mode"] == "train8":  # the format is given x - mean in 32 bits, both of them 32-bit numbers
         c = (st["x"].detach().float().reshape(n, s, groups, -1) - mean.float()).double()
-        hat = _exact_round_trip(c.reshape(n * s, ch)).reshape(n, s, groups, -1) / sd
+        kink = ((gam / sd).expand(c.shape).reshape(n * s, ch), bet.expand(c.shape).reshape(n * s, ch)) if act == "lrelu" else ()
+        hat = _exact_round_trip(c.reshape(n * s, ch), *kink).reshape(n, s, groups, -1) / sd
     else:
         hat = (xg - mean) / sd
     t = st["dy"].double().reshape(n, s, groups, -1) * slope(hat * gam + bet)
