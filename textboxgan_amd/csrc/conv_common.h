@@ -21,8 +21,8 @@ __device__ __forceinline__ bf16x8 pack_bf16x8(const float (&v)[8]) {
 // fp32 -> three bf16 terms hi + mid + lo (8 + 8 + 8 significand bits: exact for every fp32 value whose low terms stay
 // in the normal range).  Products of two bf16 values are exact in fp32, so the six largest partial products of
 // (a_hi + a_mid + a_lo)(b_hi + b_mid + b_lo) reproduce a * b to ~2^-24 relative -- the "f32x3" arithmetic of the X3 kernels.
-// Two values at a time, on packed instructions: v_cvt_pk_bf16_f32 (both conversions), shift / mask (the bf16 pair back to
-// fp32), v_pk_add_f32 (both residuals) -- 9 VALU instructions per pair.  The element-wise form ((__bf16)v, (float)b per element)
+// Two values at a time: v_cvt_pk_bf16_f32 (both conversions), shift / mask (the bf16 pair back to fp32), two subtractions (packed
+// fp32 instructions are off in this library's build) -- 11 VALU instructions per pair.  The element-wise form ((__bf16)v, (float)b per element)
 // compiled to one conversion and one v_perm per ELEMENT and term: ~10 instructions per element in the staging passes
 // (profiles/r03_ab_one_box.txt).  Same roundings, same bits.
 typedef float f32x2v __attribute__((ext_vector_type(2)));
