@@ -612,6 +612,51 @@ int tbg_ema_lerp_f32(float *dst, const float *src, long long n, float beta, void
 int tbg_demod_coefs_f32(const float *s, const float *w, float *wsq, float *d, int B, int T, int I,
                         int O, float coef, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * CHANNELS-LAST LAYERS: rows of channels, [rows][C] or [N][S][C] (S = positions of a sample), channels contiguous.
+ * `dtype` of activations and their gradients: 0 fp32, 1 bf16, 2 fp16; parameters and their gradients are fp32, statistics fp64.
+ * Row / sample pitches are in elements, so that slices of wider tensors need no copy.
+ *
+ * ACT8: 8-bit activation checkpoints.  The channels of a row in blocks of 32 (the last may be shorter), each with one power-of-two
+ * scale 2^e: for a largest magnitude m 2^k (1 <= m < 2), e = k - 6, one more where 64 m >= 127.5, held in [-126, 121]; a value is
+ * kept as q = x / 2^e rounded to the nearest integer (ties to even) within +-127, i.e. to amax / 127 or better; values of blocks below
+ * 2^-120 are kept to 2^-127.  The scale being a power of two, q 2^e has 7 significant bits: exact in bf16, fp32.  A block that holds an
+ * infinity or NaN comes back as NaN.  Storage: q int8 [rows][32 nb] (padding zero), e uint8 [rows][nb] = e + 127 (255: NaN block),
+ * nb = ceil(C / 32); q 16-byte aligned.
+ * tbg_act8_pack: x [rows][ldx] -> q, e.   tbg_act8_unpack: q, e -> x.
+ *
+ * GROUP NORM with an activation.  y = act(gamma xh + beta), xh = (x - mean) / sqrt(var + eps) over the S x C/G values of a (sample,
+ * group); act: 0 linear, 1 LeakyReLU(0.2) x sqrt2, 2 SiLU (z sigmoid(z)).  gamma, beta: [C], or [N][C] with per_sample = 1 (styles).
+ * Forward writes y [N][S][C] contiguous; stats [N][G][2] = mean, rstd if not NULL; (q, e) = ACT8 of fl32(x - fl32(mean)) if not NULL,
+ * for LeakyReLU moved by one step towards the value where rounding has put z on the other side of 0 (the backward pass takes its slope);
+ * (yq, ye) = ACT8 of y as rounded to its type if not NULL (what a following layer keeps of its input).  Backward takes x or (q, e) --
+ * the other NULL --, dy and stats, and writes dx [N][S][C] contiguous, dgamma, dbeta (shaped like gamma): with a checkpoint,
+ * xh = q 2^e rstd everywhere.  Sums are joined in a fixed order.
+ *
+ * tbg_act8_wgrad: gradients of a dense (1x1) layer y = coef x w + b, w [cin][cout], from the checkpoint of x:
+ * dw[k][n] = coef sum_r x[r][k] dy[r][n], db[n] = sum_r dy[r][n] (db NULL: not wanted), fp32 accumulation on the bf16 matrix pipe: the
+ * checkpoint is exact in bf16, dy is one (bf16), two (fp16) or three (fp32) bf16 terms.  dw, db contiguous.
+ * ---------------------------------------------------------------------------------------- */
+#define TBG_ACT_SILU 2
+typedef struct tbg_gn_desc {
+  long long xn, xs; /* sample and row pitch of x (forward; backward without a checkpoint) */
+  long long dn, ds; /* ... of dy (backward; forward: any valid value, e.g. that of y) */
+  int N, S, C, G;   /* samples, positions, channels, groups (C % G == 0) */
+  int dtype, act, per_sample;
+  float eps;
+} tbg_gn_desc;
+int tbg_act8_pack(const void *x, int dtype, long long rows, int ch, long long ldx, void *q, void *e, void *stream);
+int tbg_act8_unpack(const void *q, const void *e, long long rows, int ch, void *x, int dtype, long long ldx, void *stream);
+long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int backward);
+int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const float *gamma, const float *beta, void *y, double *stats, void *q,
+                       void *e, void *yq, void *ye, void *workspace, long long workspace_bytes, void *stream);
+int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const void *q, const void *e, const void *dy, const float *gamma,
+                       const float *beta, const double *stats, void *dx, float *dgamma, float *dbeta, void *workspace,
+                       long long workspace_bytes, void *stream);
+long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int cout, int dtype);
+int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int dtype, long long rows, int cin, int cout, long long ldy, float coef,
+                   float *dw, float *db, void *workspace, long long workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

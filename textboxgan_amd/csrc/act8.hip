@@ -1,0 +1,104 @@
+// 8-bit activation checkpoints (tbg.h "ACT8"): packing rows of channels and reading them back.
+//
+// HBM-bound both ways: es + 1 + 1/32 bytes an element.  A lane holds 8 channels of one row (16-byte loads, 8-byte stores of q), the four
+// lanes of a block find its largest magnitude with two DPP exchanges, so a value is touched once.  Items (row, group of 8 channels) are
+// laid end to end over the lanes whatever the row length, so that short and odd rows waste no lanes.
+#include "act8.h"
+
+template <class E, int V>
+__global__ __launch_bounds__(256) void act8_pack_kernel(const typename E::type *__restrict__ x, long long rows, int ch, long long ldx,
+                                                        unsigned char *__restrict__ q, unsigned char *__restrict__ e, unsigned cols) {
+  // cols = V-channel groups of a padded row (a multiple of 32 / V)
+  const long long base = (long long)blockIdx.x * 256;
+  const long long row0 = base / cols;
+  const unsigned local = (unsigned)(base - row0 * cols) + threadIdx.x;
+  const long long row = row0 + local / cols;
+  const unsigned col = local % cols;
+  if (row >= rows) return;  // whole blocks of 32 channels leave together: cols and 256 are multiples of a block's lanes
+  const int c = (int)col * V;
+  float v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = 0.f;
+  if (c < ch) {
+    const Pack<E, V> p = ld_pack<E, V>(x + row * ldx + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = E::get(p.v[i]);
+  }
+  const unsigned code = a8_code(a8_block_max<V>(v));
+  float t[V];
+  a8_round<V>(v, code, t);
+  a8_store<V>(q + row * ((long long)cols * V) + c, t);
+  if ((c & (A8_BLOCK - 1)) == 0) e[row * (cols * V / A8_BLOCK) + c / A8_BLOCK] = (unsigned char)code;
+}
+
+template <class E, int V>
+__global__ __launch_bounds__(256) void act8_unpack_kernel(const unsigned char *__restrict__ q, const unsigned char *__restrict__ e,
+                                                          long long rows, int ch, typename E::type *__restrict__ x, long long ldx,
+                                                          unsigned cols, unsigned pitch) {
+  // cols = V-channel groups of an unpadded row
+  const long long base = (long long)blockIdx.x * 256;
+  const long long row0 = base / cols;
+  const unsigned local = (unsigned)(base - row0 * cols) + threadIdx.x;
+  const long long row = row0 + local / cols;
+  const int c = (int)(local % cols) * V;
+  if (row >= rows) return;
+  float v[V];
+  a8_load<V>(q + row * pitch + c, a8_scale(e[row * (pitch / A8_BLOCK) + c / A8_BLOCK]), v);
+  Pack<E, V> p;
+#pragma unroll
+  for (int i = 0; i < V; ++i) p.v[i] = E::put(v[i]);
+  st_pack<E, V>(x + row * ldx + c, p);
+}
+
+static int act8_args(const void *x, const void *q, const void *e, int dtype, long long rows, int ch, long long ldx) {
+  if (!x || !q || !e || !dt_valid(dtype) || rows < 1 || ch < 1 || ldx < ch) return TBG_EINVAL;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return TBG_EINVAL;
+  if (ch > (1 << 24)) return TBG_ERANGE;
+  return TBG_OK;
+}
+
+template <class E>
+static int launch_pack(const void *x, int dtype, long long rows, int ch, long long ldx, void *q, void *e, hipStream_t st) {
+  const unsigned padded = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK);
+  const bool vec = ch % 8 == 0 && vec8_ok(x, dtype, ldx);
+  const unsigned cols = vec ? padded / 8 : padded;
+  const long long blocks = (rows * cols + 255) / 256;
+  if (rows > (1LL << 39) / padded || blocks > 0x7fffffffLL) return TBG_ERANGE;
+  auto *xp = reinterpret_cast<const typename E::type *>(x);
+  auto *qp = reinterpret_cast<unsigned char *>(q), *ep = reinterpret_cast<unsigned char *>(e);
+  if (vec) hipLaunchKernelGGL((act8_pack_kernel<E, 8>), dim3((unsigned)blocks), dim3(256), 0, st, xp, rows, ch, ldx, qp, ep, cols);
+  else hipLaunchKernelGGL((act8_pack_kernel<E, 1>), dim3((unsigned)blocks), dim3(256), 0, st, xp, rows, ch, ldx, qp, ep, cols);
+  TBG_LAUNCH_CHECK();
+  return TBG_OK;
+}
+
+template <class E>
+static int launch_unpack(const void *q, const void *e, int dtype, long long rows, int ch, void *x, long long ldx, hipStream_t st) {
+  const unsigned padded = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK);
+  const bool vec = ch % 8 == 0 && vec8_ok(x, dtype, ldx);
+  const unsigned cols = vec ? ch / 8 : ch;
+  const long long blocks = (rows * cols + 255) / 256;
+  if (rows > (1LL << 39) / padded || blocks > 0x7fffffffLL) return TBG_ERANGE;
+  auto *xp = reinterpret_cast<typename E::type *>(x);
+  auto *qp = reinterpret_cast<const unsigned char *>(q), *ep = reinterpret_cast<const unsigned char *>(e);
+  if (vec) hipLaunchKernelGGL((act8_unpack_kernel<E, 8>), dim3((unsigned)blocks), dim3(256), 0, st, qp, ep, rows, ch, xp, ldx, cols, padded);
+  else hipLaunchKernelGGL((act8_unpack_kernel<E, 1>), dim3((unsigned)blocks), dim3(256), 0, st, qp, ep, rows, ch, xp, ldx, cols, padded);
+  TBG_LAUNCH_CHECK();
+  return TBG_OK;
+}
+
+extern "C" int tbg_act8_pack(const void *x, int dtype, long long rows, int ch, long long ldx, void *q, void *e, void *stream) {
+  if (const int rc = act8_args(x, q, e, dtype, rows, ch, ldx)) return rc;
+  hipStream_t st = tbg_stream(stream);
+  return dtype == TBG_DT_F32 ? launch_pack<ElF32>(x, dtype, rows, ch, ldx, q, e, st)
+         : dtype == TBG_DT_BF16 ? launch_pack<ElBf16>(x, dtype, rows, ch, ldx, q, e, st)
+                                : launch_pack<ElF16>(x, dtype, rows, ch, ldx, q, e, st);
+}
+
+extern "C" int tbg_act8_unpack(const void *q, const void *e, long long rows, int ch, void *x, int dtype, long long ldx, void *stream) {
+  if (const int rc = act8_args(x, q, e, dtype, rows, ch, ldx)) return rc;
+  hipStream_t st = tbg_stream(stream);
+  return dtype == TBG_DT_F32 ? launch_unpack<ElF32>(q, e, dtype, rows, ch, x, ldx, st)
+         : dtype == TBG_DT_BF16 ? launch_unpack<ElBf16>(q, e, dtype, rows, ch, x, ldx, st)
+                                : launch_unpack<ElF16>(q, e, dtype, rows, ch, x, ldx, st);
+}

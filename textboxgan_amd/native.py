@@ -27,6 +27,7 @@ EXPORTS = [
     "tbg_units_s2_bytes", "tbg_units_pack_s2_f32", "tbg_upfirdn2d_units_s2_f32", "tbg_conv2d_units_s2_blocks", "tbg_conv2d_units_s2_tile_channels", "tbg_conv2d_units_s2_dot_slots", "tbg_conv2d_units_s2", "tbg_conv2d_wgrad_units_s2_workspace_bytes", "tbg_conv2d_wgrad_units_s2", "tbg_conv2d_units_t2_blocks", "tbg_conv2d_units_t2",
     "tbg_slab_epilogue_units_f32", "tbg_conv2d_units_small", "tbg_conv2d_units_small_blocks", "tbg_conv2d_units_small_dot_slots", "tbg_conv2d_units_small_tile_pixels", "tbg_lstm_fused_fwd_f32", "tbg_lstm_fused_bwd_f32", "tbg_lstm_cell_fused_fwd_f32", "tbg_rows_gemv_t_f32", "tbg_dec_sample_fwd_f32", "tbg_dec_sample_bwd_f32",
     "tbg_bias_act_bwd_f32", "tbg_axpby_planes_f32", "tbg_bias_act_bwd2_f32", "tbg_rgb_project_f32", "tbg_rgb_backproject_f32", "tbg_rgb_backproject_chunks", "tbg_adam_tf_f32", "tbg_ema_lerp_f32", "tbg_demod_coefs_f32",
+    "tbg_act8_pack", "tbg_act8_unpack", "tbg_group_norm_workspace_bytes", "tbg_group_norm_fwd", "tbg_group_norm_bwd", "tbg_act8_wgrad_workspace_bytes", "tbg_act8_wgrad",
 ]
 
 
@@ -65,6 +66,11 @@ class WgradDesc(C.Structure):
                                         "st_t", "st_l", "st_s")] + [("alpha", C.c_float)] +
                 # rider: the layer's bias gradient summed by the filter gradient's reduce launch (tbg.h)
                 [("bias_parts", C.c_void_p), ("bias_grad", C.c_void_p), ("bias_B", C.c_int), ("bias_nch", C.c_int)])
+
+
+class GnDesc(C.Structure):  # tbg_gn_desc
+    _fields_ = ([(n, C.c_longlong) for n in ("xn", "xs", "dn", "ds")] +
+                [(n, C.c_int) for n in ("N", "S", "C", "G", "dtype", "act", "per_sample")] + [("eps", C.c_float)])
 
 
 _lib = None
@@ -177,6 +183,15 @@ def lib():
         l.tbg_adam_tf_f32.argtypes = [vp, vp, vp, vp, ll, cf, cf, cf, cf, vp, vp]
         l.tbg_ema_lerp_f32.argtypes = [vp, vp, ll, cf, vp]
         l.tbg_demod_coefs_f32.argtypes = [vp, vp, vp, vp, ci, ci, ci, ci, cf, vp]
+        l.tbg_act8_pack.argtypes = [vp, ci, ll, ci, ll, vp, vp, vp]
+        l.tbg_act8_unpack.argtypes = [vp, vp, ll, ci, vp, ci, ll, vp]
+        l.tbg_group_norm_workspace_bytes.argtypes = [C.POINTER(GnDesc), ci]
+        l.tbg_group_norm_workspace_bytes.restype = ll
+        l.tbg_group_norm_fwd.argtypes = [C.POINTER(GnDesc)] + [vp] * 10 + [ll, vp]
+        l.tbg_group_norm_bwd.argtypes = [C.POINTER(GnDesc)] + [vp] * 11 + [ll, vp]
+        l.tbg_act8_wgrad_workspace_bytes.argtypes = [ll, ci, ci, ci]
+        l.tbg_act8_wgrad_workspace_bytes.restype = ll
+        l.tbg_act8_wgrad.argtypes = [vp, vp, vp, ci, ll, ci, ci, ll, cf, vp, vp, vp, ll, vp]
         _lib = _LibProxy(l)
     return _lib
 
