@@ -27,7 +27,10 @@ struct ElF16 {
   typedef unsigned short type;
   static constexpr int BYTES = 2;
   static __device__ __forceinline__ float get(unsigned short v) { return (float)__builtin_bit_cast(_Float16, v); }
-  static __device__ __forceinline__ unsigned short put(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
+  static __device__ __forceinline__ unsigned short put(float v) {
+    asm("" : "+v"(v));  // v is rounded to fp32 first in every kernel: without this some products become mixed-precision ones that round once
+    return __builtin_bit_cast(unsigned short, (_Float16)v);
+  }
 };
 
 // V consecutive elements of a row.  V = 8: 16-byte accesses (the caller has checked the alignment); V = 1: one element.

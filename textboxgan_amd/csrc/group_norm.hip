@@ -21,34 +21,50 @@ struct GnP {
   unsigned char *yq, *ye;              // forward: checkpoint of y, or null
   double *stats;                       // [N][G][2] mean, rstd
   double *part;                        // forward: [N][nchunk][nslot][2] sum x, sum x^2; backward: sum gamma dz, sum gamma dz xh
-  float *pch;                          // backward: [N][nchunk][Cp][2] sum dz, sum dz xh of a channel
+  float *pch;                          // backward: [N][nchunk][C][2] sum dz, sum dz xh of a channel
   float *dgamma, *dbeta;
   long long xn, xs, dn, ds;            // sample / row pitches of x and dy in elements (y, dx: contiguous)
   int N, S, C, G, Cg, affn, nb;        // affn: affine parameters' sample pitch (0 or C); nb: 8-bit blocks a row
-  int CT, ntile, lanes, RL;            // channels a tile, tiles, lanes a row, rows a pass
+  int n0, nn;                          // samples of this launch
+  int CT, ntile, lanes;                // channels a tile (a power of two), tiles, lanes a row
   int nchunk, crows, nslot;            // row ranges of the sums launch
-  int achunk, arows;                   // row ranges of the second launch
+  int split, arows;                    // the second launch's part of a row range: `split` pieces of arows rows
   int pblocks;                         // backward: first blocks of the second launch that sum dgamma / dbeta
   float eps;
 };
 
-constexpr int GN_T = 256, GN_CT = 128;  // threads a block, most channels a tile
+constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_CT = 128;  // threads a block: second launches, forward sums, backward sums; most channels a tile
 
 template <int ACT>
 __device__ __forceinline__ float gn_act(float z) {
   if constexpr (ACT == TBG_ACT_LRELU) return 1.41421356237309515f * (z > 0.f ? z : 0.2f * z);
-  if constexpr (ACT == TBG_ACT_SILU) return z / (1.f + __expf(-z));
+  if constexpr (ACT == TBG_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
   return z;
 }
-// dy act'(z).  z64: LeakyReLU's side of the kink is decided in 64 bits, so that it does not hang on the last bit of a 32-bit product
+// dy act'(z).  positive: LeakyReLU's side of the kink, decided in 64 bits so that it does not hang on the last bit of a 32-bit product
 template <int ACT>
 __device__ __forceinline__ float gn_dact(float dy, float z, bool positive) {
   if constexpr (ACT == TBG_ACT_LRELU) return dy * (positive ? 1.41421356237309515f : 0.282842712474619f);
-  if constexpr (ACT == TBG_ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return dy * (s * (1.f + z * (1.f - s)));
+  if constexpr (ACT == TBG_ACT_SILU) {  // s + z s (1 - s)
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z)), u = z * s;
+    return dy * (fmaf(-u, s, u) + s);
   }
   return dy;
+}
+
+// what a block of the sums launch works on: row range k of a tile of a sample.  Row ranges vary fastest in both launches and their count is
+// a multiple of 8 where there are that many: a row range then stays on one of the 8 XCDs, whose L2 still holds it for the second launch
+struct GnTile {
+  int n, tile, k, c0, ct;
+};
+__device__ __forceinline__ GnTile gn_tile(const GnP &p, int b) {
+  GnTile t;
+  t.k = b % p.nchunk; b /= p.nchunk;
+  t.tile = b % p.ntile;
+  t.n = p.n0 + b / p.ntile;
+  t.c0 = t.tile * p.CT;
+  t.ct = min(p.CT, p.C - t.c0);
+  return t;
 }
 
 // sums of one group's partial pairs over its tiles and the row ranges, by `sub` neighbouring lanes (a power of two), all of which get it
@@ -58,9 +74,9 @@ __device__ __forceinline__ void gn_join(const GnP &p, int n, int g, int lane, in
   const double *base = p.part + (long long)n * p.nchunk * p.nslot * 2;
   for (int i = lane; i < nt * p.nchunk; i += sub) {
     const int k = i / nt, t = t0 + i - k * nt;
-    const double *s = base + ((long long)k * p.nslot + t + g) * 2;
-    a += s[0];
-    b += s[1];
+    const double2 s = *reinterpret_cast<const double2 *>(base + ((long long)k * p.nslot + t + g) * 2);
+    a += s.x;
+    b += s.y;
   }
   for (int off = sub >> 1; off > 0; off >>= 1) {
     a += __shfl_xor(a, off, 64);
@@ -68,94 +84,101 @@ __device__ __forceinline__ void gn_join(const GnP &p, int n, int g, int lane, in
   }
 }
 
-// ---- forward, first launch: sums of x and x^2
-template <class E, int V>
-__global__ __launch_bounds__(GN_T) void gn_sums_kernel(GnP p) {
-  __shared__ double red[GN_T * V * 2];
-  int b = blockIdx.x;
-  const int k = b % p.nchunk; b /= p.nchunk;
-  const int tile = b % p.ntile, n = b / p.ntile;
-  const int c0 = tile * p.CT, ct = min(p.CT, p.C - c0);
-  const int lane = threadIdx.x % p.lanes, rl = threadIdx.x / p.lanes;
-  const int r0 = k * p.crows, r1 = min(p.S, r0 + p.crows);
-  double s1[V], s2[V];
+// ---- forward, first launch: sums of x and x^2.  V / A neighbouring channels share a group (A accumulators a lane)
+template <class E, int V, int A>
+__global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
+  constexpr int U = 4, NW = GN_TS / 64;
+  __shared__ double red[NW * (GN_CT / V) * A * 2];
+  const GnTile t = gn_tile(p, blockIdx.x);
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TS / p.lanes;
+  const int r1 = min(p.S, (t.k + 1) * p.crows);
+  double s1[A], s2[A];
 #pragma unroll
-  for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0;
-  if (rl < p.RL && lane * V < ct) {
-    const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + c0 + lane * V;
-#pragma unroll 4
-    for (int r = r0 + rl; r < r1; r += p.RL) {
-      const Pack<E, V> v = ld_pack<E, V>(x + r * p.xs);
+  for (int i = 0; i < A; ++i) s1[i] = s2[i] = 0.0;
+  if (lane * V < t.ct) {
+    const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + t.c0 + lane * V;
+    const auto add = [&](const Pack<E, V> &v) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const double d = E::get(v.v[i]);
-        s1[i] += d;
-        s2[i] = fma(d, d, s2[i]);
+        s1[i * A / V] += d;
+        s2[i * A / V] = fma(d, d, s2[i * A / V]);
       }
-    }
-  }
+    };
+    int r = t.k * p.crows + rl;
+    for (; r + (U - 1) * RL < r1; r += U * RL) {
+      Pack<E, V> v[U];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    red[(threadIdx.x * V + i) * 2] = s1[i];
-    red[(threadIdx.x * V + i) * 2 + 1] = s2[i];
-  }
-  __syncthreads();
-  const int row = p.lanes * V;  // channels of one row lane in `red`
-  for (int c = threadIdx.x; c < ct; c += GN_T) {
-    double a = red[c * 2], q = red[c * 2 + 1];
-    for (int j = 1; j < p.RL; ++j) {
-      a += red[(j * row + c) * 2];
-      q += red[(j * row + c) * 2 + 1];
+      for (int u = 0; u < U; ++u) v[u] = ld_pack<E, V>(x + (r + u * RL) * p.xs);
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(v[u]);
     }
-    red[c * 2] = a;
-    red[c * 2 + 1] = q;
+    for (; r < r1; r += RL) add(ld_pack<E, V>(x + r * p.xs));
+  }
+  // rows of a wave by lane exchanges, the waves through LDS
+  for (int off = p.lanes; off < 64; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      s1[i] += __shfl_xor(s1[i], off, 64);
+      s2[i] += __shfl_xor(s2[i], off, 64);
+    }
+  const int wave = threadIdx.x >> 6, cols = p.lanes * A;  // partial sums a wave: cols of (64 / lanes rows joined)
+  if ((threadIdx.x & 63) < p.lanes)
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      red[(wave * cols + lane * A + i) * 2] = s1[i];
+      red[(wave * cols + lane * A + i) * 2 + 1] = s2[i];
+    }
+  __syncthreads();
+  if (threadIdx.x < 2 * cols) {
+    double a = red[threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) a += red[w * 2 * cols + threadIdx.x];
+    red[threadIdx.x] = a;
   }
   __syncthreads();
-  const int g0 = c0 / p.Cg, g1 = (c0 + ct - 1) / p.Cg;
-  for (int g = g0 + threadIdx.x; g <= g1; g += GN_T) {
-    const int a0 = max(g * p.Cg - c0, 0), a1 = min((g + 1) * p.Cg - c0, ct);
-    double a = 0.0, q = 0.0;
+  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg, step = V / A;
+  for (int g = g0 + threadIdx.x; g <= g1; g += GN_TS) {
+    const int a0 = max(g * p.Cg - t.c0, 0) / step, a1 = min((g + 1) * p.Cg - t.c0, t.ct) / step;
+    double2 o = {0.0, 0.0};
     for (int c = a0; c < a1; ++c) {
-      a += red[c * 2];
-      q += red[c * 2 + 1];
+      o.x += red[c * 2];
+      o.y += red[c * 2 + 1];
     }
-    double *o = p.part + (((long long)n * p.nchunk + k) * p.nslot + tile + g) * 2;
-    o[0] = a;
-    o[1] = q;
+    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = o;
   }
 }
 
-// ---- forward, second launch
-template <class E, int V, int ACT>
+// ---- forward, second launch.  Q: checkpoints are written
+template <class E, int V, int ACT, bool Q>
 __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
+  constexpr int U = 4;
   __shared__ double st[2 * GN_CT];  // mean, rstd of the tile's groups
-  int b = blockIdx.x;
-  const int k = b % p.achunk; b /= p.achunk;
-  const int tile = b % p.ntile, n = b / p.ntile;
-  const int c0 = tile * p.CT, ct = min(p.CT, p.C - c0);
-  const int g0 = c0 / p.Cg, ng = (c0 + ct - 1) / p.Cg - g0 + 1;
+  const int piece = blockIdx.x / p.nchunk % p.split;
+  const GnTile t = gn_tile(p, blockIdx.x / p.nchunk / p.split * p.nchunk + blockIdx.x % p.nchunk);
+  const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
   int sub = 64;
   while (sub > 1 && ng * sub > GN_T) sub >>= 1;
   for (int i = threadIdx.x; i < ng * sub; i += GN_T) {
     const int g = g0 + i / sub;
     double a, q;
-    gn_join(p, n, g, i % sub, sub, a, q);
+    gn_join(p, t.n, g, i % sub, sub, a, q);
     const double m = (double)p.S * p.Cg, mean = a / m, var = q / m - mean * mean;
     const double rstd = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps);  // (a NaN stays one)
     if (i % sub == 0) {
       st[(g - g0) * 2] = mean;
       st[(g - g0) * 2 + 1] = rstd;
-      if (p.stats && k == 0 && g * p.Cg >= c0) {  // the tile in which the group begins
-        p.stats[((long long)n * p.G + g) * 2] = mean;
-        p.stats[((long long)n * p.G + g) * 2 + 1] = rstd;
+      if (p.stats && t.k == 0 && piece == 0 && g * p.Cg >= t.c0) {  // the tile in which the group begins
+        p.stats[((long long)t.n * p.G + g) * 2] = mean;
+        p.stats[((long long)t.n * p.G + g) * 2 + 1] = rstd;
       }
     }
   }
   __syncthreads();
-  const int lane = threadIdx.x % p.lanes, rl = threadIdx.x / p.lanes;
-  const int c = c0 + lane * V;
-  if (rl >= p.RL || c >= p.nb * A8_BLOCK) return;  // whole 8-bit blocks leave together
-  const bool in = lane * V < ct;                   // the others of the last block write the checkpoints' padding
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes;
+  const int c = t.c0 + lane * V;
+  if (c >= p.nb * A8_BLOCK) return;    // whole 8-bit blocks leave together
+  const bool in = lane * V < t.ct;     // the others of the last block write the checkpoints' padding
   float mu[V], sc[V], sh[V];
   double sc64[V], be64[V];  // LeakyReLU's kink in 64 bits, as the backward pass has it
 #pragma unroll
@@ -165,7 +188,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
     if (in) {
       const int g = (c + i) / p.Cg - g0;
       const double mean = st[g * 2], rstd = st[g * 2 + 1];
-      const float ga = p.gamma[(long long)n * p.affn + c + i], be = p.beta[(long long)n * p.affn + c + i];
+      const float ga = p.gamma[(long long)t.n * p.affn + c + i], be = p.beta[(long long)t.n * p.affn + c + i];
       mu[i] = (float)mean;
       sc[i] = ga * (float)rstd;
       sh[i] = (float)((double)be - (mean - (double)mu[i]) * rstd * (double)ga);
@@ -173,162 +196,190 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
       be64[i] = be;
     }
   }
-  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + c;
-  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + (long long)n * p.S * p.C + c;
-  const int r1 = min(p.S, (k + 1) * p.arows);
-#pragma unroll 2
-  for (int r = k * p.arows + rl; r < r1; r += p.RL) {
+  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + c;
+  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + (long long)t.n * p.S * p.C + c;
+  const auto write = [&](int r, const Pack<E, V> &v) {
     float d[V], o[V];
+    Pack<E, V> w;
 #pragma unroll
-    for (int i = 0; i < V; ++i) d[i] = o[i] = 0.f;
-    if (in) {
-      const Pack<E, V> v = ld_pack<E, V>(x + r * p.xs);
-      Pack<E, V> w;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        d[i] = E::get(v.v[i]) - mu[i];
-        w.v[i] = E::put(gn_act<ACT>(fmaf(d[i], sc[i], sh[i])));
-        o[i] = E::get(w.v[i]);
-      }
-      st_pack<E, V>(y + (long long)r * p.C, w);
+    for (int i = 0; i < V; ++i) {
+      d[i] = E::get(v.v[i]) - mu[i];
+      w.v[i] = E::put(gn_act<ACT>(fmaf(d[i], sc[i], sh[i])));
+      o[i] = E::get(w.v[i]);
     }
-    const long long row = (long long)n * p.S + r;
-    if (p.q) {
-      const unsigned code = a8_code(a8_block_max<V>(d));
-      float t[V];
-      a8_round<V>(d, code, t);
-      if constexpr (ACT == TBG_ACT_LRELU) {  // one step back where rounding has crossed the kink: the backward pass takes the value's own slope
-        const float scale = a8_scale(code);
+    if (!Q || in) st_pack<E, V>(y + (long long)r * p.C, w);
+    if constexpr (Q) {
+      const long long row = (long long)t.n * p.S + r;
+      if (!in) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float kept = t[i] * scale;
-          if ((fma((double)d[i], sc64[i], be64[i]) > 0.0) != (fma((double)kept, sc64[i], be64[i]) > 0.0))
-            t[i] = fminf(fmaxf(t[i] + (d[i] > kept ? 1.f : -1.f), -127.f), 127.f);
+        for (int i = 0; i < V; ++i) d[i] = o[i] = 0.f;
+      }
+      if (p.q) {
+        const unsigned code = a8_code(a8_block_max<V>(d));
+        float k[V];
+        a8_round<V>(d, code, k);
+        if constexpr (ACT == TBG_ACT_LRELU) {  // one step back where rounding has crossed the kink: the backward pass takes the value's own slope
+          const float scale = a8_scale(code);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float kept = k[i] * scale;
+            if ((fma((double)d[i], sc64[i], be64[i]) > 0.0) != (fma((double)kept, sc64[i], be64[i]) > 0.0))
+              k[i] = fminf(fmaxf(k[i] + (d[i] > kept ? 1.f : -1.f), -127.f), 127.f);
+          }
         }
+        a8_store<V>(p.q + row * p.nb * A8_BLOCK + c, k);
+        if ((c & (A8_BLOCK - 1)) == 0) p.e[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
       }
-      a8_store<V>(p.q + row * p.nb * A8_BLOCK + c, t);
-      if ((c & (A8_BLOCK - 1)) == 0) p.e[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
+      if (p.yq) {
+        const unsigned code = a8_code(a8_block_max<V>(o));
+        float k[V];
+        a8_round<V>(o, code, k);
+        a8_store<V>(p.yq + row * p.nb * A8_BLOCK + c, k);
+        if ((c & (A8_BLOCK - 1)) == 0) p.ye[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
+      }
     }
-    if (p.yq) {
-      const unsigned code = a8_code(a8_block_max<V>(o));
-      float t[V];
-      a8_round<V>(o, code, t);
-      a8_store<V>(p.yq + row * p.nb * A8_BLOCK + c, t);
-      if ((c & (A8_BLOCK - 1)) == 0) p.ye[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
-    }
+  };
+  if (!Q && !in) return;
+  const Pack<E, V> zero = {};
+  const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
+  int r = t.k * p.crows + piece * p.arows + rl;
+  for (; r + (U - 1) * RL < r1; r += U * RL) {
+    Pack<E, V> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = in ? ld_pack<E, V>(x + (r + u * RL) * p.xs) : zero;
+#pragma unroll
+    for (int u = 0; u < U; ++u) write(r + u * RL, v[u]);
   }
+  for (; r < r1; r += RL) write(r, in ? ld_pack<E, V>(x + r * p.xs) : zero);
 }
 
-// ---- backward: what a lane knows of its V channels
+// ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd: a lane keeps z = sc d + be of its V channels
 template <int V>
 struct GnCh {
-  float mu[V], lo[V], rstd[V], ga[V], be[V];
+  float mu[V], lo[V], sc[V], be[V];
   double sc64[V];
 };
 template <int V, bool Q8>
-__device__ __forceinline__ void gn_channels(const GnP &p, int n, int c, bool in, GnCh<V> &h) {
+__device__ __forceinline__ void gn_channels(const GnP &p, int n, int c, GnCh<V> &h) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    h.mu[i] = h.lo[i] = h.rstd[i] = h.ga[i] = h.be[i] = 0.f;
-    h.sc64[i] = 0.0;
-    if (in) {
-      const double *s = p.stats + ((long long)n * p.G + (c + i) / p.Cg) * 2;
-      h.mu[i] = Q8 ? 0.f : (float)s[0];
-      h.lo[i] = Q8 ? 0.f : (float)(s[0] - (double)(float)s[0]);
-      h.rstd[i] = (float)s[1];
-      h.ga[i] = p.gamma[(long long)n * p.affn + c + i];
-      h.be[i] = p.beta[(long long)n * p.affn + c + i];
-      h.sc64[i] = s[1] * (double)h.ga[i];
-    }
+    const double2 s = *reinterpret_cast<const double2 *>(p.stats + ((long long)n * p.G + (c + i) / p.Cg) * 2);
+    const float ga = p.gamma[(long long)n * p.affn + c + i];
+    h.mu[i] = Q8 ? 0.f : (float)s.x;
+    h.lo[i] = Q8 ? 0.f : (float)(s.x - (double)(float)s.x);
+    h.sc64[i] = s.y * (double)ga;
+    h.sc[i] = (float)h.sc64[i];
+    h.be[i] = p.beta[(long long)n * p.affn + c + i];
   }
 }
-// xh and dz of one row
-template <class E, int V, int ACT, bool Q8>
-__device__ __forceinline__ void gn_row(const GnP &p, const GnCh<V> &h, int n, int r, int c, float (&xh)[V], float (&dz)[V]) {
-  float d[V];
+// a row's operands as they lie in memory
+template <class E, int V, bool Q8>
+struct GnRow {
+  Pack<E, V> g, x;
+  u32x2 q;
+  unsigned e;
+};
+template <class E, int V, bool Q8>
+__device__ __forceinline__ GnRow<E, V, Q8> gn_load(const GnP &p, int n, int r, int c) {
+  GnRow<E, V, Q8> w;
   if constexpr (Q8) {
     const long long row = (long long)n * p.S + r;
-    a8_load<V>(p.q + row * p.nb * A8_BLOCK + c, a8_scale(p.e[row * p.nb + c / A8_BLOCK]), d);
+    w.e = p.e[row * p.nb + c / A8_BLOCK];
+    if constexpr (V == 8) w.q = *reinterpret_cast<const u32x2 *>(p.q + row * p.nb * A8_BLOCK + c);
+    else w.q[0] = p.q[row * p.nb * A8_BLOCK + c];
   } else {
-    const Pack<E, V> v = ld_pack<E, V>(reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + r * p.xs + c);
-#pragma unroll
-    for (int i = 0; i < V; ++i) d[i] = (E::get(v.v[i]) - h.mu[i]) - h.lo[i];
+    w.x = ld_pack<E, V>(reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + r * p.xs + c);
   }
-  const Pack<E, V> g = ld_pack<E, V>(reinterpret_cast<const typename E::type *>(p.dy) + n * p.dn + r * p.ds + c);
+  w.g = ld_pack<E, V>(reinterpret_cast<const typename E::type *>(p.dy) + n * p.dn + r * p.ds + c);
+  return w;
+}
+// d and dz of a row
+template <class E, int V, int ACT, bool Q8>
+__device__ __forceinline__ void gn_row(const GnRow<E, V, Q8> &w, const GnCh<V> &h, float (&d)[V], float (&dz)[V]) {
+  const float scale = Q8 ? a8_scale(w.e) : 1.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    xh[i] = d[i] * h.rstd[i];
-    const float z = fmaf(xh[i], h.ga[i], h.be[i]);
+    if constexpr (Q8) d[i] = (float)(int)(signed char)(w.q[i >> 2] >> (8 * (i & 3)) & 0xff) * scale;
+    else d[i] = (E::get(w.x.v[i]) - h.mu[i]) - h.lo[i];
+    const float z = ACT == TBG_ACT_SILU ? fmaf(d[i], h.sc[i], h.be[i]) : 0.f;
     const bool pos = ACT == TBG_ACT_LRELU ? fma((double)d[i], h.sc64[i], (double)h.be[i]) > 0.0 : false;
-    dz[i] = gn_dact<ACT>(E::get(g.v[i]), z, pos);
+    dz[i] = gn_dact<ACT>(E::get(w.g.v[i]), z, pos);
   }
 }
 
 // ---- backward, first launch: sums of dz and dz xh of every channel, and of gamma dz and gamma dz xh of every group
 template <class E, int V, int ACT, bool Q8>
-__global__ __launch_bounds__(GN_T) void gn_bwd_sums_kernel(GnP p) {
-  __shared__ float red[GN_T * V * 2];
-  int b = blockIdx.x;
-  const int k = b % p.nchunk; b /= p.nchunk;
-  const int tile = b % p.ntile, n = b / p.ntile;
-  const int c0 = tile * p.CT, ct = min(p.CT, p.C - c0);
-  const int lane = threadIdx.x % p.lanes, rl = threadIdx.x / p.lanes;
-  const int r1 = min(p.S, (k + 1) * p.crows), c = c0 + lane * V;
+__global__ __launch_bounds__(GN_TB, V == 8 ? 4 : 8) void gn_bwd_sums_kernel(GnP p) {
+  constexpr int U = 2, NW = GN_TB / 64;
+  __shared__ float red[NW * GN_CT * 2];
+  const GnTile t = gn_tile(p, blockIdx.x);
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TB / p.lanes;
+  const int r1 = min(p.S, (t.k + 1) * p.crows), c = t.c0 + lane * V;
   float s1[V], s2[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-  if (rl < p.RL && lane * V < ct) {
+  if (lane * V < t.ct) {
     GnCh<V> h;
-    gn_channels<V, Q8>(p, n, c, true, h);
-#pragma unroll 2
-    for (int r = k * p.crows + rl; r < r1; r += p.RL) {
-      float xh[V], dz[V];
-      gn_row<E, V, ACT, Q8>(p, h, n, r, c, xh, dz);
+    gn_channels<V, Q8>(p, t.n, c, h);
+    const auto add = [&](const GnRow<E, V, Q8> &w) {
+      float d[V], dz[V];
+      gn_row<E, V, ACT, Q8>(w, h, d, dz);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         s1[i] += dz[i];
-        s2[i] = fmaf(dz[i], xh[i], s2[i]);
+        s2[i] = fmaf(dz[i], d[i], s2[i]);
       }
-    }
-  }
+    };
+    int r = t.k * p.crows + rl;
+    for (; r + (U - 1) * RL < r1; r += U * RL) {
+      GnRow<E, V, Q8> w[U];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    red[(threadIdx.x * V + i) * 2] = s1[i];
-    red[(threadIdx.x * V + i) * 2 + 1] = s2[i];
-  }
-  __syncthreads();
-  const int row = p.lanes * V;
-  for (int j = threadIdx.x; j < ct; j += GN_T) {
-    float a = red[j * 2], q = red[j * 2 + 1];
-    for (int l = 1; l < p.RL; ++l) {
-      a += red[(l * row + j) * 2];
-      q += red[(l * row + j) * 2 + 1];
+      for (int u = 0; u < U; ++u) w[u] = gn_load<E, V, Q8>(p, t.n, r + u * RL, c);
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(w[u]);
     }
-    red[j * 2] = a;
-    red[j * 2 + 1] = q;
-    float *o = p.pch + (((long long)n * p.nchunk + k) * p.C + c0 + j) * 2;
-    o[0] = a;
-    o[1] = q;
+    for (; r < r1; r += RL) add(gn_load<E, V, Q8>(p, t.n, r, c));
+  }
+  for (int off = p.lanes; off < 64; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s1[i] += __shfl_xor(s1[i], off, 64);
+      s2[i] += __shfl_xor(s2[i], off, 64);
+    }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) < p.lanes)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      red[(wave * p.CT + lane * V + i) * 2] = s1[i];
+      red[(wave * p.CT + lane * V + i) * 2 + 1] = s2[i];
+    }
+  __syncthreads();
+  if (threadIdx.x < 2 * t.ct) {
+    float a = red[threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) a += red[w * 2 * p.CT + threadIdx.x];
+    if (threadIdx.x & 1) a *= (float)p.stats[((long long)t.n * p.G + (t.c0 + (threadIdx.x >> 1)) / p.Cg) * 2 + 1];  // d -> xh
+    red[threadIdx.x] = a;
+    p.pch[(((long long)t.n * p.nchunk + t.k) * p.C + t.c0) * 2 + threadIdx.x] = a;
   }
   __syncthreads();
-  const int g0 = c0 / p.Cg, g1 = (c0 + ct - 1) / p.Cg;
-  for (int g = g0 + threadIdx.x; g <= g1; g += GN_T) {
-    const int a0 = max(g * p.Cg - c0, 0), a1 = min((g + 1) * p.Cg - c0, ct);
-    double a = 0.0, q = 0.0;
+  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg;
+  for (int g = g0 + threadIdx.x; g <= g1; g += GN_TB) {
+    const int a0 = max(g * p.Cg - t.c0, 0), a1 = min((g + 1) * p.Cg - t.c0, t.ct);
+    double2 o = {0.0, 0.0};
     for (int j = a0; j < a1; ++j) {
-      const double ga = p.gamma[(long long)n * p.affn + c0 + j];
-      a = fma(ga, (double)red[j * 2], a);
-      q = fma(ga, (double)red[j * 2 + 1], q);
+      const double ga = p.gamma[(long long)t.n * p.affn + t.c0 + j];
+      o.x = fma(ga, (double)red[j * 2], o.x);
+      o.y = fma(ga, (double)red[j * 2 + 1], o.y);
     }
-    double *o = p.part + (((long long)n * p.nchunk + k) * p.nslot + tile + g) * 2;
-    o[0] = a;
-    o[1] = q;
+    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = o;
   }
 }
 
 // ---- backward, second launch: dx, and in its first blocks dgamma / dbeta
 template <class E, int V, int ACT, bool Q8>
-__global__ __launch_bounds__(GN_T) void gn_bwd_dx_kernel(GnP p) {
+__global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) {
+  constexpr int U = 2;
   __shared__ double st[2 * GN_CT];  // means of gamma dz and gamma dz xh over the tile's groups
   int b = blockIdx.x;
   if (b < p.pblocks) {  // 8 lanes a channel: the row ranges (and samples, where the parameters are shared) in a fixed order
@@ -340,9 +391,9 @@ __global__ __launch_bounds__(GN_T) void gn_bwd_dx_kernel(GnP p) {
       const long long len = (long long)(p.affn ? 1 : p.N) * p.nchunk;
       double a = 0.0, q = 0.0;
       for (long long i = sub; i < len; i += 8) {
-        const float *s = p.pch + (((long long)n * p.nchunk + i) * p.C + c) * 2;
-        a += s[0];
-        q += s[1];
+        const float2 s = *reinterpret_cast<const float2 *>(p.pch + (((long long)n * p.nchunk + i) * p.C + c) * 2);
+        a += s.x;
+        q += s.y;
       }
 #pragma unroll
       for (int off = 4; off > 0; off >>= 1) {
@@ -357,15 +408,14 @@ __global__ __launch_bounds__(GN_T) void gn_bwd_dx_kernel(GnP p) {
     return;
   }
   b -= p.pblocks;
-  const int k = b % p.achunk; b /= p.achunk;
-  const int tile = b % p.ntile, n = b / p.ntile;
-  const int c0 = tile * p.CT, ct = min(p.CT, p.C - c0);
-  const int g0 = c0 / p.Cg, ng = (c0 + ct - 1) / p.Cg - g0 + 1;
+  const int piece = b / p.nchunk % p.split;
+  const GnTile t = gn_tile(p, b / p.nchunk / p.split * p.nchunk + b % p.nchunk);
+  const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
   int sub = 64;
   while (sub > 1 && ng * sub > GN_T) sub >>= 1;
   for (int i = threadIdx.x; i < ng * sub; i += GN_T) {
     double a, q;
-    gn_join(p, n, g0 + i / sub, i % sub, sub, a, q);
+    gn_join(p, t.n, g0 + i / sub, i % sub, sub, a, q);
     const double m = (double)p.S * p.Cg;
     if (i % sub == 0) {
       st[(i / sub) * 2] = a / m;
@@ -373,29 +423,38 @@ __global__ __launch_bounds__(GN_T) void gn_bwd_dx_kernel(GnP p) {
     }
   }
   __syncthreads();
-  const int lane = threadIdx.x % p.lanes, rl = threadIdx.x / p.lanes;
-  if (rl >= p.RL || lane * V >= ct) return;
-  const int c = c0 + lane * V;
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes;
+  if (lane * V >= t.ct) return;
+  const int c = t.c0 + lane * V;
   GnCh<V> h;
-  gn_channels<V, Q8>(p, n, c, true, h);
-  float m1[V], m2[V];
+  gn_channels<V, Q8>(p, t.n, c, h);
+  float m1[V], m2[V];  // dx = sc dz - m1 - d m2, m1 = rstd mean(gamma dz), m2 = rstd^2 mean(gamma dz xh)
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int g = (c + i) / p.Cg - g0;
-    m1[i] = (float)st[g * 2];
-    m2[i] = (float)st[g * 2 + 1];
+    const double rstd = p.stats[((long long)t.n * p.G + g0 + g) * 2 + 1];
+    m1[i] = (float)(rstd * st[g * 2]);
+    m2[i] = (float)(rstd * rstd * st[g * 2 + 1]);
   }
-  typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + (long long)n * p.S * p.C + c;
-  const int r1 = min(p.S, (k + 1) * p.arows);
-#pragma unroll 2
-  for (int r = k * p.arows + rl; r < r1; r += p.RL) {
-    float xh[V], dz[V];
-    gn_row<E, V, ACT, Q8>(p, h, n, r, c, xh, dz);
-    Pack<E, V> w;
+  typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + (long long)t.n * p.S * p.C + c;
+  const auto write = [&](int r, const GnRow<E, V, Q8> &w) {
+    float d[V], dz[V];
+    gn_row<E, V, ACT, Q8>(w, h, d, dz);
+    Pack<E, V> o;
 #pragma unroll
-    for (int i = 0; i < V; ++i) w.v[i] = E::put(h.rstd[i] * ((h.ga[i] * dz[i] - m1[i]) - xh[i] * m2[i]));
-    st_pack<E, V>(dx + (long long)r * p.C, w);
+    for (int i = 0; i < V; ++i) o.v[i] = E::put(fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i])));
+    st_pack<E, V>(dx + (long long)r * p.C, o);
+  };
+  const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
+  int r = t.k * p.crows + piece * p.arows + rl;
+  for (; r + (U - 1) * RL < r1; r += U * RL) {
+    GnRow<E, V, Q8> w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = gn_load<E, V, Q8>(p, t.n, r + u * RL, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) write(r + u * RL, w[u]);
   }
+  for (; r < r1; r += RL) write(r, gn_load<E, V, Q8>(p, t.n, r, c));
 }
 
 // ---- host side
@@ -404,31 +463,43 @@ static bool gn_desc_ok(const tbg_gn_desc *d) {
   return d && d->N >= 1 && d->S >= 1 && d->C >= 1 && d->G >= 1 && d->C % d->G == 0 && dt_valid(d->dtype) && d->act >= TBG_ACT_LINEAR &&
          d->act <= TBG_ACT_SILU && (d->per_sample == 0 || d->per_sample == 1) && d->eps > 0.f && d->xs >= d->C && d->xn >= 0 && d->ds >= d->C && d->dn >= 0;
 }
-static int gn_geometry(const tbg_gn_desc *d, bool vec, GnP &p) {
+// Row ranges: the sums launch has at most 32 a tile (64 where the samples and tiles are few), each joined by every block of the second
+// launch that needs it; that launch cuts them into pieces for about 8 blocks a CU, of 8 rows a lane or more.
+static int gn_geometry(const tbg_gn_desc *d, bool vec, bool backward, GnP &p) {
   if (d->S > (1 << 30) || d->C > (1 << 24)) return TBG_ERANGE;
   const int V = vec ? 8 : 1;
   p.N = d->N; p.S = d->S; p.C = d->C; p.G = d->G; p.Cg = d->C / d->G; p.affn = d->per_sample ? d->C : 0;
   p.nb = (d->C + A8_BLOCK - 1) / A8_BLOCK;
   p.xn = d->xn; p.xs = d->xs; p.dn = d->dn; p.ds = d->ds; p.eps = d->eps;
-  const int padded = p.nb * A8_BLOCK, most = vec ? GN_CT : 64;
-  p.CT = padded < most ? padded : most;  // (a multiple of 32: a row's 8-bit block never spans two tiles)
+  // the tile (a power of two; a row's 8-bit block never spans two) that leaves the fewest lanes without channels
+  const int padded = p.nb * A8_BLOCK;
+  p.CT = 0;
+  for (int ct = vec ? GN_CT : 64, best = 0; ct >= 32; ct >>= 1) {
+    const int used = (int)(1000LL * padded / ((long long)(padded + ct - 1) / ct * ct));
+    if (used > best && (ct > 32 || padded == 32 || !p.CT)) { best = used; p.CT = ct; }
+  }
   p.ntile = (d->C + p.CT - 1) / p.CT;
   p.lanes = p.CT / V;
-  p.RL = GN_T / p.lanes;
   p.nslot = p.ntile + p.G - 1;
-  const auto ranges = [&](int target, int least, int &count, int &rows) {  // row ranges: about `target` blocks, `least` passes each
-    long long want = target / ((long long)p.N * p.ntile);
-    if (want < 1) want = 1;
-    const long long most_c = (p.S + (long long)p.RL * least - 1) / ((long long)p.RL * least);
-    if (want > most_c) want = most_c;
-    rows = (int)((p.S + want - 1) / want);
-    rows = (rows + p.RL - 1) / p.RL * p.RL;
-    count = (p.S + rows - 1) / rows;
-  };
-  ranges(1024, 4, p.nchunk, p.crows);
-  ranges(2048, 4, p.achunk, p.arows);
+  const int RL = (backward ? GN_TB : GN_TS) / p.lanes, RA = GN_T / p.lanes;
+  const long long tiles = (long long)p.N * p.ntile;
+  long long want = 512 / tiles;
+  const long long cap = tiles < 8 ? 64 : 32, most = (p.S + 4LL * RL - 1) / (4LL * RL);
+  want = want > cap ? cap : want;
+  want = want > most ? most : want;
+  if (want >= 8) want &= ~7LL;
+  if (want < 1) want = 1;
+  long long rows = (p.S + want - 1) / want;
+  p.crows = (int)((rows + RL - 1) / RL * RL);
+  p.nchunk = (int)((p.S + p.crows - 1LL) / p.crows);
+  long long split = 2048 / (tiles * p.nchunk);
+  const long long least = p.crows / (8LL * RA);
+  split = split > least ? least : split;
+  if (split < 1) split = 1;
+  p.arows = (int)(((p.crows + split - 1) / split + RA - 1) / RA * RA);
+  p.split = (p.crows + p.arows - 1) / p.arows;
   const long long count = d->per_sample ? (long long)d->N * d->C : d->C;
-  if ((long long)p.N * p.ntile * p.achunk > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
+  if (tiles * p.nchunk * p.split > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
   p.pblocks = (int)((count + GN_T / 8 - 1) / (GN_T / 8));
   return TBG_OK;
 }
@@ -440,7 +511,7 @@ extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int ba
   long long most = 0;
   for (int vec = 0; vec < 2; ++vec) {
     GnP p{};
-    if (const int rc = gn_geometry(d, vec != 0, p)) return rc;
+    if (const int rc = gn_geometry(d, vec != 0, backward != 0, p)) return rc;
     const long long b = gn_part_bytes(p) + (backward ? gn_pch_bytes(p) : 0);
     if (b > most) most = b;
   }
@@ -449,17 +520,21 @@ extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int ba
 
 template <class E, int V, int ACT>
 static int gn_run_fwd(const GnP &p, hipStream_t st) {
-  hipLaunchKernelGGL((gn_sums_kernel<E, V>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_T), 0, st, p);
+  const auto sums = V == 1 || p.Cg % 8 == 0 ? gn_sums_kernel<E, V, 1>
+                    : p.Cg % 4 == 0 ? gn_sums_kernel<E, V, V == 8 ? 2 : 1>
+                    : p.Cg % 2 == 0 ? gn_sums_kernel<E, V, V == 8 ? 4 : 1> : gn_sums_kernel<E, V, V>;
+  hipLaunchKernelGGL(sums, dim3(p.nn * p.ntile * p.nchunk), dim3(GN_TS), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((gn_apply_kernel<E, V, ACT>), dim3(p.N * p.ntile * p.achunk), dim3(GN_T), 0, st, p);
+  const auto apply = p.q || p.yq ? gn_apply_kernel<E, V, ACT, true> : gn_apply_kernel<E, V, ACT, false>;
+  hipLaunchKernelGGL(apply, dim3(p.nn * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
 template <class E, int V, int ACT, bool Q8>
 static int gn_run_bwd(const GnP &p, hipStream_t st) {
-  hipLaunchKernelGGL((gn_bwd_sums_kernel<E, V, ACT, Q8>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_T), 0, st, p);
+  hipLaunchKernelGGL((gn_bwd_sums_kernel<E, V, ACT, Q8>), dim3(p.nn * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, V, ACT, Q8>), dim3(p.pblocks + p.N * p.ntile * p.achunk), dim3(GN_T), 0, st, p);
+  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, V, ACT, Q8>), dim3(p.pblocks + p.nn * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
@@ -478,7 +553,9 @@ static int gn_run_type(const GnP &p, bool vec, int act, bool backward, hipStream
          : act == TBG_ACT_LRELU ? gn_run<E, 1, TBG_ACT_LRELU>(p, backward, st)
                                 : gn_run<E, 1, TBG_ACT_SILU>(p, backward, st);
 }
-static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool vec, bool backward, void *stream) {
+static int gn_dispatch(const tbg_gn_desc *d, GnP &p, bool vec, bool backward, void *stream) {
+  p.n0 = 0;
+  p.nn = p.N;
   hipStream_t st = tbg_stream(stream);
   return d->dtype == TBG_DT_F32 ? gn_run_type<ElF32>(p, vec, d->act, backward, st)
          : d->dtype == TBG_DT_BF16 ? gn_run_type<ElBf16>(p, vec, d->act, backward, st)
@@ -490,10 +567,10 @@ extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const flo
                                   void *q, void *e, void *yq, void *ye, void *workspace, long long workspace_bytes, void *stream) {
   if (!gn_desc_ok(d) || !x || !gamma || !beta || !y || !workspace || (q == nullptr) != (e == nullptr) || (yq == nullptr) != (ye == nullptr))
     return TBG_EINVAL;
-  if (gn_misaligned(q, yq) || gn_misaligned(workspace, nullptr)) return TBG_EINVAL;
+  if (gn_misaligned(q, yq) || gn_misaligned(workspace, stats)) return TBG_EINVAL;
   const bool vec = d->C % 8 == 0 && vec8_ok(x, d->dtype, d->xs, d->xn) && vec8_ok(y, d->dtype, d->C);
   GnP p{};
-  if (const int rc = gn_geometry(d, vec, p)) return rc;
+  if (const int rc = gn_geometry(d, vec, false, p)) return rc;
   if (gn_part_bytes(p) > workspace_bytes) return TBG_EINVAL;
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = y; p.stats = stats; p.part = reinterpret_cast<double *>(workspace);
   p.q = reinterpret_cast<unsigned char *>(q); p.e = reinterpret_cast<unsigned char *>(e);
@@ -507,10 +584,10 @@ extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const voi
   if (!gn_desc_ok(d) || !dy || !gamma || !beta || !stats || !dx || !dgamma || !dbeta || !workspace || (q == nullptr) != (e == nullptr) ||
       (x == nullptr) == (q == nullptr))
     return TBG_EINVAL;
-  if (gn_misaligned(q, workspace)) return TBG_EINVAL;
+  if (gn_misaligned(q, workspace) || gn_misaligned(stats, nullptr)) return TBG_EINVAL;
   const bool vec = d->C % 8 == 0 && (!x || vec8_ok(x, d->dtype, d->xs, d->xn)) && vec8_ok(dy, d->dtype, d->ds, d->dn) && vec8_ok(dx, d->dtype, d->C);
   GnP p{};
-  if (const int rc = gn_geometry(d, vec, p)) return rc;
+  if (const int rc = gn_geometry(d, vec, true, p)) return rc;
   if (gn_part_bytes(p) + gn_pch_bytes(p) > workspace_bytes) return TBG_EINVAL;
   p.x = x; p.dy = dy; p.gamma = gamma; p.beta = beta; p.y = dx; p.stats = const_cast<double *>(stats);
   p.q = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(q));

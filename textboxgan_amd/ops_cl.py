@@ -45,8 +45,11 @@ class Act8(NamedTuple):
         return self.q.numel() + self.e.numel()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 class _on:
-    """Run launches on the device of ``t`` (the current one as a rule: then nothing is switched)."""
+    """Run launches on the device of ``t`` (the current one as a rule: then nothing is switched), on its current stream."""
     __slots__ = ("prev", "idx")
 
     def __init__(self, t: torch.Tensor):
@@ -57,7 +60,7 @@ class _on:
         if cur != self.idx:
             self.prev = cur
             torch.cuda.set_device(self.idx)
-        return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(self.idx)
 
     def __exit__(self, *exc):
         if self.prev is not None:
