@@ -67,6 +67,24 @@ __device__ __forceinline__ void st_pack(typename E::type *p, const Pack<E, V> &r
   }
 }
 
+// V values rounded to the type, two conversions an instruction where the type has one
+template <class E, int V>
+__device__ __forceinline__ Pack<E, V> put_pack(const float (&v)[V]) {
+  Pack<E, V> r;
+  if constexpr (V == 8 && __is_same(E, ElBf16)) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, bf16x2));
+    __builtin_memcpy(&r, w, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = E::put(v[i]);
+  }
+  return r;
+}
+
 // ---- ACT8.  The lanes that hold one block of 32 channels are neighbours: 4 lanes of 8 channels or 32 lanes of one.
 constexpr int A8_BLOCK = 32;
 constexpr unsigned A8_NAN = 255u;
@@ -93,28 +111,35 @@ __device__ __forceinline__ unsigned a8_code(unsigned amax_bits) {
   const int e = (int)((amax_bits + 0x10000u) >> 23) - 6;
   return (unsigned)min(max(e, 1), 248);
 }
-// x in steps of its block's scale, rounded to the nearest integer (ties to even) within +-127, as floats.  x 2^-e is exact.  The clamp
-// matters for code 248 only, whose block may hold values up to 128 2^121.
+// x in steps of its block's scale, rounded to the nearest integer (ties to even) within +-127, as 1.5 2^23 + that integer: x 2^-e is exact, so
+// the one rounding is that of the sum, and the low byte of the result is the integer in two's complement.  Only a block of code 248 may hold
+// values beyond 127.5 steps (up to 128).  Values of a block that is not finite are of no account (a8_store writes zeros).
+constexpr float A8_MAGIC = 12582912.f;
 template <int V>
 __device__ __forceinline__ void a8_round(const float (&x)[V], unsigned code, float (&t)[V]) {
-  const float inv = code == A8_NAN ? 0.f : __uint_as_float((254u - code) << 23);
+  const float inv = __uint_as_float((254u - code) << 23);
 #pragma unroll
-  for (int i = 0; i < V; ++i) t[i] = code == A8_NAN ? 0.f : rintf(fminf(fmaxf(x[i] * inv, -127.f), 127.f));
+  for (int i = 0; i < V; ++i) t[i] = fmaf(x[i], inv, A8_MAGIC);
+  if (code == 248u) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = fminf(fmaxf(t[i], A8_MAGIC - 127.f), A8_MAGIC + 127.f);
+  }
 }
 __device__ __forceinline__ float a8_scale(unsigned code) { return __uint_as_float(code == A8_NAN ? 0x7fc00000u : code << 23); }
-// whole numbers within +-127 -> bytes: adding 1.5 2^23 leaves them in the low byte in two's complement
+// what a8_round has left -> bytes
 template <int V>
-__device__ __forceinline__ void a8_store(unsigned char *q, const float (&t)[V]) {
-  unsigned b[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) b[i] = __float_as_uint(t[i] + 12582912.f) & 0xffu;
+__device__ __forceinline__ void a8_store(unsigned char *q, unsigned code, const float (&t)[V]) {
   if constexpr (V == 8) {
     u32x2 w;
-    w[0] = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-    w[1] = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 1]), __float_as_uint(t[4 * k]), 0x0c0c0400u);
+      const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 3]), __float_as_uint(t[4 * k + 2]), 0x04000c0cu);
+      w[k] = code == A8_NAN ? 0u : lo | hi;
+    }
     *reinterpret_cast<u32x2 *>(q) = w;
   } else {
-    *q = (unsigned char)b[0];
+    *q = code == A8_NAN ? 0 : (unsigned char)(__float_as_uint(t[0]) & 0xffu);
   }
 }
 template <int V>

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const typename E::type *
   const unsigned code = a8_code(a8_block_max<V>(v));
   float t[V];
   a8_round<V>(v, code, t);
-  a8_store<V>(q + row * ((long long)cols * V) + c, t);
+  a8_store<V>(q + row * ((long long)cols * V) + c, code, t);
   if ((c & (A8_BLOCK - 1)) == 0) e[row * (cols * V / A8_BLOCK) + c / A8_BLOCK] = (unsigned char)code;
 }
 
@@ -44,10 +44,7 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(const unsigned char *_
   if (row >= rows) return;
   float v[V];
   a8_load<V>(q + row * pitch + c, a8_scale(e[row * (pitch / A8_BLOCK) + c / A8_BLOCK]), v);
-  Pack<E, V> p;
-#pragma unroll
-  for (int i = 0; i < V; ++i) p.v[i] = E::put(v[i]);
-  st_pack<E, V>(x + row * ldx + c, p);
+  st_pack<E, V>(x + row * ldx + c, put_pack<E, V>(v));
 }
 
 static int act8_args(const void *x, const void *q, const void *e, int dtype, long long rows, int ch, long long ldx) {

@@ -83,59 +83,86 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(A8wP p) {
   constexpr int XR = 256 / (TK / 8), DR = 256 / (TN / 8);  // rows between a lane's pieces
   const int xrow = tid / (TK / 8), xc = (tid % (TK / 8)) * 8, drow = tid / (TN / 8), dc = (tid % (TN / 8)) * 8;
   const bool xin = k0 + xc < p.pitch, din = n0 + dc < p.cout;
+  const int epitch = p.pitch / A8_BLOCK;
   const unsigned char *qp = p.q + (r0 + xrow) * p.pitch + k0 + xc;
-  const unsigned char *ep = p.e + (r0 + xrow) * (p.pitch / A8_BLOCK) + (k0 + xc) / A8_BLOCK;
+  const unsigned char *ep = p.e + (r0 + xrow) * epitch + (k0 + xc) / A8_BLOCK;
   const typename E::type *dp = reinterpret_cast<const typename E::type *>(p.dy) + (r0 + drow) * p.ldy + n0 + dc;
   u32x2 xq[WM];
   unsigned xe[WM];
   Pack<E, 8> dv[WN];
-  auto fetch = [&](long long r) {  // stage of rows r .. r + 31; rows and columns that do not exist are zeros
 #pragma unroll
-    for (int i = 0; i < WM; ++i) {
-      xq[i] = u32x2{0, 0};
-      xe[i] = 0;
-      if (xin && r + xrow + XR * i < rend) {
-        xq[i] = *reinterpret_cast<const u32x2 *>(qp + (r - r0 + XR * i) * p.pitch);
-        xe[i] = ep[(r - r0 + XR * i) * (p.pitch / A8_BLOCK)];
-      }
+  for (int i = 0; i < WM; ++i) { xq[i] = u32x2{0, 0}; xe[i] = 0; }
+#pragma unroll
+  for (int i = 0; i < WN; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dv[i].v[j] = 0;
+  auto fetch_dy = [&](Pack<E, 8> &v, const typename E::type *src) {
+    if constexpr (VEC) {
+      if (din) v = ld_pack<E, 8>(src);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n0 + dc + j < p.cout) v.v[j] = src[j];
     }
+  };
+  auto fetch = [&](long long r) {  // the next stage, rows r .. r + 31; rows and columns that do not exist are zeros
+    if (r + A8W_RB <= rend) {
+      if (xin) {
 #pragma unroll
-    for (int i = 0; i < WN; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dv[i].v[j] = 0;
-      if (r + drow + DR * i < rend) {
-        const typename E::type *src = dp + (r - r0 + DR * i) * p.ldy;
-        if constexpr (VEC) {
-          if (din) dv[i] = ld_pack<E, 8>(src);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (n0 + dc + j < p.cout) dv[i].v[j] = src[j];
+        for (int i = 0; i < WM; ++i) {
+          xq[i] = *reinterpret_cast<const u32x2 *>(qp + XR * i * p.pitch);
+          xe[i] = ep[XR * i * epitch];
         }
       }
+#pragma unroll
+      for (int i = 0; i < WN; ++i) fetch_dy(dv[i], dp + DR * i * p.ldy);
+    } else {
+#pragma unroll
+      for (int i = 0; i < WM; ++i) {
+        xq[i] = u32x2{0, 0};
+        xe[i] = 0;
+        if (xin && r + xrow + XR * i < rend) {
+          xq[i] = *reinterpret_cast<const u32x2 *>(qp + XR * i * p.pitch);
+          xe[i] = ep[XR * i * epitch];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < WN; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dv[i].v[j] = 0;
+        if (r + drow + DR * i < rend) fetch_dy(dv[i], dp + DR * i * p.ldy);
+      }
     }
+    qp += A8W_RB * p.pitch;
+    ep += A8W_RB * epitch;
+    dp += A8W_RB * p.ldy;
   };
   auto stage = [&](unsigned short *buf) {
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
       const float s = a8_scale(xe[i]);
-      Pack<ElBf16, 8> w;
+      float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w.v[j] = ElBf16::put((float)(int)(signed char)(xq[i][j >> 2] >> (8 * (j & 3)) & 0xff) * s);
-      st_pack<ElBf16, 8>(buf + (xrow + XR * i) * PK + xc, w);
+      for (int j = 0; j < 8; ++j) v[j] = (float)(int)(signed char)(xq[i][j >> 2] >> (8 * (j & 3)) & 0xff) * s;
+      st_pack<ElBf16, 8>(buf + (xrow + XR * i) * PK + xc, put_pack<ElBf16, 8>(v));
     }
 #pragma unroll
     for (int i = 0; i < WN; ++i) {
       Pack<ElBf16, 8> w[NP];
+      if constexpr (NP == 1) {
+        __builtin_memcpy(&w[0], &dv[i], 16);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = E::get(dv[i].v[j]);
-        unsigned short t[NP];
-        if constexpr (NP == 1) t[0] = dv[i].v[j];
-        else a8w_terms<NP>(v, t);
+        for (int j = 0; j < 8; ++j) {
+          unsigned short t[NP];
+          a8w_terms<NP>(E::get(dv[i].v[j]), t);
 #pragma unroll
-        for (int m = 0; m < NP; ++m) w[m].v[j] = t[m];
-        dbs[j] += v;
+          for (int m = 0; m < NP; ++m) w[m].v[j] = t[m];
+        }
+      }
+      if (do_db) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dbs[j] += E::get(dv[i].v[j]);
       }
 #pragma unroll
       for (int m = 0; m < NP; ++m) st_pack<ElBf16, 8>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
@@ -193,25 +220,31 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(A8wP p) {
   }
 }
 
-// dw = coef sum of the splits' products, db = sum of theirs; V neighbouring entries a lane
+// dw = coef sum of the splits' products, db = sum of theirs.  A lane takes V neighbouring entries; the 4 waves of a block every fourth split of
+// the same entries each, joined through LDS: the loads are what there is to wait for, and small products have few entries.
 template <int V>
 __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, const float *dbws, float *dw, float *db, long long kn, int cout,
                                                               int nsplit, float coef) {
-  long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V;
+  typedef float vec __attribute__((ext_vector_type(V)));
+  __shared__ vec red[256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  long long i = ((long long)blockIdx.x * 64 + lane) * V;
   const bool bias = i >= kn;
   if (bias) i -= kn;
-  if (bias && (!db || i >= cout)) return;
+  const bool live = !bias || (db && i < cout);
   const long long len = bias ? cout : kn;
   const float *src = (bias ? dbws : ws) + i;
-  float *dst = (bias ? db : dw) + i;
-  const float f = bias ? 1.f : coef;
-  typedef float vec __attribute__((ext_vector_type(V)));
   vec a;
 #pragma unroll
   for (int j = 0; j < V; ++j) a[j] = 0.f;
-#pragma unroll 16
-  for (int z = 0; z < nsplit; ++z) a += *reinterpret_cast<const vec *>(src + z * len);
-  *reinterpret_cast<vec *>(dst) = f * a;
+  if (live) {
+#pragma unroll 8
+    for (int z = wave; z < nsplit; z += 4) a += *reinterpret_cast<const vec *>(src + z * len);
+  }
+  red[threadIdx.x] = a;
+  __syncthreads();
+  if (wave == 0 && live)
+    *reinterpret_cast<vec *>((bias ? db : dw) + i) = (bias ? 1.f : coef) * ((red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]));
 }
 
 struct A8wGeo {
@@ -294,7 +327,7 @@ extern "C" int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int 
   if (rc || g.nsplit == 1) return rc;
   const bool v4 = cout % 4 == 0 && ((reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(db)) & 15) == 0;
   const long long lanes = (kn + (db ? cout : 0) + (v4 ? 3 : 0)) / (v4 ? 4 : 1);
-  hipLaunchKernelGGL(v4 ? act8_wgrad_join_kernel<4> : act8_wgrad_join_kernel<1>, dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, ws,
+  hipLaunchKernelGGL(v4 ? act8_wgrad_join_kernel<4> : act8_wgrad_join_kernel<1>, dim3((unsigned)((lanes + 63) / 64)), dim3(256), 0, st, ws,
                      ws + g.nsplit * kn, dw, db, kn, cout, g.nsplit, coef);
   TBG_LAUNCH_CHECK();
   return TBG_OK;

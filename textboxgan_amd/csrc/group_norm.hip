@@ -9,9 +9,11 @@
 // leaves partial sums per (sample, row range, tile, group), the second launch joins those of its groups in a fixed order (no atomics) and
 // writes the result.
 //
-// The statistics are 64-bit sums of x and x^2 (fp64 adds run at half the fp32 rate here, far from the bound of a streaming pass): one pass,
-// and mean(x^2) - mean^2 loses nothing that matters even for |mean| = 10^5 standard deviations.  The mean is used as fp32 + its remainder.
+// The statistics are 64-bit sums of x and x^2: one pass, and mean(x^2) - mean^2 loses nothing that matters for fp32 values of
+// |mean| = 10^5 standard deviations, nor for 16-bit ones, which do not resolve more than 2^11 of them.  The mean is used as fp32 + its remainder.
 #include "act8.h"
+
+#include <type_traits>
 
 struct GnP {
   const void *x, *dy;
@@ -25,7 +27,6 @@ struct GnP {
   float *dgamma, *dbeta;
   long long xn, xs, dn, ds;            // sample / row pitches of x and dy in elements (y, dx: contiguous)
   int N, S, C, G, Cg, affn, nb;        // affn: affine parameters' sample pitch (0 or C); nb: 8-bit blocks a row
-  int n0, nn;                          // samples of this launch
   int CT, ntile, lanes;                // channels a tile (a power of two), tiles, lanes a row
   int nchunk, crows, nslot;            // row ranges of the sums launch
   int split, arows;                    // the second launch's part of a row range: `split` pieces of arows rows
@@ -33,6 +34,9 @@ struct GnP {
   float eps;
 };
 
+#ifndef GN_BLOCKS
+#define GN_BLOCKS 2048
+#endif
 constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_CT = 128;  // threads a block: second launches, forward sums, backward sums; most channels a tile
 
 template <int ACT>
@@ -45,12 +49,21 @@ __device__ __forceinline__ float gn_act(float z) {
 template <int ACT>
 __device__ __forceinline__ float gn_dact(float dy, float z, bool positive) {
   if constexpr (ACT == TBG_ACT_LRELU) return dy * (positive ? 1.41421356237309515f : 0.282842712474619f);
-  if constexpr (ACT == TBG_ACT_SILU) {  // s + z s (1 - s)
-    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z)), u = z * s;
-    return dy * (fmaf(-u, s, u) + s);
+  if constexpr (ACT == TBG_ACT_SILU) {  // z comes times -log2(e): s = 1 / (1 + e^-z), act' = s + z s (1 - s)
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)), u = z * s;
+    return dy * fmaf(fmaf(-u, s, u), -0.693147180559945309f, s);
   }
   return dy;
 }
+
+// group of channel c, and of the channels after it one by one
+struct GnGroup {
+  int g, left;
+  __device__ __forceinline__ GnGroup(int c, int Cg) : g(c / Cg), left(Cg - (c - c / Cg * Cg)) {}
+  __device__ __forceinline__ void next(int Cg) {
+    if (--left == 0) { ++g; left = Cg; }
+  }
+};
 
 // what a block of the sums launch works on: row range k of a tile of a sample.  Row ranges vary fastest in both launches and their count is
 // a multiple of 8 where there are that many: a row range then stays on one of the 8 XCDs, whose L2 still holds it for the second launch
@@ -61,7 +74,7 @@ __device__ __forceinline__ GnTile gn_tile(const GnP &p, int b) {
   GnTile t;
   t.k = b % p.nchunk; b /= p.nchunk;
   t.tile = b % p.ntile;
-  t.n = p.n0 + b / p.ntile;
+  t.n = b / p.ntile;
   t.c0 = t.tile * p.CT;
   t.ct = min(p.CT, p.C - t.c0);
   return t;
@@ -97,23 +110,51 @@ __global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
   for (int i = 0; i < A; ++i) s1[i] = s2[i] = 0.0;
   if (lane * V < t.ct) {
     const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + t.c0 + lane * V;
-    const auto add = [&](const Pack<E, V> &v) {
+    // 16-bit types: 8 values and 8 squares are added in fp32 before they are in fp64 (values of 8 or 11 bits within 13 or 10 binades: the
+    // first sum is exact, the second off by 2^-24 at most, random over the sums of a group)
+    constexpr bool PRE = E::BYTES == 2;
+    constexpr int B = PRE ? (A < U ? A : U) : 1;  // rows added up before
+    const auto add = [&](const Pack<E, V> *v, auto rows) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const double d = E::get(v.v[i]);
-        s1[i * A / V] += d;
-        s2[i * A / V] = fma(d, d, s2[i * A / V]);
+      for (int a = 0; a < A; ++a) {
+        if constexpr (PRE) {
+          float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+          for (int u = 0; u < rows.value; ++u)
+#pragma unroll
+            for (int i = a * V / A; i < (a + 1) * V / A; ++i) {
+              const float d = E::get(v[u].v[i]);
+              t1 += d;
+              t2 = fmaf(d, d, t2);
+            }
+          s1[a] += (double)t1;
+          s2[a] += (double)t2;
+        } else {
+#pragma unroll
+          for (int u = 0; u < rows.value; ++u)
+#pragma unroll
+            for (int i = a * V / A; i < (a + 1) * V / A; ++i) {
+              const double d = E::get(v[u].v[i]);
+              s1[a] += d;
+              s2[a] = fma(d, d, s2[a]);
+            }
+        }
       }
     };
     int r = t.k * p.crows + rl;
+    const typename E::type *xr = x + r * p.xs;
+    const long long step = RL * p.xs;
     for (; r + (U - 1) * RL < r1; r += U * RL) {
       Pack<E, V> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = ld_pack<E, V>(x + (r + u * RL) * p.xs);
+      for (int u = 0; u < U; ++u, xr += step) v[u] = ld_pack<E, V>(xr);
 #pragma unroll
-      for (int u = 0; u < U; ++u) add(v[u]);
+      for (int u = 0; u < U; u += B) add(v + u, std::integral_constant<int, B>());
     }
-    for (; r < r1; r += RL) add(ld_pack<E, V>(x + r * p.xs));
+    for (; r < r1; r += RL, xr += step) {
+      const Pack<E, V> v = ld_pack<E, V>(xr);
+      add(&v, std::integral_constant<int, 1>());
+    }
   }
   // rows of a wave by lane exchanges, the waves through LDS
   for (int off = p.lanes; off < 64; off <<= 1)
@@ -181,12 +222,13 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
   const bool in = lane * V < t.ct;     // the others of the last block write the checkpoints' padding
   float mu[V], sc[V], sh[V];
   double sc64[V], be64[V];  // LeakyReLU's kink in 64 bits, as the backward pass has it
+  GnGroup at(c, p.Cg);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < V; ++i, at.next(p.Cg)) {
     mu[i] = sc[i] = sh[i] = 0.f;
     sc64[i] = be64[i] = 0.0;
     if (in) {
-      const int g = (c + i) / p.Cg - g0;
+      const int g = at.g - g0;
       const double mean = st[g * 2], rstd = st[g * 2 + 1];
       const float ga = p.gamma[(long long)t.n * p.affn + c + i], be = p.beta[(long long)t.n * p.affn + c + i];
       mu[i] = (float)mean;
@@ -196,80 +238,77 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
       be64[i] = be;
     }
   }
-  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + c;
-  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + (long long)t.n * p.S * p.C + c;
-  const auto write = [&](int r, const Pack<E, V> &v) {
+  const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
+  int r = t.k * p.crows + piece * p.arows + rl;
+  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + r * p.xs + c;
+  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + ((long long)t.n * p.S + r) * p.C + c;
+  const long long xstep = RL * p.xs, ystep = (long long)RL * p.C;
+  const long long row0 = (long long)t.n * p.S;
+  const auto keep = [&](const float (&v)[V], unsigned char *q, unsigned char *e, long long row, bool kink) {
+    const unsigned code = a8_code(a8_block_max<V>(v));
+    float k[V];
+    a8_round<V>(v, code, k);
+    if (ACT == TBG_ACT_LRELU && kink) {  // one step back where rounding has crossed the kink: the backward pass takes the value's own slope
+      const float scale = a8_scale(code);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float kept = (k[i] - A8_MAGIC) * scale;
+        if ((fma((double)v[i], sc64[i], be64[i]) > 0.0) != (fma((double)kept, sc64[i], be64[i]) > 0.0))
+          k[i] = fminf(fmaxf(k[i] + (v[i] > kept ? 1.f : -1.f), A8_MAGIC - 127.f), A8_MAGIC + 127.f);
+      }
+    }
+    a8_store<V>(q + row * p.nb * A8_BLOCK + c, code, k);
+    if ((c & (A8_BLOCK - 1)) == 0) e[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
+  };
+  const auto write = [&](int row, const Pack<E, V> &v) {
     float d[V], o[V];
-    Pack<E, V> w;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       d[i] = E::get(v.v[i]) - mu[i];
-      w.v[i] = E::put(gn_act<ACT>(fmaf(d[i], sc[i], sh[i])));
-      o[i] = E::get(w.v[i]);
+      o[i] = gn_act<ACT>(fmaf(d[i], sc[i], sh[i]));
     }
-    if (!Q || in) st_pack<E, V>(y + (long long)r * p.C, w);
+    const Pack<E, V> w = put_pack<E, V>(o);
+    if (!Q || in) st_pack<E, V>(y, w);
+    y += ystep;
     if constexpr (Q) {
-      const long long row = (long long)t.n * p.S + r;
-      if (!in) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = o[i] = 0.f;
-      }
-      if (p.q) {
-        const unsigned code = a8_code(a8_block_max<V>(d));
-        float k[V];
-        a8_round<V>(d, code, k);
-        if constexpr (ACT == TBG_ACT_LRELU) {  // one step back where rounding has crossed the kink: the backward pass takes the value's own slope
-          const float scale = a8_scale(code);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float kept = k[i] * scale;
-            if ((fma((double)d[i], sc64[i], be64[i]) > 0.0) != (fma((double)kept, sc64[i], be64[i]) > 0.0))
-              k[i] = fminf(fmaxf(k[i] + (d[i] > kept ? 1.f : -1.f), -127.f), 127.f);
-          }
-        }
-        a8_store<V>(p.q + row * p.nb * A8_BLOCK + c, k);
-        if ((c & (A8_BLOCK - 1)) == 0) p.e[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
-      }
-      if (p.yq) {
-        const unsigned code = a8_code(a8_block_max<V>(o));
-        float k[V];
-        a8_round<V>(o, code, k);
-        a8_store<V>(p.yq + row * p.nb * A8_BLOCK + c, k);
-        if ((c & (A8_BLOCK - 1)) == 0) p.ye[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
-      }
+      for (int i = 0; i < V; ++i) o[i] = in ? E::get(w.v[i]) : 0.f;  // (beyond the channels x and mu are 0 already)
+      if (p.q) keep(d, p.q, p.e, row0 + row, true);
+      if (p.yq) keep(o, p.yq, p.ye, row0 + row, false);
     }
   };
   if (!Q && !in) return;
   const Pack<E, V> zero = {};
-  const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
-  int r = t.k * p.crows + piece * p.arows + rl;
   for (; r + (U - 1) * RL < r1; r += U * RL) {
     Pack<E, V> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = in ? ld_pack<E, V>(x + (r + u * RL) * p.xs) : zero;
+    for (int u = 0; u < U; ++u, x += xstep) v[u] = in ? ld_pack<E, V>(x) : zero;
 #pragma unroll
     for (int u = 0; u < U; ++u) write(r + u * RL, v[u]);
   }
-  for (; r < r1; r += RL) write(r, in ? ld_pack<E, V>(x + r * p.xs) : zero);
+  for (; r < r1; r += RL, x += xstep) write(r, in ? ld_pack<E, V>(x) : zero);
 }
 
 // ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd: a lane keeps z = sc d + be of its V channels
 template <int V>
 struct GnCh {
-  float mu[V], lo[V], sc[V], be[V];
-  double sc64[V];
+  float mu[V], lo[V], sc[V], za[V], zb[V];  // za, zb: the same times -log2(e), for the exponential
+  double sc64[V], be64[V];
 };
 template <int V, bool Q8>
 __device__ __forceinline__ void gn_channels(const GnP &p, int n, int c, GnCh<V> &h) {
+  GnGroup at(c, p.Cg);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const double2 s = *reinterpret_cast<const double2 *>(p.stats + ((long long)n * p.G + (c + i) / p.Cg) * 2);
+  for (int i = 0; i < V; ++i, at.next(p.Cg)) {
+    const double2 s = *reinterpret_cast<const double2 *>(p.stats + ((long long)n * p.G + at.g) * 2);
     const float ga = p.gamma[(long long)n * p.affn + c + i];
     h.mu[i] = Q8 ? 0.f : (float)s.x;
     h.lo[i] = Q8 ? 0.f : (float)(s.x - (double)(float)s.x);
     h.sc64[i] = s.y * (double)ga;
     h.sc[i] = (float)h.sc64[i];
-    h.be[i] = p.beta[(long long)n * p.affn + c + i];
+    h.be64[i] = p.beta[(long long)n * p.affn + c + i];
+    h.za[i] = (float)(-1.44269504088896341 * h.sc64[i]);
+    h.zb[i] = (float)(-1.44269504088896341 * h.be64[i]);
   }
 }
 // a row's operands as they lie in memory
@@ -279,20 +318,35 @@ struct GnRow {
   u32x2 q;
   unsigned e;
 };
+// where a lane stands, and a step of `rows` rows
 template <class E, int V, bool Q8>
-__device__ __forceinline__ GnRow<E, V, Q8> gn_load(const GnP &p, int n, int r, int c) {
-  GnRow<E, V, Q8> w;
-  if constexpr (Q8) {
+struct GnAt {
+  const typename E::type *x, *g;
+  const unsigned char *q, *e;
+  __device__ __forceinline__ GnAt(const GnP &p, int n, int r, int c) {
     const long long row = (long long)n * p.S + r;
-    w.e = p.e[row * p.nb + c / A8_BLOCK];
-    if constexpr (V == 8) w.q = *reinterpret_cast<const u32x2 *>(p.q + row * p.nb * A8_BLOCK + c);
-    else w.q[0] = p.q[row * p.nb * A8_BLOCK + c];
-  } else {
-    w.x = ld_pack<E, V>(reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + r * p.xs + c);
+    x = reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + r * p.xs + c;
+    g = reinterpret_cast<const typename E::type *>(p.dy) + n * p.dn + r * p.ds + c;
+    q = p.q + row * p.nb * A8_BLOCK + c;
+    e = p.e + row * p.nb + c / A8_BLOCK;
   }
-  w.g = ld_pack<E, V>(reinterpret_cast<const typename E::type *>(p.dy) + n * p.dn + r * p.ds + c);
-  return w;
-}
+  __device__ __forceinline__ GnRow<E, V, Q8> next(const GnP &p, int rows) {
+    GnRow<E, V, Q8> w;
+    if constexpr (Q8) {
+      w.e = *e;
+      if constexpr (V == 8) w.q = *reinterpret_cast<const u32x2 *>(q);
+      else w.q[0] = *q;
+      q += (long long)rows * p.nb * A8_BLOCK;
+      e += (long long)rows * p.nb;
+    } else {
+      w.x = ld_pack<E, V>(x);
+      x += rows * p.xs;
+    }
+    w.g = ld_pack<E, V>(g);
+    g += rows * p.ds;
+    return w;
+  }
+};
 // d and dz of a row
 template <class E, int V, int ACT, bool Q8>
 __device__ __forceinline__ void gn_row(const GnRow<E, V, Q8> &w, const GnCh<V> &h, float (&d)[V], float (&dz)[V]) {
@@ -301,8 +355,8 @@ __device__ __forceinline__ void gn_row(const GnRow<E, V, Q8> &w, const GnCh<V> &
   for (int i = 0; i < V; ++i) {
     if constexpr (Q8) d[i] = (float)(int)(signed char)(w.q[i >> 2] >> (8 * (i & 3)) & 0xff) * scale;
     else d[i] = (E::get(w.x.v[i]) - h.mu[i]) - h.lo[i];
-    const float z = ACT == TBG_ACT_SILU ? fmaf(d[i], h.sc[i], h.be[i]) : 0.f;
-    const bool pos = ACT == TBG_ACT_LRELU ? fma((double)d[i], h.sc64[i], (double)h.be[i]) > 0.0 : false;
+    const float z = ACT == TBG_ACT_SILU ? fmaf(d[i], h.za[i], h.zb[i]) : 0.f;
+    const bool pos = ACT == TBG_ACT_LRELU ? fma((double)d[i], h.sc64[i], h.be64[i]) > 0.0 : false;
     dz[i] = gn_dact<ACT>(E::get(w.g.v[i]), z, pos);
   }
 }
@@ -331,14 +385,15 @@ __global__ __launch_bounds__(GN_TB, V == 8 ? 4 : 8) void gn_bwd_sums_kernel(GnP 
       }
     };
     int r = t.k * p.crows + rl;
+    GnAt<E, V, Q8> at(p, t.n, r, c);
     for (; r + (U - 1) * RL < r1; r += U * RL) {
       GnRow<E, V, Q8> w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = gn_load<E, V, Q8>(p, t.n, r + u * RL, c);
+      for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
 #pragma unroll
       for (int u = 0; u < U; ++u) add(w[u]);
     }
-    for (; r < r1; r += RL) add(gn_load<E, V, Q8>(p, t.n, r, c));
+    for (; r < r1; r += RL) add(at.next(p, RL));
   }
   for (int off = p.lanes; off < 64; off <<= 1)
 #pragma unroll
@@ -380,7 +435,7 @@ __global__ __launch_bounds__(GN_TB, V == 8 ? 4 : 8) void gn_bwd_sums_kernel(GnP 
 template <class E, int V, int ACT, bool Q8>
 __global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) {
   constexpr int U = 2;
-  __shared__ double st[2 * GN_CT];  // means of gamma dz and gamma dz xh over the tile's groups
+  __shared__ double st[2 * GN_CT];  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh)
   int b = blockIdx.x;
   if (b < p.pblocks) {  // 8 lanes a channel: the row ranges (and samples, where the parameters are shared) in a fixed order
     const long long idx = (long long)b * (GN_T / 8) + threadIdx.x / 8;
@@ -418,8 +473,9 @@ __global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) 
     gn_join(p, t.n, g0 + i / sub, i % sub, sub, a, q);
     const double m = (double)p.S * p.Cg;
     if (i % sub == 0) {
-      st[(i / sub) * 2] = a / m;
-      st[(i / sub) * 2 + 1] = q / m;
+      const double rstd = p.stats[((long long)t.n * p.G + g0 + i / sub) * 2 + 1];
+      st[(i / sub) * 2] = rstd * (a / m);
+      st[(i / sub) * 2 + 1] = rstd * rstd * (q / m);
     }
   }
   __syncthreads();
@@ -428,33 +484,33 @@ __global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) 
   const int c = t.c0 + lane * V;
   GnCh<V> h;
   gn_channels<V, Q8>(p, t.n, c, h);
-  float m1[V], m2[V];  // dx = sc dz - m1 - d m2, m1 = rstd mean(gamma dz), m2 = rstd^2 mean(gamma dz xh)
+  float m1[V], m2[V];  // dx = sc dz - m1 - d m2
+  GnGroup cg(c, p.Cg);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int g = (c + i) / p.Cg - g0;
-    const double rstd = p.stats[((long long)t.n * p.G + g0 + g) * 2 + 1];
-    m1[i] = (float)(rstd * st[g * 2]);
-    m2[i] = (float)(rstd * rstd * st[g * 2 + 1]);
+  for (int i = 0; i < V; ++i, cg.next(p.Cg)) {
+    m1[i] = (float)st[(cg.g - g0) * 2];
+    m2[i] = (float)st[(cg.g - g0) * 2 + 1];
   }
-  typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + (long long)t.n * p.S * p.C + c;
-  const auto write = [&](int r, const GnRow<E, V, Q8> &w) {
-    float d[V], dz[V];
-    gn_row<E, V, ACT, Q8>(w, h, d, dz);
-    Pack<E, V> o;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o.v[i] = E::put(fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i])));
-    st_pack<E, V>(dx + (long long)r * p.C, o);
-  };
   const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
   int r = t.k * p.crows + piece * p.arows + rl;
+  GnAt<E, V, Q8> at(p, t.n, r, c);
+  typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + ((long long)t.n * p.S + r) * p.C + c;
+  const auto write = [&](const GnRow<E, V, Q8> &w) {
+    float d[V], dz[V];
+    gn_row<E, V, ACT, Q8>(w, h, d, dz);
+#pragma unroll
+    for (int i = 0; i < V; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
+    st_pack<E, V>(dx, put_pack<E, V>(dz));
+    dx += (long long)RL * p.C;
+  };
   for (; r + (U - 1) * RL < r1; r += U * RL) {
     GnRow<E, V, Q8> w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = gn_load<E, V, Q8>(p, t.n, r + u * RL, c);
+    for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
 #pragma unroll
-    for (int u = 0; u < U; ++u) write(r + u * RL, w[u]);
+    for (int u = 0; u < U; ++u) write(w[u]);
   }
-  for (; r < r1; r += RL) write(r, gn_load<E, V, Q8>(p, t.n, r, c));
+  for (; r < r1; r += RL) write(at.next(p, RL));
 }
 
 // ---- host side
@@ -492,7 +548,7 @@ static int gn_geometry(const tbg_gn_desc *d, bool vec, bool backward, GnP &p) {
   long long rows = (p.S + want - 1) / want;
   p.crows = (int)((rows + RL - 1) / RL * RL);
   p.nchunk = (int)((p.S + p.crows - 1LL) / p.crows);
-  long long split = 2048 / (tiles * p.nchunk);
+  long long split = GN_BLOCKS / (tiles * p.nchunk);
   const long long least = p.crows / (8LL * RA);
   split = split > least ? least : split;
   if (split < 1) split = 1;
@@ -523,18 +579,18 @@ static int gn_run_fwd(const GnP &p, hipStream_t st) {
   const auto sums = V == 1 || p.Cg % 8 == 0 ? gn_sums_kernel<E, V, 1>
                     : p.Cg % 4 == 0 ? gn_sums_kernel<E, V, V == 8 ? 2 : 1>
                     : p.Cg % 2 == 0 ? gn_sums_kernel<E, V, V == 8 ? 4 : 1> : gn_sums_kernel<E, V, V>;
-  hipLaunchKernelGGL(sums, dim3(p.nn * p.ntile * p.nchunk), dim3(GN_TS), 0, st, p);
-  TBG_LAUNCH_CHECK();
   const auto apply = p.q || p.yq ? gn_apply_kernel<E, V, ACT, true> : gn_apply_kernel<E, V, ACT, false>;
-  hipLaunchKernelGGL(apply, dim3(p.nn * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
+  hipLaunchKernelGGL(sums, dim3(p.N * p.ntile * p.nchunk), dim3(GN_TS), 0, st, p);
+  TBG_LAUNCH_CHECK();
+  hipLaunchKernelGGL(apply, dim3(p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
 template <class E, int V, int ACT, bool Q8>
 static int gn_run_bwd(const GnP &p, hipStream_t st) {
-  hipLaunchKernelGGL((gn_bwd_sums_kernel<E, V, ACT, Q8>), dim3(p.nn * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
+  hipLaunchKernelGGL((gn_bwd_sums_kernel<E, V, ACT, Q8>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, V, ACT, Q8>), dim3(p.pblocks + p.nn * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
+  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, V, ACT, Q8>), dim3(p.pblocks + p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
@@ -553,9 +609,7 @@ static int gn_run_type(const GnP &p, bool vec, int act, bool backward, hipStream
          : act == TBG_ACT_LRELU ? gn_run<E, 1, TBG_ACT_LRELU>(p, backward, st)
                                 : gn_run<E, 1, TBG_ACT_SILU>(p, backward, st);
 }
-static int gn_dispatch(const tbg_gn_desc *d, GnP &p, bool vec, bool backward, void *stream) {
-  p.n0 = 0;
-  p.nn = p.N;
+static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool vec, bool backward, void *stream) {
   hipStream_t st = tbg_stream(stream);
   return d->dtype == TBG_DT_F32 ? gn_run_type<ElF32>(p, vec, d->act, backward, st)
          : d->dtype == TBG_DT_BF16 ? gn_run_type<ElBf16>(p, vec, d->act, backward, st)
