@@ -33,7 +33,11 @@ struct ElF16 {
   }
 };
 
-// V consecutive elements of a row.  V = 8: 16-byte accesses (the caller has checked the alignment); V = 1: one element.
+// 16-byte accesses to elements of a row wherever the row begins: the card takes them at any address
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// V consecutive elements of a row.  V = 8: 16-byte accesses; V = 1: one element.
 template <class E, int V>
 struct Pack {
   typename E::type v[V];
@@ -42,10 +46,10 @@ template <class E, int V>
 __device__ __forceinline__ Pack<E, V> ld_pack(const typename E::type *p) {
   Pack<E, V> r;
   if constexpr (V == 8 && E::BYTES == 2) {
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+    const u32x4 w = *reinterpret_cast<const u32x4_any *>(p);
     __builtin_memcpy(&r, &w, 16);
   } else if constexpr (V == 8) {
-    const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+    const f32x4 a = reinterpret_cast<const f32x4_any *>(p)[0], b = reinterpret_cast<const f32x4_any *>(p)[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { r.v[i] = a[i]; r.v[4 + i] = b[i]; }
   } else {

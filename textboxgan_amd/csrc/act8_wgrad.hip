@@ -25,7 +25,7 @@ struct A8wP {
   int want_db;
 };
 
-constexpr int A8W_RB = 32, A8W_PAD = 16;  // rows a stage; elements between two LDS rows (4 rows x 32 B of one transposing read: 4 bank groups)
+constexpr int A8W_RB = 32, A8W_PAD = 32;  // rows a stage; elements between two LDS rows (the 4 rows x 64 B of two transposing reads: all 64 banks)
 
 // the bf16 terms of dy, largest first, by truncation: every remainder is exact and nothing overflows
 template <int NP>
@@ -40,15 +40,19 @@ __device__ __forceinline__ void a8w_terms(float v, unsigned short (&t)[NP]) {
   }
 }
 
-// One barrier a stage: the block multiplies stage t out of one LDS buffer, writes stage t + 1 (loaded into registers a stage ago) to the other
-// and issues the loads of stage t + 2, so a global load has a whole stage to land.  2 blocks a CU cover each other's waits.
-template <class E, int NP, int WM, int WN, bool VEC>
-__global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(A8wP p) {
-  constexpr int TK = 64 * WM, TN = 64 * WN, PK = TK + A8W_PAD, PN = TN + A8W_PAD;
+// KW x NW waves of WM x WN products of 32 x 32.  One barrier a stage: the block multiplies stage t out of one LDS buffer, writes stage t + 1,
+// which its registers hold, to the other, and issues the loads of stage t + 1 + DEPTH into the registers that this frees: a stage is 0.2 to
+// 0.5 us of matrix work, a load under way takes three times that.  Whole stages only; rows left over go through a stage of their own at the end.
+template <class E, int NP, int WM, int WN, int KW, int NW, int DEPTH, bool VEC>
+__global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
+  constexpr int T = 64 * KW * NW, TK = 32 * WM * KW, TN = 32 * WN * NW, PK = TK + A8W_PAD, PN = TN + A8W_PAD;
   constexpr int BUF = A8W_RB * (PK + NP * PN);  // elements of one buffer: the checkpoint's tile, then dy's terms
+  // a lane stages the same column of every stage: 8 channels of XN rows of the checkpoint, 8 columns of DN rows of dy
+  constexpr int XR = T / (TK / 8), DR = T / (TN / 8), XN = A8W_RB / XR, DN = A8W_RB / DR;
+  static_assert(XN * XR == A8W_RB && DN * DR == A8W_RB && XR * (TK / 8) == T && DR * (TN / 8) == T, "pieces of a stage");
   extern __shared__ __align__(16) char smem[];
   unsigned short *lds = reinterpret_cast<unsigned short *>(smem);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave & 1, wn = wave >> 1;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave % KW, wn = wave / KW;
   // 8 neighbouring splits x all tiles of a split: blocks go round the 8 XCDs, so the tiles that share a split's rows share an L2
   const int tiles = p.tk * p.tn;
   int b = blockIdx.x;
@@ -79,103 +83,79 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(A8wP p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) dbs[i] = 0.f;
 
-  // a lane stages the same column of every stage: 8 channels of WM rows of the checkpoint and 8 columns of WN rows of dy
-  constexpr int XR = 256 / (TK / 8), DR = 256 / (TN / 8);  // rows between a lane's pieces
-  const int xrow = tid / (TK / 8), xc = (tid % (TK / 8)) * 8, drow = tid / (TN / 8), dc = (tid % (TN / 8)) * 8;
-  const bool xin = k0 + xc < p.pitch, din = n0 + dc < p.cout;
-  const int epitch = p.pitch / A8_BLOCK;
-  const unsigned char *qp = p.q + (r0 + xrow) * p.pitch + k0 + xc;
-  const unsigned char *ep = p.e + (r0 + xrow) * epitch + (k0 + xc) / A8_BLOCK;
-  const typename E::type *dp = reinterpret_cast<const typename E::type *>(p.dy) + (r0 + drow) * p.ldy + n0 + dc;
-  u32x2 xq[WM];
-  unsigned xe[WM];
-  Pack<E, 8> dv[WN];
-#pragma unroll
-  for (int i = 0; i < WM; ++i) { xq[i] = u32x2{0, 0}; xe[i] = 0; }
-#pragma unroll
-  for (int i = 0; i < WN; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dv[i].v[j] = 0;
-  auto fetch_dy = [&](Pack<E, 8> &v, const typename E::type *src) {
-    if constexpr (VEC) {
-      if (din) v = ld_pack<E, 8>(src);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (n0 + dc + j < p.cout) v.v[j] = src[j];
-    }
+  struct Regs {
+    u32x2 xq[XN];
+    unsigned xe[XN];
+    Pack<E, 8> dv[DN];
   };
-  auto fetch = [&](long long r) {  // the next stage, rows r .. r + 31; rows and columns that do not exist are zeros
-    if (r + A8W_RB <= rend) {
-      if (xin) {
+  const int xrow = tid / (TK / 8), xc = (tid % (TK / 8)) * 8, drow = tid / (TN / 8), dc = (tid % (TN / 8)) * 8, epitch = p.pitch / A8_BLOCK;
+  // pieces beyond the last channel read one that exists (their products are not stored)
+  const int xat = min(k0 + xc, p.pitch - 8), dat = VEC ? min(n0 + dc, p.cout - 8) : min(n0 + dc, p.cout - 1);
+  const typename E::type *dy = reinterpret_cast<const typename E::type *>(p.dy);
+  const unsigned qoff = xrow * p.pitch + xat, eoff = xrow * epitch + xat / A8_BLOCK, doff = drow * (unsigned)p.ldy + dat;
+  auto fetch = [&](Regs &g, long long r) {  // a whole stage, rows r .. r + 31
+    const unsigned char *qp = p.q + r * p.pitch, *ep = p.e + r * epitch;
+    const typename E::type *dp = dy + r * p.ldy;
 #pragma unroll
-        for (int i = 0; i < WM; ++i) {
-          xq[i] = *reinterpret_cast<const u32x2 *>(qp + XR * i * p.pitch);
-          xe[i] = ep[XR * i * epitch];
-        }
-      }
+    for (int i = 0; i < XN; ++i) {
+      g.xq[i] = *reinterpret_cast<const u32x2 *>(qp + (size_t)XR * i * p.pitch + qoff);
+      g.xe[i] = (ep + (size_t)XR * i * epitch)[eoff];
+    }
 #pragma unroll
-      for (int i = 0; i < WN; ++i) fetch_dy(dv[i], dp + DR * i * p.ldy);
-    } else {
+    for (int i = 0; i < DN; ++i) g.dv[i] = ld_pack<E, 8>(dp + (size_t)DR * i * p.ldy + doff);
+  };
+  auto fetch_some = [&](Regs &g, long long r) {  // fewer rows, the others zero; dy by elements
 #pragma unroll
-      for (int i = 0; i < WM; ++i) {
-        xq[i] = u32x2{0, 0};
-        xe[i] = 0;
-        if (xin && r + xrow + XR * i < rend) {
-          xq[i] = *reinterpret_cast<const u32x2 *>(qp + XR * i * p.pitch);
-          xe[i] = ep[XR * i * epitch];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < WN; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dv[i].v[j] = 0;
-        if (r + drow + DR * i < rend) fetch_dy(dv[i], dp + DR * i * p.ldy);
+    for (int i = 0; i < XN; ++i) {
+      g.xq[i] = u32x2{0, 0};
+      g.xe[i] = 0;
+      if (r + xrow + XR * i < rend) {
+        g.xq[i] = *reinterpret_cast<const u32x2 *>(p.q + (r + XR * i) * p.pitch + qoff);
+        g.xe[i] = p.e[(r + XR * i) * epitch + eoff];
       }
     }
-    qp += A8W_RB * p.pitch;
-    ep += A8W_RB * epitch;
-    dp += A8W_RB * p.ldy;
-  };
-  auto stage = [&](unsigned short *buf) {
 #pragma unroll
-    for (int i = 0; i < WM; ++i) {
-      const float s = a8_scale(xe[i]);
+    for (int i = 0; i < DN; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g.dv[i].v[j] = 0;
+        if (r + drow + DR * i < rend && n0 + dc + j < p.cout) g.dv[i].v[j] = dy[(r + drow + DR * i) * p.ldy + n0 + dc + j];
+      }
+  };
+  auto stage = [&](unsigned short *buf, const Regs &g) {
+#pragma unroll
+    for (int i = 0; i < XN; ++i) {
+      const float s = a8_scale(g.xe[i]);
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (float)(int)(signed char)(xq[i][j >> 2] >> (8 * (j & 3)) & 0xff) * s;
+      for (int j = 0; j < 8; ++j) v[j] = (float)(int)(signed char)(g.xq[i][j >> 2] >> (8 * (j & 3)) & 0xff) * s;
       st_pack<ElBf16, 8>(buf + (xrow + XR * i) * PK + xc, put_pack<ElBf16, 8>(v));
     }
 #pragma unroll
-    for (int i = 0; i < WN; ++i) {
+    for (int i = 0; i < DN; ++i) {
       Pack<ElBf16, 8> w[NP];
       if constexpr (NP == 1) {
-        __builtin_memcpy(&w[0], &dv[i], 16);
+        __builtin_memcpy(&w[0], &g.dv[i], 16);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           unsigned short t[NP];
-          a8w_terms<NP>(E::get(dv[i].v[j]), t);
+          a8w_terms<NP>(E::get(g.dv[i].v[j]), t);
 #pragma unroll
           for (int m = 0; m < NP; ++m) w[m].v[j] = t[m];
         }
       }
-      if (do_db) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dbs[j] += E::get(dv[i].v[j]);
-      }
 #pragma unroll
       for (int m = 0; m < NP; ++m) st_pack<ElBf16, 8>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
     }
+    if (do_db) {
+#pragma unroll
+      for (int i = 0; i < DN; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dbs[j] += E::get(g.dv[i].v[j]);
+    }
   };
-
-  fetch(r0);
-  stage(lds);
-  fetch(r0 + A8W_RB);
-  __syncthreads();
-  int cur = 0;
-  for (long long r = r0; r < rend; r += A8W_RB) {
-    const unsigned short *buf = lds + cur * BUF;
+  auto multiply = [&](const unsigned short *buf) {
 #pragma unroll
     for (int s = 0; s < A8W_RB / 16; ++s) {
       bf16x8 a[WM];
@@ -190,31 +170,68 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_kernel(A8wP p) {
           for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], d, acc[i][j], 0, 0, 0);
         }
     }
-    cur ^= 1;
-    stage(lds + cur * BUF);
-    fetch(r + 2 * A8W_RB);
+  };
+
+  // whole stages.  Where the columns are not a multiple of 8, a load of 8 may pass a row's end by 7: the last rows, whose loads would pass the
+  // tensor's end, are left to the masked stages
+  const long long margin = VEC ? 0 : (6 + p.ldy) / p.ldy;
+  const int full = (int)max((min(rend, p.rows - margin) - r0) / A8W_RB, 0LL);
+  unsigned short *cur = lds, *other = lds + BUF;
+  if (full > 0) {
+    Regs g[DEPTH];
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) fetch(g[u], r0 + (long long)min(u, full - 1) * A8W_RB);
+    stage(cur, g[0]);
+    fetch(g[0], r0 + (long long)min(DEPTH, full - 1) * A8W_RB);
+    __syncthreads();
+    for (int t = 0; t < full; t += DEPTH) {
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        if (t + u < full) {
+          multiply(cur);
+          if (t + u + 1 < full) stage(other, g[(u + 1) % DEPTH]);
+          fetch(g[(u + 1) % DEPTH], r0 + (long long)min(t + u + 1 + DEPTH, full - 1) * A8W_RB);
+          __syncthreads();
+          unsigned short *x = cur; cur = other; other = x;
+        }
+      }
+    }
+  }
+  for (long long r = r0 + (long long)full * A8W_RB; r < rend; r += A8W_RB) {  // (nobody reads this buffer any more: the barriers above, below)
+    Regs g;
+    fetch_some(g, r);
+    stage(cur, g);
+    __syncthreads();
+    multiply(cur);
     __syncthreads();
   }
 
   float *out = p.out + (long long)z * p.cin * p.cout;
   const float f = p.nsplit == 1 ? p.coef : 1.f;
+  const bool whole = k0 + TK <= p.cin && n0 + TN <= p.cout;
+  const int kl = k0 + wk * 32 * WM + 4 * (lane >> 5), nl = n0 + wn * 32 * WN + (lane & 31);
 #pragma unroll
   for (int i = 0; i < WM; ++i)
 #pragma unroll
-    for (int j = 0; j < WN; ++j)
+    for (int j = 0; j < WN; ++j) {
+      float *o = out + (long long)(kl + 32 * i) * p.cout + nl + 32 * j;
+      if (whole) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int k = k0 + wk * 32 * WM + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n = n0 + wn * 32 * WN + 32 * j + (lane & 31);
-        if (k < p.cin && n < p.cout) out[(long long)k * p.cout + n] = f * acc[i][j][r];
+        for (int r = 0; r < 16; ++r) o[(8 * (r >> 2) + (r & 3)) * (long long)p.cout] = f * acc[i][j][r];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kl + 32 * i + 8 * (r >> 2) + (r & 3) < p.cin && nl + 32 * j < p.cout) o[(8 * (r >> 2) + (r & 3)) * (long long)p.cout] = f * acc[i][j][r];
       }
+    }
   if (do_db) {
-    float *red = reinterpret_cast<float *>(smem);  // [256][8]; every wave is past its last operand read
+    float *red = reinterpret_cast<float *>(smem);  // [T][8]; every wave is past its last operand read
 #pragma unroll
     for (int j = 0; j < 8; ++j) red[tid * 8 + j] = dbs[j];
     __syncthreads();
     if (tid < TN && n0 + tid < p.cout) {
       float a = 0.f;
-      for (int l = 0; l < 256 / (TN / 8); ++l) a += red[(l * (TN / 8) + tid / 8) * 8 + (tid & 7)];
+      for (int l = 0; l < DR; ++l) a += red[(l * (TN / 8) + tid / 8) * 8 + (tid & 7)];
       p.dbout[(long long)z * p.cout + n0 + tid] = a;
     }
   }
@@ -247,26 +264,27 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, c
     *reinterpret_cast<vec *>((bias ? db : dw) + i) = (bias ? 1.f : coef) * ((red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]));
 }
 
+// Tile and row splits.  The tile: the largest that the channels fill (fewer re-reads of both operands, fewer operand reads an MFMA), made
+// smaller while the launch would have less than a block a CU with splits of 256 rows; the splits then fill the card once.
 struct A8wGeo {
-  int wm, wn, tk, tn, nsplit;
+  int form, tk, tn, nsplit;
   long long rsplit;
 };
-// Tile 64 wm x 64 wn and row splits: the largest tile that the channels fill (fewer re-reads of both operands and fewer operand reads an
-// MFMA), made smaller while the launch has less than a block a CU; splits of 128 rows or more, for 2 blocks a CU.
+struct A8wForm {
+  int tk, tn, per_cu;
+};
+static constexpr A8wForm A8W_FORMS[] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 2}, {64, 128, 2}, {64, 64, 4}};
 static A8wGeo a8w_geometry(long long rows, int cin, int cout, int dtype) {
   A8wGeo g;
-  g.wm = cin > 64 ? 2 : 1;
-  g.wn = cout > 128 && dtype == TBG_DT_BF16 ? 4 : cout > 64 ? 2 : 1;
-  const long long most = (rows + 4 * A8W_RB - 1) / (4 * A8W_RB);
-  for (;;) {
-    g.tk = (cin + 64 * g.wm - 1) / (64 * g.wm);
-    g.tn = (cout + 64 * g.wn - 1) / (64 * g.wn);
-    if ((long long)g.tk * g.tn * most >= 256 || (g.wm == 1 && g.wn == 1)) break;
-    if (g.wn > g.wm || g.wm == 1) g.wn >>= 1;
-    else g.wm >>= 1;
+  const long long most = (rows + 8 * A8W_RB - 1) / (8 * A8W_RB);
+  for (g.form = cin > 128 && cout > 128 && dtype == TBG_DT_BF16 ? 0 : cin > 64 ? (cout > 64 ? 1 : 2) : (cout > 64 ? 3 : 4);; g.form = g.form == 0 ? 1 : 4) {
+    g.tk = (cin + A8W_FORMS[g.form].tk - 1) / A8W_FORMS[g.form].tk;
+    g.tn = (cout + A8W_FORMS[g.form].tn - 1) / A8W_FORMS[g.form].tn;
+    if ((long long)g.tk * g.tn * most >= 256 || g.form == 4) break;
   }
-  long long want = 512 / ((long long)g.tk * g.tn);
-  if (want > most) want = most;
+  long long want = 256LL * A8W_FORMS[g.form].per_cu / ((long long)g.tk * g.tn);
+  const long long cap = g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
+  if (want > cap) want = cap;
   if (want < 1) want = 1;
   g.rsplit = ((rows + want - 1) / want + A8W_RB - 1) / A8W_RB * A8W_RB;
   g.nsplit = (int)((rows + g.rsplit - 1) / g.rsplit);
@@ -285,29 +303,35 @@ extern "C" long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int
   return g.nsplit == 1 ? 0 : (long long)g.nsplit * ((long long)cin * cout + cout) * (long long)sizeof(float);
 }
 
-template <class E, int NP, int WM, int WN>
+template <class E, int NP, int WM, int WN, int KW, int NW, int DEPTH>
 static int a8w_launch(const A8wP &p, bool vec, hipStream_t st) {
-  constexpr size_t lds = 2 * (size_t)A8W_RB * (64 * WM + A8W_PAD + NP * (64 * WN + A8W_PAD)) * 2;
+  constexpr size_t lds = 2 * (size_t)A8W_RB * (32 * WM * KW + A8W_PAD + NP * (32 * WN * NW + A8W_PAD)) * 2;
   const unsigned blocks = (unsigned)((p.nsplit + 7) / 8 * 8 * p.tk * p.tn);
-  const auto kern = vec ? act8_wgrad_kernel<E, NP, WM, WN, true> : act8_wgrad_kernel<E, NP, WM, WN, false>;
+  const auto kern = vec ? act8_wgrad_kernel<E, NP, WM, WN, KW, NW, DEPTH, true> : act8_wgrad_kernel<E, NP, WM, WN, KW, NW, DEPTH, false>;
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return TBG_EHIP;
-  hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(kern, dim3(blocks), dim3(64 * KW * NW), lds, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
 template <class E, int NP>
 static int a8w_tiles(const A8wP &p, const A8wGeo &g, bool vec, hipStream_t st) {
-  if constexpr (NP == 1)
-    if (g.wn == 4) return g.wm == 2 ? a8w_launch<E, NP, 2, 4>(p, vec, st) : a8w_launch<E, NP, 1, 4>(p, vec, st);
-  if (g.wm == 2) return g.wn == 2 ? a8w_launch<E, NP, 2, 2>(p, vec, st) : a8w_launch<E, NP, 2, 1>(p, vec, st);
-  return g.wn == 2 ? a8w_launch<E, NP, 1, 2>(p, vec, st) : a8w_launch<E, NP, 1, 1>(p, vec, st);
+  switch (g.form) {
+    case 0:
+      if constexpr (NP == 1) return a8w_launch<E, NP, 4, 2, 2, 4, 2>(p, vec, st);
+      return TBG_EINVAL;
+    case 1: return a8w_launch<E, NP, 2, 2, 2, 2, 2>(p, vec, st);
+    case 2: return a8w_launch<E, NP, 2, 1, 2, 2, 2>(p, vec, st);
+    case 3: return a8w_launch<E, NP, 1, 2, 2, 2, 2>(p, vec, st);
+    default: return a8w_launch<E, NP, 1, 1, 2, 2, 2>(p, vec, st);
+  }
 }
 
 extern "C" int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int dtype, long long rows, int cin, int cout, long long ldy,
                               float coef, float *dw, float *db, void *workspace, long long workspace_bytes, void *stream) {
   if (!q || !e || !dy || !dw || ldy < cout || (reinterpret_cast<uintptr_t>(q) & 15) != 0) return TBG_EINVAL;
   if (const int rc = a8w_args(rows, cin, cout, dtype)) return rc;
+  if (ldy > (1LL << 26)) return TBG_ERANGE;
   const A8wGeo g = a8w_geometry(rows, cin, cout, dtype);
   if ((long long)(g.nsplit + 7) * g.tk * g.tn > 0x7fffffffLL) return TBG_ERANGE;
   const long long kn = (long long)cin * cout, need = g.nsplit == 1 ? 0 : g.nsplit * (kn + cout) * (long long)sizeof(float);
@@ -319,7 +343,7 @@ extern "C" int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int 
   float *ws = reinterpret_cast<float *>(workspace);
   p.out = g.nsplit == 1 ? dw : ws;
   p.dbout = g.nsplit == 1 ? db : ws + g.nsplit * kn;
-  const bool vec = cout % 8 == 0 && vec8_ok(dy, dtype, ldy);
+  const bool vec = cout % 8 == 0;
   hipStream_t st = tbg_stream(stream);
   const int rc = dtype == TBG_DT_F32 ? a8w_tiles<ElF32, 3>(p, g, vec, st)
                  : dtype == TBG_DT_BF16 ? a8w_tiles<ElBf16, 1>(p, g, vec, st)
