@@ -10,6 +10,8 @@
 // launch in a fixed order.
 #include "act8.h"
 
+#include <type_traits>
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -40,10 +42,10 @@ __device__ __forceinline__ void a8w_terms(float v, unsigned short (&t)[NP]) {
   }
 }
 
-// KW x NW waves of WM x WN products of 32 x 32.  One barrier a stage: the block multiplies stage t out of one LDS buffer, writes stage t + 1,
-// which its registers hold, to the other, and issues the loads of stage t + 1 + DEPTH into the registers that this frees: a stage is 0.2 to
-// 0.5 us of matrix work, a load under way takes three times that.  Whole stages only; rows left over go through a stage of their own at the end.
-template <class E, int NP, int WM, int WN, int KW, int NW, int DEPTH, bool VEC>
+// KW x NW waves of WM x WN products of 32 x 32.  Three LDS buffers and one barrier a stage: while the block multiplies stage t it writes stage
+// t + 2, which its registers hold, and reads the first operands of stage t + 1, so that the matrix pipe has work right behind the barrier; the
+// loads of stage t + 4 go into the registers that this frees.  Whole stages only; rows left over go through stages of their own at the end.
+template <class E, int NP, int WM, int WN, int KW, int NW, bool VEC>
 __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
   constexpr int T = 64 * KW * NW, TK = 32 * WM * KW, TN = 32 * WN * NW, PK = TK + A8W_PAD, PN = TN + A8W_PAD;
   constexpr int BUF = A8W_RB * (PK + NP * PN);  // elements of one buffer: the checkpoint's tile, then dy's terms
@@ -148,61 +150,87 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
 #pragma unroll
       for (int m = 0; m < NP; ++m) st_pack<ElBf16, 8>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
     }
-    if (do_db) {
-#pragma unroll
-      for (int i = 0; i < DN; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dbs[j] += E::get(g.dv[i].v[j]);
-    }
   };
-  auto multiply = [&](const unsigned short *buf) {
+  auto column_sums = [&](const Regs &g) {
 #pragma unroll
-    for (int s = 0; s < A8W_RB / 16; ++s) {
-      bf16x8 a[WM];
+    for (int i = 0; i < DN; ++i)
 #pragma unroll
-      for (int i = 0; i < WM; ++i) a[i] = rd(buf + a_off + 16 * s * PK + 32 * i, PK);
-#pragma unroll
-      for (int j = 0; j < WN; ++j)
-#pragma unroll
-        for (int m = NP - 1; m >= 0; --m) {  // smallest terms first
-          const bf16x8 d = rd(buf + b_off + (m * A8W_RB + 16 * s) * PN + 32 * j, PN);
-#pragma unroll
-          for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], d, acc[i][j], 0, 0, 0);
-        }
-    }
+      for (int j = 0; j < 8; ++j) dbs[j] += E::get(g.dv[i].v[j]);
   };
-
+  struct Ops {  // 16 rows' operands
+    bf16x8 a[WM], d[WN][NP];
+  };
+  auto operands = [&](const unsigned short *buf, int s) {
+    Ops o;
+#pragma unroll
+    for (int i = 0; i < WM; ++i) o.a[i] = rd(buf + a_off + 16 * s * PK + 32 * i, PK);
+#pragma unroll
+    for (int j = 0; j < WN; ++j)
+#pragma unroll
+      for (int m = 0; m < NP; ++m) o.d[j][m] = rd(buf + b_off + (m * A8W_RB + 16 * s) * PN + 32 * j, PN);
+    return o;
+  };
+  auto multiply = [&](const Ops &o) {
+#pragma unroll
+    for (int j = 0; j < WN; ++j)
+#pragma unroll
+      for (int m = NP - 1; m >= 0; --m)  // smallest terms first
+#pragma unroll
+        for (int i = 0; i < WM; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.a[i], o.d[j][m], acc[i][j], 0, 0, 0);
+  };
   // whole stages.  Where the columns are not a multiple of 8, a load of 8 may pass a row's end by 7: the last rows, whose loads would pass the
   // tensor's end, are left to the masked stages
   const long long margin = VEC ? 0 : (6 + p.ldy) / p.ldy;
   const int full = (int)max((min(rend, p.rows - margin) - r0) / A8W_RB, 0LL);
-  unsigned short *cur = lds, *other = lds + BUF;
-  if (full > 0) {
-    Regs g[DEPTH];
+  unsigned short *cur = lds, *next = lds + BUF, *last = lds + 2 * BUF;
+  auto whole_stages = [&](auto sums) {
+    Regs g[2];
+    const auto load = [&](Regs &to, int t) { fetch(to, r0 + (long long)min(t, full - 1) * A8W_RB); };  // (behind the last stage: that one again)
+    const auto put = [&](unsigned short *buf, const Regs &from, bool counts) {
+      stage(buf, from);
+      if (sums.value) {  // branch-free, as the whole loop body is
 #pragma unroll
-    for (int u = 0; u < DEPTH; ++u) fetch(g[u], r0 + (long long)min(u, full - 1) * A8W_RB);
-    stage(cur, g[0]);
-    fetch(g[0], r0 + (long long)min(DEPTH, full - 1) * A8W_RB);
+        for (int i = 0; i < DN; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dbs[j] += counts ? E::get(from.dv[i].v[j]) : 0.f;
+      }
+    };
+    load(g[0], 0);
+    load(g[1], 1);
+    put(cur, g[0], true);
+    load(g[0], 2);
+    put(next, g[1], 1 < full);
+    load(g[1], 3);
     __syncthreads();
-    for (int t = 0; t < full; t += DEPTH) {
+    Ops lo = operands(cur, 0);
+    for (int t = 0; t < full; t += 2) {
 #pragma unroll
-      for (int u = 0; u < DEPTH; ++u) {
+      for (int u = 0; u < 2; ++u) {
         if (t + u < full) {
-          multiply(cur);
-          if (t + u + 1 < full) stage(other, g[(u + 1) % DEPTH]);
-          fetch(g[(u + 1) % DEPTH], r0 + (long long)min(t + u + 1 + DEPTH, full - 1) * A8W_RB);
+          const Ops hi = operands(cur, 1);
+          multiply(lo);
+          lo = operands(next, 0);
+          put(last, g[u], t + u + 2 < full);
+          load(g[u], t + u + 4);
+          multiply(hi);
           __syncthreads();
-          unsigned short *x = cur; cur = other; other = x;
+          unsigned short *x = cur; cur = next; next = last; last = x;
         }
       }
     }
+  };
+  if (full > 0) {
+    if (do_db) whole_stages(std::true_type());
+    else whole_stages(std::false_type());
   }
   for (long long r = r0 + (long long)full * A8W_RB; r < rend; r += A8W_RB) {  // (nobody reads this buffer any more: the barriers above, below)
     Regs g;
     fetch_some(g, r);
     stage(cur, g);
+    if (do_db) column_sums(g);
     __syncthreads();
-    multiply(cur);
+    multiply(operands(cur, 0));
+    multiply(operands(cur, 1));
     __syncthreads();
   }
 
@@ -303,11 +331,11 @@ extern "C" long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int
   return g.nsplit == 1 ? 0 : (long long)g.nsplit * ((long long)cin * cout + cout) * (long long)sizeof(float);
 }
 
-template <class E, int NP, int WM, int WN, int KW, int NW, int DEPTH>
+template <class E, int NP, int WM, int WN, int KW, int NW>
 static int a8w_launch(const A8wP &p, bool vec, hipStream_t st) {
-  constexpr size_t lds = 2 * (size_t)A8W_RB * (32 * WM * KW + A8W_PAD + NP * (32 * WN * NW + A8W_PAD)) * 2;
+  constexpr size_t lds = 3 * (size_t)A8W_RB * (32 * WM * KW + A8W_PAD + NP * (32 * WN * NW + A8W_PAD)) * 2;
   const unsigned blocks = (unsigned)((p.nsplit + 7) / 8 * 8 * p.tk * p.tn);
-  const auto kern = vec ? act8_wgrad_kernel<E, NP, WM, WN, KW, NW, DEPTH, true> : act8_wgrad_kernel<E, NP, WM, WN, KW, NW, DEPTH, false>;
+  const auto kern = vec ? act8_wgrad_kernel<E, NP, WM, WN, KW, NW, true> : act8_wgrad_kernel<E, NP, WM, WN, KW, NW, false>;
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return TBG_EHIP;
   hipLaunchKernelGGL(kern, dim3(blocks), dim3(64 * KW * NW), lds, st, p);
@@ -318,12 +346,12 @@ template <class E, int NP>
 static int a8w_tiles(const A8wP &p, const A8wGeo &g, bool vec, hipStream_t st) {
   switch (g.form) {
     case 0:
-      if constexpr (NP == 1) return a8w_launch<E, NP, 4, 2, 2, 4, 2>(p, vec, st);
+      if constexpr (NP == 1) return a8w_launch<E, NP, 4, 2, 2, 4>(p, vec, st);
       return TBG_EINVAL;
-    case 1: return a8w_launch<E, NP, 2, 2, 2, 2, 2>(p, vec, st);
-    case 2: return a8w_launch<E, NP, 2, 1, 2, 2, 2>(p, vec, st);
-    case 3: return a8w_launch<E, NP, 1, 2, 2, 2, 2>(p, vec, st);
-    default: return a8w_launch<E, NP, 1, 1, 2, 2, 2>(p, vec, st);
+    case 1: return a8w_launch<E, NP, 2, 2, 2, 2>(p, vec, st);
+    case 2: return a8w_launch<E, NP, 2, 1, 2, 2>(p, vec, st);
+    case 3: return a8w_launch<E, NP, 1, 2, 2, 2>(p, vec, st);
+    default: return a8w_launch<E, NP, 1, 1, 2, 2>(p, vec, st);
   }
 }
 
