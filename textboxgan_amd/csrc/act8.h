@@ -33,49 +33,108 @@ struct ElF16 {
   }
 };
 
-// 16-byte accesses to elements of a row wherever the row begins: the card takes them at any address
+// 8 neighbouring channels of a row, moved in 16-byte pieces wherever the row begins: the card takes them at any address
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
-// V consecutive elements of a row.  V = 8: 16-byte accesses; V = 1: one element.
-template <class E, int V>
-struct Pack {
-  typename E::type v[V];
+template <class E>
+struct Pack8 {
+  typename E::type v[8];
 };
-template <class E, int V>
-__device__ __forceinline__ Pack<E, V> ld_pack(const typename E::type *p) {
-  Pack<E, V> r;
-  if constexpr (V == 8 && E::BYTES == 2) {
+template <class E>
+__device__ __forceinline__ Pack8<E> ld8(const typename E::type *p) {
+  Pack8<E> r;
+  if constexpr (E::BYTES == 2) {
     const u32x4 w = *reinterpret_cast<const u32x4_any *>(p);
     __builtin_memcpy(&r, &w, 16);
-  } else if constexpr (V == 8) {
+  } else {
     const f32x4 a = reinterpret_cast<const f32x4_any *>(p)[0], b = reinterpret_cast<const f32x4_any *>(p)[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { r.v[i] = a[i]; r.v[4 + i] = b[i]; }
-  } else {
-    r.v[0] = *p;
   }
   return r;
 }
-template <class E, int V>
-__device__ __forceinline__ void st_pack(typename E::type *p, const Pack<E, V> &r) {
-  if constexpr (V == 8 && E::BYTES == 2) {
+template <class E>
+__device__ __forceinline__ void st8(typename E::type *p, const Pack8<E> &r) {
+  if constexpr (E::BYTES == 2) {
     u32x4 w;
     __builtin_memcpy(&w, &r, 16);
-    *reinterpret_cast<u32x4 *>(p) = w;
-  } else if constexpr (V == 8) {
-    reinterpret_cast<f32x4 *>(p)[0] = f32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
-    reinterpret_cast<f32x4 *>(p)[1] = f32x4{r.v[4], r.v[5], r.v[6], r.v[7]};
+    *reinterpret_cast<u32x4_any *>(p) = w;
   } else {
-    *p = r.v[0];
+    reinterpret_cast<f32x4_any *>(p)[0] = f32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
+    reinterpret_cast<f32x4_any *>(p)[1] = f32x4{r.v[4], r.v[5], r.v[6], r.v[7]};
   }
 }
+// moved down by k elements (k the same in all lanes), zeros above
+template <class E>
+__device__ __forceinline__ Pack8<E> shift_down(const Pack8<E> &r, int k) {
+  if constexpr (E::BYTES == 2) {
+    unsigned w[4];
+    __builtin_memcpy(w, &r, 16);
+    if (k & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = w[3] = 0; }
+    if (k & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = 0; }
+    if (k & 1) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) w[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], 16);
+      w[3] >>= 16;
+    }
+    Pack8<E> o;
+    __builtin_memcpy(&o, w, 16);
+    return o;
+  } else {
+    Pack8<E> o = r;
+#pragma unroll
+    for (int step = 4; step > 0; step >>= 1)
+      if (k & step) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.v[i] = i + step < 8 ? o.v[i + step] : (typename E::type)0;
+      }
+    return o;
+  }
+}
+// A lane's channels c .. c + 7 of rows of C.  TAIL (C % 8 != 0): the lane that holds the last C % 8 channels reads the row's last 8 and moves
+// them down, so that nothing beyond the row is touched; its other values are zeros and are not stored.  Rows of fewer than 8 go by elements.
+template <class E, bool TAIL>
+struct Row8 {
+  int off, left;  // where the lane reads; channels of the lane (8, fewer in the last one)
+  int C;
+  __device__ __forceinline__ Row8(int c, int C_) : off(c), left(8), C(C_) {
+    if (TAIL && c + 8 > C) {
+      left = C - c;
+      off = C >= 8 ? C - 8 : 0;
+    }
+  }
+  __device__ __forceinline__ Pack8<E> load(const typename E::type *row) const {
+    if constexpr (!TAIL) return ld8<E>(row + off);
+    Pack8<E> r;
+    if (C >= 8) {
+      r = ld8<E>(row + off);
+      const Pack8<E> low = shift_down(r, 8 - (C & 7));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = left < 8 ? low.v[i] : r.v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = i < C ? row[i] : (typename E::type)0;
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(typename E::type *row, const Pack8<E> &r) const {
+    if (!TAIL || left == 8) {
+      st8<E>(row + off, r);
+    } else {
+      typename E::type *to = row + (C & ~7);
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < (C & 7)) to[i] = r.v[i];
+    }
+  }
+};
 
-// V values rounded to the type, two conversions an instruction where the type has one
-template <class E, int V>
-__device__ __forceinline__ Pack<E, V> put_pack(const float (&v)[V]) {
-  Pack<E, V> r;
-  if constexpr (V == 8 && __is_same(E, ElBf16)) {
+// 8 values rounded to the type, two conversions an instruction where the type has one
+template <class E>
+__device__ __forceinline__ Pack8<E> put8(const float (&v)[8]) {
+  Pack8<E> r;
+  if constexpr (__is_same(E, ElBf16)) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     unsigned w[4];
@@ -84,28 +143,22 @@ __device__ __forceinline__ Pack<E, V> put_pack(const float (&v)[V]) {
     __builtin_memcpy(&r, w, 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = E::put(v[i]);
+    for (int i = 0; i < 8; ++i) r.v[i] = E::put(v[i]);
   }
   return r;
 }
 
-// ---- ACT8.  The lanes that hold one block of 32 channels are neighbours: 4 lanes of 8 channels or 32 lanes of one.
+// ---- ACT8.  A lane holds 8 channels of a block of 32, neighbouring lanes its other 24
 constexpr int A8_BLOCK = 32;
 constexpr unsigned A8_NAN = 255u;
 
 // largest bit pattern of |x| in the block.  Bit patterns of non-negative floats order like the floats, infinities and NaN on top.
-template <int V>
-__device__ __forceinline__ unsigned a8_block_max(const float (&x)[V]) {
+__device__ __forceinline__ unsigned a8_block_max(const float (&x)[8]) {
   unsigned m = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-  if constexpr (V == 8) {
-    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
-    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
-  } else {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
-  }
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
+  m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
   return m;
 }
 // scale code of a block: e + 127 with e = floor(log2 amax) - 6, one more where amax 2^-e would round to 128 (mantissa >= 127.5 / 64,
@@ -119,43 +172,29 @@ __device__ __forceinline__ unsigned a8_code(unsigned amax_bits) {
 // the one rounding is that of the sum, and the low byte of the result is the integer in two's complement.  Only a block of code 248 may hold
 // values beyond 127.5 steps (up to 128).  Values of a block that is not finite are of no account (a8_store writes zeros).
 constexpr float A8_MAGIC = 12582912.f;
-template <int V>
-__device__ __forceinline__ void a8_round(const float (&x)[V], unsigned code, float (&t)[V]) {
+__device__ __forceinline__ void a8_round(const float (&x)[8], unsigned code, float (&t)[8]) {
   const float inv = __uint_as_float((254u - code) << 23);
 #pragma unroll
-  for (int i = 0; i < V; ++i) t[i] = fmaf(x[i], inv, A8_MAGIC);
+  for (int i = 0; i < 8; ++i) t[i] = fmaf(x[i], inv, A8_MAGIC);
   if (code == 248u) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = fminf(fmaxf(t[i], A8_MAGIC - 127.f), A8_MAGIC + 127.f);
+    for (int i = 0; i < 8; ++i) t[i] = fminf(fmaxf(t[i], A8_MAGIC - 127.f), A8_MAGIC + 127.f);
   }
 }
 __device__ __forceinline__ float a8_scale(unsigned code) { return __uint_as_float(code == A8_NAN ? 0x7fc00000u : code << 23); }
 // what a8_round has left -> bytes
-template <int V>
-__device__ __forceinline__ void a8_store(unsigned char *q, unsigned code, const float (&t)[V]) {
-  if constexpr (V == 8) {
-    u32x2 w;
+__device__ __forceinline__ void a8_store(unsigned char *q, unsigned code, const float (&t)[8]) {
+  u32x2 w;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 1]), __float_as_uint(t[4 * k]), 0x0c0c0400u);
-      const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 3]), __float_as_uint(t[4 * k + 2]), 0x04000c0cu);
-      w[k] = code == A8_NAN ? 0u : lo | hi;
-    }
-    *reinterpret_cast<u32x2 *>(q) = w;
-  } else {
-    *q = code == A8_NAN ? 0 : (unsigned char)(__float_as_uint(t[0]) & 0xffu);
+  for (int k = 0; k < 2; ++k) {
+    const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 1]), __float_as_uint(t[4 * k]), 0x0c0c0400u);
+    const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 3]), __float_as_uint(t[4 * k + 2]), 0x04000c0cu);
+    w[k] = code == A8_NAN ? 0u : lo | hi;
   }
+  *reinterpret_cast<u32x2 *>(q) = w;
 }
-template <int V>
-__device__ __forceinline__ void a8_load(const unsigned char *q, float scale, float (&x)[V]) {
-  if constexpr (V == 8) {
-    const u32x2 w = *reinterpret_cast<const u32x2 *>(q);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)(int)(signed char)(w[i >> 2] >> (8 * (i & 3)) & 0xff) * scale;
-  } else {
-    x[0] = (float)(int)(signed char)*q * scale;
-  }
-}
+// one value of eight packed bytes, in steps
+__device__ __forceinline__ float a8_value(const u32x2 &w, int i) { return (float)(int)(signed char)(w[i >> 2] >> (8 * (i & 3)) & 0xff); }
 
 // ---- dispatch
 #define TBG_DT_F32 0
@@ -163,8 +202,3 @@ __device__ __forceinline__ void a8_load(const unsigned char *q, float scale, flo
 #define TBG_DT_F16 2
 static inline int dt_bytes(int dtype) { return dtype == TBG_DT_F32 ? 4 : 2; }
 static inline bool dt_valid(int dtype) { return dtype >= TBG_DT_F32 && dtype <= TBG_DT_F16; }
-// 16-byte accesses of 8 channels: base and row / sample pitches (elements) allow them
-static inline bool vec8_ok(const void *p, int dtype, long long pitch_a, long long pitch_b = 0) {
-  const long long unit = 16 / dt_bytes(dtype);
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch_a % unit == 0 && pitch_b % unit == 0;
-}

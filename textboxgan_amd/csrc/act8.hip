@@ -2,49 +2,52 @@
 //
 // HBM-bound both ways: es + 1 + 1/32 bytes an element.  A lane holds 8 channels of one row (16-byte loads, 8-byte stores of q), the four
 // lanes of a block find its largest magnitude with two DPP exchanges, so a value is touched once.  Items (row, group of 8 channels) are
-// laid end to end over the lanes whatever the row length, so that short and odd rows waste no lanes.
+// laid end to end over the lanes whatever the row length, so that short and odd rows waste no lanes, and rows that begin anywhere are read in
+// 16-byte pieces all the same.
 #include "act8.h"
 
-template <class E, int V>
+template <class E, bool TAIL>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const typename E::type *__restrict__ x, long long rows, int ch, long long ldx,
                                                         unsigned char *__restrict__ q, unsigned char *__restrict__ e, unsigned cols) {
-  // cols = V-channel groups of a padded row (a multiple of 32 / V)
+  // cols = 8-channel groups of a padded row (a multiple of 4)
   const long long base = (long long)blockIdx.x * 256;
   const long long row0 = base / cols;
   const unsigned local = (unsigned)(base - row0 * cols) + threadIdx.x;
   const long long row = row0 + local / cols;
-  const unsigned col = local % cols;
+  const int c = (int)(local % cols) * 8;
   if (row >= rows) return;  // whole blocks of 32 channels leave together: cols and 256 are multiples of a block's lanes
-  const int c = (int)col * V;
-  float v[V];
+  float v[8];
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = 0.f;
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
   if (c < ch) {
-    const Pack<E, V> p = ld_pack<E, V>(x + row * ldx + c);
+    const Pack8<E> p = Row8<E, TAIL>(c, ch).load(x + row * ldx);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = E::get(p.v[i]);
+    for (int i = 0; i < 8; ++i) v[i] = E::get(p.v[i]);
   }
-  const unsigned code = a8_code(a8_block_max<V>(v));
-  float t[V];
-  a8_round<V>(v, code, t);
-  a8_store<V>(q + row * ((long long)cols * V) + c, code, t);
-  if ((c & (A8_BLOCK - 1)) == 0) e[row * (cols * V / A8_BLOCK) + c / A8_BLOCK] = (unsigned char)code;
+  const unsigned code = a8_code(a8_block_max(v));
+  float t[8];
+  a8_round(v, code, t);
+  a8_store(q + row * ((long long)cols * 8) + c, code, t);
+  if ((c & (A8_BLOCK - 1)) == 0) e[row * (cols / 4) + c / A8_BLOCK] = (unsigned char)code;
 }
 
-template <class E, int V>
+template <class E, bool TAIL>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(const unsigned char *__restrict__ q, const unsigned char *__restrict__ e,
                                                           long long rows, int ch, typename E::type *__restrict__ x, long long ldx,
                                                           unsigned cols, unsigned pitch) {
-  // cols = V-channel groups of an unpadded row
+  // cols = 8-channel groups of an unpadded row
   const long long base = (long long)blockIdx.x * 256;
   const long long row0 = base / cols;
   const unsigned local = (unsigned)(base - row0 * cols) + threadIdx.x;
   const long long row = row0 + local / cols;
-  const int c = (int)(local % cols) * V;
+  const int c = (int)(local % cols) * 8;
   if (row >= rows) return;
-  float v[V];
-  a8_load<V>(q + row * pitch + c, a8_scale(e[row * (pitch / A8_BLOCK) + c / A8_BLOCK]), v);
-  st_pack<E, V>(x + row * ldx + c, put_pack<E, V>(v));
+  const u32x2 w = *reinterpret_cast<const u32x2 *>(q + row * pitch + c);
+  const float scale = a8_scale(e[row * (pitch / A8_BLOCK) + c / A8_BLOCK]);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = a8_value(w, i) * scale;
+  Row8<E, TAIL>(c, ch).store(x + row * ldx, put8<E>(v));
 }
 
 static int act8_args(const void *x, const void *q, const void *e, int dtype, long long rows, int ch, long long ldx) {
@@ -55,31 +58,29 @@ static int act8_args(const void *x, const void *q, const void *e, int dtype, lon
 }
 
 template <class E>
-static int launch_pack(const void *x, int dtype, long long rows, int ch, long long ldx, void *q, void *e, hipStream_t st) {
+static int launch_pack(const void *x, long long rows, int ch, long long ldx, void *q, void *e, hipStream_t st) {
   const unsigned padded = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK);
-  const bool vec = ch % 8 == 0 && vec8_ok(x, dtype, ldx);
-  const unsigned cols = vec ? padded / 8 : padded;
+  const unsigned cols = padded / 8;
   const long long blocks = (rows * cols + 255) / 256;
   if (rows > (1LL << 39) / padded || blocks > 0x7fffffffLL) return TBG_ERANGE;
   auto *xp = reinterpret_cast<const typename E::type *>(x);
   auto *qp = reinterpret_cast<unsigned char *>(q), *ep = reinterpret_cast<unsigned char *>(e);
-  if (vec) hipLaunchKernelGGL((act8_pack_kernel<E, 8>), dim3((unsigned)blocks), dim3(256), 0, st, xp, rows, ch, ldx, qp, ep, cols);
-  else hipLaunchKernelGGL((act8_pack_kernel<E, 1>), dim3((unsigned)blocks), dim3(256), 0, st, xp, rows, ch, ldx, qp, ep, cols);
+  hipLaunchKernelGGL((ch % 8 ? act8_pack_kernel<E, true> : act8_pack_kernel<E, false>), dim3((unsigned)blocks), dim3(256), 0, st, xp, rows, ch, ldx,
+                     qp, ep, cols);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
 
 template <class E>
-static int launch_unpack(const void *q, const void *e, int dtype, long long rows, int ch, void *x, long long ldx, hipStream_t st) {
+static int launch_unpack(const void *q, const void *e, long long rows, int ch, void *x, long long ldx, hipStream_t st) {
   const unsigned padded = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK);
-  const bool vec = ch % 8 == 0 && vec8_ok(x, dtype, ldx);
-  const unsigned cols = vec ? ch / 8 : ch;
+  const unsigned cols = (ch + 7) / 8;
   const long long blocks = (rows * cols + 255) / 256;
   if (rows > (1LL << 39) / padded || blocks > 0x7fffffffLL) return TBG_ERANGE;
   auto *xp = reinterpret_cast<typename E::type *>(x);
   auto *qp = reinterpret_cast<const unsigned char *>(q), *ep = reinterpret_cast<const unsigned char *>(e);
-  if (vec) hipLaunchKernelGGL((act8_unpack_kernel<E, 8>), dim3((unsigned)blocks), dim3(256), 0, st, qp, ep, rows, ch, xp, ldx, cols, padded);
-  else hipLaunchKernelGGL((act8_unpack_kernel<E, 1>), dim3((unsigned)blocks), dim3(256), 0, st, qp, ep, rows, ch, xp, ldx, cols, padded);
+  hipLaunchKernelGGL((ch % 8 ? act8_unpack_kernel<E, true> : act8_unpack_kernel<E, false>), dim3((unsigned)blocks), dim3(256), 0, st, qp, ep, rows,
+                     ch, xp, ldx, cols, padded);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
@@ -87,15 +88,15 @@ static int launch_unpack(const void *q, const void *e, int dtype, long long rows
 extern "C" int tbg_act8_pack(const void *x, int dtype, long long rows, int ch, long long ldx, void *q, void *e, void *stream) {
   if (const int rc = act8_args(x, q, e, dtype, rows, ch, ldx)) return rc;
   hipStream_t st = tbg_stream(stream);
-  return dtype == TBG_DT_F32 ? launch_pack<ElF32>(x, dtype, rows, ch, ldx, q, e, st)
-         : dtype == TBG_DT_BF16 ? launch_pack<ElBf16>(x, dtype, rows, ch, ldx, q, e, st)
-                                : launch_pack<ElF16>(x, dtype, rows, ch, ldx, q, e, st);
+  return dtype == TBG_DT_F32 ? launch_pack<ElF32>(x, rows, ch, ldx, q, e, st)
+         : dtype == TBG_DT_BF16 ? launch_pack<ElBf16>(x, rows, ch, ldx, q, e, st)
+                                : launch_pack<ElF16>(x, rows, ch, ldx, q, e, st);
 }
 
 extern "C" int tbg_act8_unpack(const void *q, const void *e, long long rows, int ch, void *x, int dtype, long long ldx, void *stream) {
   if (const int rc = act8_args(x, q, e, dtype, rows, ch, ldx)) return rc;
   hipStream_t st = tbg_stream(stream);
-  return dtype == TBG_DT_F32 ? launch_unpack<ElF32>(q, e, dtype, rows, ch, x, ldx, st)
-         : dtype == TBG_DT_BF16 ? launch_unpack<ElBf16>(q, e, dtype, rows, ch, x, ldx, st)
-                                : launch_unpack<ElF16>(q, e, dtype, rows, ch, x, ldx, st);
+  return dtype == TBG_DT_F32 ? launch_unpack<ElF32>(q, e, rows, ch, x, ldx, st)
+         : dtype == TBG_DT_BF16 ? launch_unpack<ElBf16>(q, e, rows, ch, x, ldx, st)
+                                : launch_unpack<ElF16>(q, e, rows, ch, x, ldx, st);
 }

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
   struct Regs {
     u32x2 xq[XN];
     unsigned xe[XN];
-    Pack<E, 8> dv[DN];
+    Pack8<E> dv[DN];
   };
   const int xrow = tid / (TK / 8), xc = (tid % (TK / 8)) * 8, drow = tid / (TN / 8), dc = (tid % (TN / 8)) * 8, epitch = p.pitch / A8_BLOCK;
   // pieces beyond the last channel read one that exists (their products are not stored)
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
       g.xe[i] = (ep + (size_t)XR * i * epitch)[eoff];
     }
 #pragma unroll
-    for (int i = 0; i < DN; ++i) g.dv[i] = ld_pack<E, 8>(dp + (size_t)DR * i * p.ldy + doff);
+    for (int i = 0; i < DN; ++i) g.dv[i] = ld8<E>(dp + (size_t)DR * i * p.ldy + doff);
   };
   auto fetch_some = [&](Regs &g, long long r) {  // fewer rows, the others zero; dy by elements
 #pragma unroll
@@ -130,12 +130,12 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
       const float s = a8_scale(g.xe[i]);
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (float)(int)(signed char)(g.xq[i][j >> 2] >> (8 * (j & 3)) & 0xff) * s;
-      st_pack<ElBf16, 8>(buf + (xrow + XR * i) * PK + xc, put_pack<ElBf16, 8>(v));
+      for (int j = 0; j < 8; ++j) v[j] = a8_value(g.xq[i], j) * s;
+      st8<ElBf16>(buf + (xrow + XR * i) * PK + xc, put8<ElBf16>(v));
     }
 #pragma unroll
     for (int i = 0; i < DN; ++i) {
-      Pack<ElBf16, 8> w[NP];
+      Pack8<ElBf16> w[NP];
       if constexpr (NP == 1) {
         __builtin_memcpy(&w[0], &g.dv[i], 16);
       } else {
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
         }
       }
 #pragma unroll
-      for (int m = 0; m < NP; ++m) st_pack<ElBf16, 8>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
+      for (int m = 0; m < NP; ++m) st8<ElBf16>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
     }
   };
   auto column_sums = [&](const Regs &g) {

@@ -4,7 +4,7 @@
 //   xh = (x - mean) rstd,  z = gamma xh + beta,  y = act(z)
 //   dz = dy act'(z),  dbeta = sum dz,  dgamma = sum dz xh,  dx = rstd (gamma dz - mean(gamma dz) - xh mean(gamma dz xh))
 //
-// HBM-bound.  A block works on a tile of CT channels (every lane has V fixed neighbouring ones) and a range of rows, so all accesses are
+// HBM-bound.  A block works on a tile of CT channels (every lane has 8 fixed neighbouring ones) and a range of rows, so all accesses are
 // whole 16-byte pieces of rows whatever the group width: groups need not line up with tiles.  Direction forward / backward: a sums launch
 // leaves partial sums per (sample, row range, tile, group), the second launch joins those of its groups in a fixed order (no atomics) and
 // writes the result.
@@ -12,8 +12,6 @@
 // The statistics are 64-bit sums of x and x^2: one pass, and mean(x^2) - mean^2 loses nothing that matters for fp32 values of
 // |mean| = 10^5 standard deviations, nor for 16-bit ones, which do not resolve more than 2^11 of them.  The mean is used as fp32 + its remainder.
 #include "act8.h"
-
-#include <type_traits>
 
 struct GnP {
   const void *x, *dy;
@@ -34,10 +32,14 @@ struct GnP {
   float eps;
 };
 
+#ifndef GN_NOWHOLE
+#define GN_NOWHOLE 0
+#endif
 #ifndef GN_BLOCKS
 #define GN_BLOCKS 2048
 #endif
-constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_CT = 128;  // threads a block: second launches, forward sums, backward sums; most channels a tile
+// threads a block: second launches, forward sums, backward sums, whole forward; most channels a tile; rows a lane of the whole forward keeps
+constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_TW = 512, GN_CT = 128, GN_R = 8;
 
 template <int ACT>
 __device__ __forceinline__ float gn_act(float z) {
@@ -45,10 +47,28 @@ __device__ __forceinline__ float gn_act(float z) {
   if constexpr (ACT == TBG_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
   return z;
 }
-// dy act'(z).  positive: LeakyReLU's side of the kink, decided in 64 bits so that it does not hang on the last bit of a 32-bit product
+// LeakyReLU's slope where z = scale d + be > 0, scale = sc + lo.  The side of the kink is decided as in 64 bits, so that it does not hang on the
+// last bit of a 32-bit product: that one, off by 2^-24 (|be| + 3 |z|) at most, says it unless |z| <= 2^-22 |be|.
+__device__ __forceinline__ void gn_slope(const float (&d)[8], const float (&sc)[8], const float (&lo)[8], const float (&be)[8], float (&f)[8]) {
+  bool close = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float z = fmaf(d[i], sc[i], be[i]);
+    close |= fabsf(z) * 4194304.f <= fabsf(be[i]);
+    f[i] = z > 0.f ? 1.41421356237309515f : 0.282842712474619f;
+  }
+  if (close) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float s = sc[i], l = lo[i], b = be[i];
+      asm volatile("" : "+v"(s), "+v"(l), "+v"(b));  // (their 64-bit forms are not worth keeping in registers over the rows)
+      f[i] = fma((double)d[i], (double)s + (double)l, (double)b) > 0.0 ? 1.41421356237309515f : 0.282842712474619f;
+    }
+  }
+}
+// dy act'(z), LeakyReLU apart
 template <int ACT>
-__device__ __forceinline__ float gn_dact(float dy, float z, bool positive) {
-  if constexpr (ACT == TBG_ACT_LRELU) return dy * (positive ? 1.41421356237309515f : 0.282842712474619f);
+__device__ __forceinline__ float gn_dact(float dy, float z) {
   if constexpr (ACT == TBG_ACT_SILU) {  // z comes times -log2(e): s = 1 / (1 + e^-z), act' = s + z s (1 - s)
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)), u = z * s;
     return dy * fmaf(fmaf(-u, s, u), -0.693147180559945309f, s);
@@ -56,14 +76,17 @@ __device__ __forceinline__ float gn_dact(float dy, float z, bool positive) {
   return dy;
 }
 
-// group of channel c, and of the channels after it one by one
-struct GnGroup {
-  int g, left;
-  __device__ __forceinline__ GnGroup(int c, int Cg) : g(c / Cg), left(Cg - (c - c / Cg * Cg)) {}
-  __device__ __forceinline__ void next(int Cg) {
-    if (--left == 0) { ++g; left = Cg; }
+// groups of a lane's 8 channels (of the last channel for those that do not exist)
+__device__ __forceinline__ void gn_groups(const GnP &p, int c, int (&g)[8]) {
+  int at = min(c, p.C - 1) / p.Cg, left = (at + 1) * p.Cg - c;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    g[i] = min(at, p.G - 1);
+    --left;
+    at += left <= 0;
+    left = left <= 0 ? p.Cg : left;
   }
-};
+}
 
 // what a block of the sums launch works on: row range k of a tile of a sample.  Row ranges vary fastest in both launches and their count is
 // a multiple of 8 where there are that many: a row range then stays on one of the 8 XCDs, whose L2 still holds it for the second launch
@@ -97,73 +120,48 @@ __device__ __forceinline__ void gn_join(const GnP &p, int n, int g, int lane, in
   }
 }
 
-// ---- forward, first launch: sums of x and x^2.  V / A neighbouring channels share a group (A accumulators a lane)
-template <class E, int V, int A>
-__global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
-  constexpr int U = 4, NW = GN_TS / 64;
-  __shared__ double red[NW * (GN_CT / V) * A * 2];
-  const GnTile t = gn_tile(p, blockIdx.x);
-  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TS / p.lanes;
-  const int r1 = min(p.S, (t.k + 1) * p.crows);
-  double s1[A], s2[A];
+// ---- forward: sums of x and x^2.  8 / A neighbouring channels share a group (A accumulators a lane).
+// 16-bit types: up to 8 values and squares are added in fp32 before they are in fp64 (values of 8 or 11 bits within 13 or 10 binades: the
+// first sum is exact; the second is off by 2^-24 at most, at random over the sums of a group)
+template <class E, int A, int ROWS>
+__device__ __forceinline__ void gn_add(const Pack8<E> *v, double (&s1)[A], double (&s2)[A]) {
 #pragma unroll
-  for (int i = 0; i < A; ++i) s1[i] = s2[i] = 0.0;
-  if (lane * V < t.ct) {
-    const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + t.c0 + lane * V;
-    // 16-bit types: 8 values and 8 squares are added in fp32 before they are in fp64 (values of 8 or 11 bits within 13 or 10 binades: the
-    // first sum is exact, the second off by 2^-24 at most, random over the sums of a group)
-    constexpr bool PRE = E::BYTES == 2;
-    constexpr int B = PRE ? (A < U ? A : U) : 1;  // rows added up before
-    const auto add = [&](const Pack<E, V> *v, auto rows) {
+  for (int a = 0; a < A; ++a) {
+    if constexpr (E::BYTES == 2) {
+      float t1 = 0.f, t2 = 0.f;
 #pragma unroll
-      for (int a = 0; a < A; ++a) {
-        if constexpr (PRE) {
-          float t1 = 0.f, t2 = 0.f;
+      for (int u = 0; u < ROWS; ++u)
 #pragma unroll
-          for (int u = 0; u < rows.value; ++u)
-#pragma unroll
-            for (int i = a * V / A; i < (a + 1) * V / A; ++i) {
-              const float d = E::get(v[u].v[i]);
-              t1 += d;
-              t2 = fmaf(d, d, t2);
-            }
-          s1[a] += (double)t1;
-          s2[a] += (double)t2;
-        } else {
-#pragma unroll
-          for (int u = 0; u < rows.value; ++u)
-#pragma unroll
-            for (int i = a * V / A; i < (a + 1) * V / A; ++i) {
-              const double d = E::get(v[u].v[i]);
-              s1[a] += d;
-              s2[a] = fma(d, d, s2[a]);
-            }
+        for (int i = a * 8 / A; i < (a + 1) * 8 / A; ++i) {
+          const float d = E::get(v[u].v[i]);
+          t1 += d;
+          t2 = fmaf(d, d, t2);
         }
-      }
-    };
-    int r = t.k * p.crows + rl;
-    const typename E::type *xr = x + r * p.xs;
-    const long long step = RL * p.xs;
-    for (; r + (U - 1) * RL < r1; r += U * RL) {
-      Pack<E, V> v[U];
+      s1[a] += (double)t1;
+      s2[a] += (double)t2;
+    } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u, xr += step) v[u] = ld_pack<E, V>(xr);
+      for (int u = 0; u < ROWS; ++u)
 #pragma unroll
-      for (int u = 0; u < U; u += B) add(v + u, std::integral_constant<int, B>());
-    }
-    for (; r < r1; r += RL, xr += step) {
-      const Pack<E, V> v = ld_pack<E, V>(xr);
-      add(&v, std::integral_constant<int, 1>());
+        for (int i = a * 8 / A; i < (a + 1) * 8 / A; ++i) {
+          const double d = E::get(v[u].v[i]);
+          s1[a] += d;
+          s2[a] = fma(d, d, s2[a]);
+        }
     }
   }
-  // rows of a wave by lane exchanges, the waves through LDS
+}
+// a block's sums of each 8 / A channels of the tile, in red[2 c], red[2 c + 1]: rows of a wave by lane exchanges, the waves through LDS
+template <int A, int T>
+__device__ __forceinline__ void gn_block_sums(const GnP &p, double (&s1)[A], double (&s2)[A], double *red) {
+  constexpr int NW = T / 64;
+  const int lane = threadIdx.x & (p.lanes - 1), wave = threadIdx.x >> 6, cols = p.lanes * A;
   for (int off = p.lanes; off < 64; off <<= 1)
 #pragma unroll
     for (int i = 0; i < A; ++i) {
       s1[i] += __shfl_xor(s1[i], off, 64);
       s2[i] += __shfl_xor(s2[i], off, 64);
     }
-  const int wave = threadIdx.x >> 6, cols = p.lanes * A;  // partial sums a wave: cols of (64 / lanes rows joined)
   if ((threadIdx.x & 63) < p.lanes)
 #pragma unroll
     for (int i = 0; i < A; ++i) {
@@ -178,216 +176,324 @@ __global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
     red[threadIdx.x] = a;
   }
   __syncthreads();
-  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg, step = V / A;
-  for (int g = g0 + threadIdx.x; g <= g1; g += GN_TS) {
-    const int a0 = max(g * p.Cg - t.c0, 0) / step, a1 = min((g + 1) * p.Cg - t.c0, t.ct) / step;
-    double2 o = {0.0, 0.0};
-    for (int c = a0; c < a1; ++c) {
-      o.x += red[c * 2];
-      o.y += red[c * 2 + 1];
-    }
-    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = o;
+}
+// ... of the part of group g that lies in the tile
+template <int A>
+__device__ __forceinline__ double2 gn_group_sums(const GnP &p, const GnTile &t, int g, const double *red) {
+  constexpr int step = 8 / A;
+  const int a0 = max(g * p.Cg - t.c0, 0) / step, a1 = min((g + 1) * p.Cg - t.c0, t.ct) / step;
+  double2 o = {0.0, 0.0};
+  for (int c = a0; c < a1; ++c) {
+    o.x += red[c * 2];
+    o.y += red[c * 2 + 1];
   }
+  return o;
+}
+__device__ __forceinline__ double2 gn_stats(const GnP &p, double a, double q) {  // mean, rstd
+  const double m = (double)p.S * p.Cg, mean = a / m, var = q / m - mean * mean;
+  return {mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps)};  // (a NaN stays one)
 }
 
-// ---- forward, second launch.  Q: checkpoints are written
-template <class E, int V, int ACT, bool Q>
-__global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
-  constexpr int U = 4;
-  __shared__ double st[2 * GN_CT];  // mean, rstd of the tile's groups
-  const int piece = blockIdx.x / p.nchunk % p.split;
-  const GnTile t = gn_tile(p, blockIdx.x / p.nchunk / p.split * p.nchunk + blockIdx.x % p.nchunk);
-  const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
-  int sub = 64;
-  while (sub > 1 && ng * sub > GN_T) sub >>= 1;
-  for (int i = threadIdx.x; i < ng * sub; i += GN_T) {
-    const int g = g0 + i / sub;
-    double a, q;
-    gn_join(p, t.n, g, i % sub, sub, a, q);
-    const double m = (double)p.S * p.Cg, mean = a / m, var = q / m - mean * mean;
-    const double rstd = 1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps);  // (a NaN stays one)
-    if (i % sub == 0) {
-      st[(g - g0) * 2] = mean;
-      st[(g - g0) * 2 + 1] = rstd;
-      if (p.stats && t.k == 0 && piece == 0 && g * p.Cg >= t.c0) {  // the tile in which the group begins
-        p.stats[((long long)t.n * p.G + g) * 2] = mean;
-        p.stats[((long long)t.n * p.G + g) * 2 + 1] = rstd;
-      }
-    }
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes;
-  const int c = t.c0 + lane * V;
-  if (c >= p.nb * A8_BLOCK) return;    // whole 8-bit blocks leave together
-  const bool in = lane * V < t.ct;     // the others of the last block write the checkpoints' padding
-  float mu[V], sc[V], sh[V];
-  double sc64[V], be64[V];  // LeakyReLU's kink in 64 bits, as the backward pass has it
-  GnGroup at(c, p.Cg);
+template <class E, int A, bool TAIL>
+__global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
+  constexpr int U = 4, B = A < U ? A : U;  // rows loaded at a time, rows added up before fp64
+  __shared__ double red[GN_TS / 64 * (GN_CT / 8) * A * 2];
+  const GnTile t = gn_tile(p, blockIdx.x);
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TS / p.lanes;
+  const int r1 = min(p.S, (t.k + 1) * p.crows);
+  double s1[A], s2[A];
 #pragma unroll
-  for (int i = 0; i < V; ++i, at.next(p.Cg)) {
-    mu[i] = sc[i] = sh[i] = 0.f;
-    sc64[i] = be64[i] = 0.0;
-    if (in) {
-      const int g = at.g - g0;
-      const double mean = st[g * 2], rstd = st[g * 2 + 1];
-      const float ga = p.gamma[(long long)t.n * p.affn + c + i], be = p.beta[(long long)t.n * p.affn + c + i];
-      mu[i] = (float)mean;
-      sc[i] = ga * (float)rstd;
-      sh[i] = (float)((double)be - (mean - (double)mu[i]) * rstd * (double)ga);
-      sc64[i] = rstd * (double)ga;
-      be64[i] = be;
+  for (int i = 0; i < A; ++i) s1[i] = s2[i] = 0.0;
+  if (lane * 8 < t.ct) {
+    int r = t.k * p.crows + rl;
+    const Row8<E, TAIL> row(t.c0 + lane * 8, p.C);
+    const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + r * p.xs;
+    const long long step = RL * p.xs;
+    for (; r + (U - 1) * RL < r1; r += U * RL) {
+      Pack8<E> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u, x += step) v[u] = row.load(x);
+#pragma unroll
+      for (int u = 0; u < U; u += B) gn_add<E, A, B>(v + u, s1, s2);
+    }
+    for (; r < r1; r += RL, x += step) {
+      const Pack8<E> v = row.load(x);
+      gn_add<E, A, 1>(&v, s1, s2);
     }
   }
-  const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
-  int r = t.k * p.crows + piece * p.arows + rl;
-  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + r * p.xs + c;
-  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + ((long long)t.n * p.S + r) * p.C + c;
-  const long long xstep = RL * p.xs, ystep = (long long)RL * p.C;
-  const long long row0 = (long long)t.n * p.S;
-  const auto keep = [&](const float (&v)[V], unsigned char *q, unsigned char *e, long long row, bool kink) {
-    const unsigned code = a8_code(a8_block_max<V>(v));
-    float k[V];
-    a8_round<V>(v, code, k);
+  gn_block_sums<A, GN_TS>(p, s1, s2, red);
+  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg;
+  for (int g = g0 + threadIdx.x; g <= g1; g += GN_TS)
+    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = gn_group_sums<A>(p, t, g, red);
+}
+
+// ---- forward: what a lane does to a row.  Q: checkpoints are written
+template <class E, int ACT, bool Q, bool TAIL>
+struct GnOut {
+  const GnP &p;
+  Row8<E, TAIL> row;
+  int c;
+  bool in;
+  float mu[8], sc[8], sh[8];
+  float lo[8], be[8];  // LeakyReLU's kink: the scale's remainder, beta
+
+  __device__ __forceinline__ GnOut(const GnP &p_, int c_) : p(p_), row(c_, p_.C), c(c_), in(c_ < p_.C) {}
+  // affine parameters (loaded before the statistics are waited for)
+  __device__ __forceinline__ void affine(int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long long at = (long long)n * p.affn + min(c + i, p.C - 1);
+      sc[i] = p.gamma[at];
+      sh[i] = p.beta[at];
+    }
+  }
+  // st: mean, rstd of the groups from g0 on
+  __device__ __forceinline__ void stats(const double *st, int g0) {
+    int g[8];
+    gn_groups(p, c, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool real = !TAIL || c + i < p.C;
+      const double2 s = *reinterpret_cast<const double2 *>(st + (g[i] - g0) * 2);
+      const double ga = real ? (double)sc[i] : 0.0, b = real ? (double)sh[i] : 0.0;
+      const double scale = s.y * ga;
+      mu[i] = real ? (float)s.x : 0.f;
+      be[i] = (float)b;
+      sc[i] = (float)scale;
+      lo[i] = (float)(scale - (double)sc[i]);
+      sh[i] = (float)(b - (s.x - (double)(float)s.x) * scale);
+    }
+  }
+  __device__ __forceinline__ void keep(const float (&v)[8], unsigned char *q, unsigned char *e, long long r, bool kink) const {
+    const unsigned code = a8_code(a8_block_max(v));
+    float k[8];
+    a8_round(v, code, k);
     if (ACT == TBG_ACT_LRELU && kink) {  // one step back where rounding has crossed the kink: the backward pass takes the value's own slope
       const float scale = a8_scale(code);
+      float kept[8], f[8], g[8];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float kept = (k[i] - A8_MAGIC) * scale;
-        if ((fma((double)v[i], sc64[i], be64[i]) > 0.0) != (fma((double)kept, sc64[i], be64[i]) > 0.0))
-          k[i] = fminf(fmaxf(k[i] + (v[i] > kept ? 1.f : -1.f), A8_MAGIC - 127.f), A8_MAGIC + 127.f);
-      }
+      for (int i = 0; i < 8; ++i) kept[i] = (k[i] - A8_MAGIC) * scale;
+      gn_slope(v, sc, lo, be, f);
+      gn_slope(kept, sc, lo, be, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (f[i] != g[i]) k[i] = fminf(fmaxf(k[i] + (v[i] > kept[i] ? 1.f : -1.f), A8_MAGIC - 127.f), A8_MAGIC + 127.f);
     }
-    a8_store<V>(q + row * p.nb * A8_BLOCK + c, code, k);
-    if ((c & (A8_BLOCK - 1)) == 0) e[row * p.nb + c / A8_BLOCK] = (unsigned char)code;
-  };
-  const auto write = [&](int row, const Pack<E, V> &v) {
-    float d[V], o[V];
+    a8_store(q + r * p.nb * A8_BLOCK + c, code, k);
+    if ((c & (A8_BLOCK - 1)) == 0) e[r * p.nb + c / A8_BLOCK] = (unsigned char)code;
+  }
+  // v: channels of row r (of all samples' rows; zeros where there are none), y: where the row goes
+  __device__ __forceinline__ void write(const Pack8<E> &v, typename E::type *y, long long r) const {
+    float d[8], o[8];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < 8; ++i) {
       d[i] = E::get(v.v[i]) - mu[i];
       o[i] = gn_act<ACT>(fmaf(d[i], sc[i], sh[i]));
     }
-    const Pack<E, V> w = put_pack<E, V>(o);
-    if (!Q || in) st_pack<E, V>(y, w);
-    y += ystep;
+    const Pack8<E> w = put8<E>(o);
+    if (!Q || in) row.store(y, w);
     if constexpr (Q) {
+      if (p.q) {
+        if (!in) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = in ? E::get(w.v[i]) : 0.f;  // (beyond the channels x and mu are 0 already)
-      if (p.q) keep(d, p.q, p.e, row0 + row, true);
-      if (p.yq) keep(o, p.yq, p.ye, row0 + row, false);
+          for (int i = 0; i < 8; ++i) d[i] = 0.f;
+        }
+        keep(d, p.q, p.e, r, true);
+      }
+      if (p.yq) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = in && (!TAIL || c + i < p.C) ? E::get(w.v[i]) : 0.f;
+        keep(o, p.yq, p.ye, r, false);
+      }
     }
-  };
-  if (!Q && !in) return;
-  const Pack<E, V> zero = {};
-  for (; r + (U - 1) * RL < r1; r += U * RL) {
-    Pack<E, V> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u, x += xstep) v[u] = in ? ld_pack<E, V>(x) : zero;
-#pragma unroll
-    for (int u = 0; u < U; ++u) write(r + u * RL, v[u]);
   }
-  for (; r < r1; r += RL, x += xstep) write(r, in ? ld_pack<E, V>(x) : zero);
+};
+
+template <class E, int ACT, bool Q, bool TAIL>
+__global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
+  constexpr int U = 4;
+  __shared__ double2 st[GN_CT];  // mean, rstd of the tile's groups
+  const int piece = blockIdx.x / p.nchunk % p.split;
+  const GnTile t = gn_tile(p, blockIdx.x / p.nchunk / p.split * p.nchunk + blockIdx.x % p.nchunk);
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes;
+  GnOut<E, ACT, Q, TAIL> out(p, t.c0 + lane * 8);
+  out.affine(t.n);
+  const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
+  int sub = 64;
+  while (sub > 1 && ng * sub > GN_T) sub >>= 1;
+  if (threadIdx.x < ng * sub) {
+    const int i = threadIdx.x / sub, g = g0 + i;
+    double a, q;
+    gn_join(p, t.n, g, threadIdx.x & (sub - 1), sub, a, q);
+    if ((threadIdx.x & (sub - 1)) == 0) {
+      st[i] = gn_stats(p, a, q);
+      if (p.stats && t.k == 0 && piece == 0 && g * p.Cg >= t.c0)  // the tile in which the group begins
+        *reinterpret_cast<double2 *>(p.stats + ((long long)t.n * p.G + g) * 2) = st[i];
+    }
+  }
+  __syncthreads();
+  if (out.c >= p.nb * A8_BLOCK || (!Q && !out.in)) return;  // whole 8-bit blocks leave together; those beyond the last channel write the padding
+  out.stats(reinterpret_cast<const double *>(st), g0);
+  const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
+  int r = t.k * p.crows + piece * p.arows + rl;
+  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn + r * p.xs;
+  const long long row0 = (long long)t.n * p.S, xstep = RL * p.xs, ystep = (long long)RL * p.C;
+  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + (row0 + r) * p.C;
+  const Pack8<E> zero = {};
+  for (; r + (U - 1) * RL < r1; r += U * RL) {
+    Pack8<E> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u, x += xstep) v[u] = out.in ? out.row.load(x) : zero;
+#pragma unroll
+    for (int u = 0; u < U; ++u, y += ystep) out.write(v[u], y, row0 + r + u * RL);
+  }
+  for (; r < r1; r += RL, x += xstep, y += ystep) out.write(out.in ? out.row.load(x) : zero, y, row0 + r);
 }
 
-// ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd: a lane keeps z = sc d + be of its V channels
-template <int V>
-struct GnCh {
-  float mu[V], lo[V], sc[V], za[V], zb[V];  // za, zb: the same times -log2(e), for the exponential
-  double sc64[V], be64[V];
-};
-template <int V, bool Q8>
-__device__ __forceinline__ void gn_channels(const GnP &p, int n, int c, GnCh<V> &h) {
-  GnGroup at(c, p.Cg);
+// ---- forward in one launch, where the rows of a tile of whole groups fit a block's registers: x is read once
+template <class E, int A, int ACT, bool Q, bool TAIL>
+__global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
+  __shared__ double red[GN_TW / 64 * (GN_CT / 8) * A * 2];
+  __shared__ double2 st[GN_CT];
+  const GnTile t = gn_tile(p, blockIdx.x);
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TW / p.lanes;
+  GnOut<E, ACT, Q, TAIL> out(p, t.c0 + lane * 8);
+  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn;
+  Pack8<E> v[GN_R] = {};
+  double s1[A], s2[A];
 #pragma unroll
-  for (int i = 0; i < V; ++i, at.next(p.Cg)) {
-    const double2 s = *reinterpret_cast<const double2 *>(p.stats + ((long long)n * p.G + at.g) * 2);
-    const float ga = p.gamma[(long long)n * p.affn + c + i];
+  for (int i = 0; i < A; ++i) s1[i] = s2[i] = 0.0;
+  if (out.in) {
+#pragma unroll
+    for (int u = 0; u < GN_R; ++u)
+      if (rl + u * RL < p.S) v[u] = out.row.load(x + (rl + u * RL) * p.xs);
+  }
+  out.affine(t.n);
+  if (out.in) {
+#pragma unroll
+    for (int u = 0; u < GN_R; ++u) gn_add<E, A, 1>(v + u, s1, s2);  // (rows that do not exist are zeros)
+  }
+  gn_block_sums<A, GN_TW>(p, s1, s2, red);
+  const int g0 = t.c0 / p.Cg, ng = (t.ct + p.Cg - 1) / p.Cg;
+  if (threadIdx.x < ng) {
+    const double2 s = gn_group_sums<A>(p, t, g0 + threadIdx.x, red);
+    st[threadIdx.x] = gn_stats(p, s.x, s.y);
+    if (p.stats) *reinterpret_cast<double2 *>(p.stats + ((long long)t.n * p.G + g0 + threadIdx.x) * 2) = st[threadIdx.x];
+  }
+  __syncthreads();
+  if (out.c >= p.nb * A8_BLOCK || (!Q && !out.in)) return;
+  out.stats(reinterpret_cast<const double *>(st), g0);
+  const long long row0 = (long long)t.n * p.S;
+  typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + row0 * p.C;
+#pragma unroll
+  for (int u = 0; u < GN_R; ++u)
+    if (rl + u * RL < p.S) out.write(v[u], y + (long long)(rl + u * RL) * p.C, row0 + rl + u * RL);
+}
+
+// ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd and z = sc d + be
+struct GnCh {
+  float mu[8], mlo[8], sc[8], lo[8], be[8], za[8], zb[8];  // mean, scale: and their remainders; za, zb: sc, be times -log2(e), for the exponential
+};
+template <bool Q8>
+__device__ __forceinline__ void gn_channels(const GnP &p, int n, int c, GnCh &h) {
+  int g[8];
+  gn_groups(p, c, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double2 s = *reinterpret_cast<const double2 *>(p.stats + ((long long)n * p.G + g[i]) * 2);
+    const long long at = (long long)n * p.affn + min(c + i, p.C - 1);
     h.mu[i] = Q8 ? 0.f : (float)s.x;
-    h.lo[i] = Q8 ? 0.f : (float)(s.x - (double)(float)s.x);
-    h.sc64[i] = s.y * (double)ga;
-    h.sc[i] = (float)h.sc64[i];
-    h.be64[i] = p.beta[(long long)n * p.affn + c + i];
-    h.za[i] = (float)(-1.44269504088896341 * h.sc64[i]);
-    h.zb[i] = (float)(-1.44269504088896341 * h.be64[i]);
+    h.mlo[i] = Q8 ? 0.f : (float)(s.x - (double)(float)s.x);
+    const double scale = s.y * (double)p.gamma[at];
+    h.sc[i] = (float)scale;
+    h.lo[i] = (float)(scale - (double)h.sc[i]);
+    h.be[i] = p.beta[at];
+    h.za[i] = (float)(-1.44269504088896341 * scale);
+    h.zb[i] = (float)(-1.44269504088896341 * (double)h.be[i]);
   }
 }
 // a row's operands as they lie in memory
-template <class E, int V, bool Q8>
+template <class E, bool Q8>
 struct GnRow {
-  Pack<E, V> g, x;
+  Pack8<E> g, x;
   u32x2 q;
   unsigned e;
 };
 // where a lane stands, and a step of `rows` rows
-template <class E, int V, bool Q8>
+template <class E, bool Q8, bool TAIL>
 struct GnAt {
+  Row8<E, TAIL> row;
   const typename E::type *x, *g;
   const unsigned char *q, *e;
-  __device__ __forceinline__ GnAt(const GnP &p, int n, int r, int c) {
-    const long long row = (long long)n * p.S + r;
-    x = reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + r * p.xs + c;
-    g = reinterpret_cast<const typename E::type *>(p.dy) + n * p.dn + r * p.ds + c;
-    q = p.q + row * p.nb * A8_BLOCK + c;
-    e = p.e + row * p.nb + c / A8_BLOCK;
+  __device__ __forceinline__ GnAt(const GnP &p, int n, int r, int c) : row(c, p.C) {
+    const long long at = (long long)n * p.S + r;
+    x = reinterpret_cast<const typename E::type *>(p.x) + n * p.xn + r * p.xs;
+    g = reinterpret_cast<const typename E::type *>(p.dy) + n * p.dn + r * p.ds;
+    q = p.q + at * p.nb * A8_BLOCK + c;
+    e = p.e + at * p.nb + c / A8_BLOCK;
   }
-  __device__ __forceinline__ GnRow<E, V, Q8> next(const GnP &p, int rows) {
-    GnRow<E, V, Q8> w;
+  __device__ __forceinline__ GnRow<E, Q8> next(const GnP &p, int rows) {
+    GnRow<E, Q8> w;
     if constexpr (Q8) {
       w.e = *e;
-      if constexpr (V == 8) w.q = *reinterpret_cast<const u32x2 *>(q);
-      else w.q[0] = *q;
+      w.q = *reinterpret_cast<const u32x2 *>(q);
       q += (long long)rows * p.nb * A8_BLOCK;
       e += (long long)rows * p.nb;
     } else {
-      w.x = ld_pack<E, V>(x);
+      w.x = row.load(x);
       x += rows * p.xs;
     }
-    w.g = ld_pack<E, V>(g);
+    w.g = row.load(g);
     g += rows * p.ds;
     return w;
   }
 };
 // d and dz of a row
-template <class E, int V, int ACT, bool Q8>
-__device__ __forceinline__ void gn_row(const GnRow<E, V, Q8> &w, const GnCh<V> &h, float (&d)[V], float (&dz)[V]) {
+template <class E, int ACT, bool Q8>
+__device__ __forceinline__ void gn_row(const GnRow<E, Q8> &w, const GnCh &h, float (&d)[8], float (&dz)[8]) {
   const float scale = Q8 ? a8_scale(w.e) : 1.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (Q8) d[i] = (float)(int)(signed char)(w.q[i >> 2] >> (8 * (i & 3)) & 0xff) * scale;
-    else d[i] = (E::get(w.x.v[i]) - h.mu[i]) - h.lo[i];
-    const float z = ACT == TBG_ACT_SILU ? fmaf(d[i], h.za[i], h.zb[i]) : 0.f;
-    const bool pos = ACT == TBG_ACT_LRELU ? fma((double)d[i], h.sc64[i], h.be64[i]) > 0.0 : false;
-    dz[i] = gn_dact<ACT>(E::get(w.g.v[i]), z, pos);
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (Q8) d[i] = a8_value(w.q, i) * scale;
+    else d[i] = (E::get(w.x.v[i]) - h.mu[i]) - h.mlo[i];
+  }
+  if constexpr (ACT == TBG_ACT_LRELU) {
+    gn_slope(d, h.sc, h.lo, h.be, dz);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dz[i] *= E::get(w.g.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dz[i] = gn_dact<ACT>(E::get(w.g.v[i]), ACT == TBG_ACT_SILU ? fmaf(d[i], h.za[i], h.zb[i]) : 0.f);
   }
 }
 
 // ---- backward, first launch: sums of dz and dz xh of every channel, and of gamma dz and gamma dz xh of every group
-template <class E, int V, int ACT, bool Q8>
-__global__ __launch_bounds__(GN_TB, V == 8 ? 4 : 8) void gn_bwd_sums_kernel(GnP p) {
+template <class E, int ACT, bool Q8, bool TAIL>
+__global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
   constexpr int U = 2, NW = GN_TB / 64;
   __shared__ float red[NW * GN_CT * 2];
   const GnTile t = gn_tile(p, blockIdx.x);
   const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TB / p.lanes;
-  const int r1 = min(p.S, (t.k + 1) * p.crows), c = t.c0 + lane * V;
-  float s1[V], s2[V];
+  const int r1 = min(p.S, (t.k + 1) * p.crows), c = t.c0 + lane * 8;
+  float s1[8], s2[8];
 #pragma unroll
-  for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.f;
-  if (lane * V < t.ct) {
-    GnCh<V> h;
-    gn_channels<V, Q8>(p, t.n, c, h);
-    const auto add = [&](const GnRow<E, V, Q8> &w) {
-      float d[V], dz[V];
-      gn_row<E, V, ACT, Q8>(w, h, d, dz);
+  for (int i = 0; i < 8; ++i) s1[i] = s2[i] = 0.f;
+  if (lane * 8 < t.ct) {
+    GnCh h;
+    gn_channels<Q8>(p, t.n, c, h);
+    const auto add = [&](const GnRow<E, Q8> &w) {
+      float d[8], dz[8];
+      gn_row<E, ACT, Q8>(w, h, d, dz);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int i = 0; i < 8; ++i) {
         s1[i] += dz[i];
         s2[i] = fmaf(dz[i], d[i], s2[i]);
       }
     };
     int r = t.k * p.crows + rl;
-    GnAt<E, V, Q8> at(p, t.n, r, c);
+    GnAt<E, Q8, TAIL> at(p, t.n, r, c);
     for (; r + (U - 1) * RL < r1; r += U * RL) {
-      GnRow<E, V, Q8> w[U];
+      GnRow<E, Q8> w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
 #pragma unroll
@@ -397,16 +503,16 @@ __global__ __launch_bounds__(GN_TB, V == 8 ? 4 : 8) void gn_bwd_sums_kernel(GnP 
   }
   for (int off = p.lanes; off < 64; off <<= 1)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < 8; ++i) {
       s1[i] += __shfl_xor(s1[i], off, 64);
       s2[i] += __shfl_xor(s2[i], off, 64);
     }
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) < p.lanes)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      red[(wave * p.CT + lane * V + i) * 2] = s1[i];
-      red[(wave * p.CT + lane * V + i) * 2 + 1] = s2[i];
+    for (int i = 0; i < 8; ++i) {
+      red[(wave * p.CT + lane * 8 + i) * 2] = s1[i];
+      red[(wave * p.CT + lane * 8 + i) * 2 + 1] = s2[i];
     }
   __syncthreads();
   if (threadIdx.x < 2 * t.ct) {
@@ -432,10 +538,10 @@ __global__ __launch_bounds__(GN_TB, V == 8 ? 4 : 8) void gn_bwd_sums_kernel(GnP 
 }
 
 // ---- backward, second launch: dx, and in its first blocks dgamma / dbeta
-template <class E, int V, int ACT, bool Q8>
-__global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) {
+template <class E, int ACT, bool Q8, bool TAIL>
+__global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   constexpr int U = 2;
-  __shared__ double st[2 * GN_CT];  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh)
+  __shared__ double2 st[GN_CT];  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh)
   int b = blockIdx.x;
   if (b < p.pblocks) {  // 8 lanes a channel: the row ranges (and samples, where the parameters are shared) in a fixed order
     const long long idx = (long long)b * (GN_T / 8) + threadIdx.x / 8;
@@ -465,46 +571,49 @@ __global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) 
   b -= p.pblocks;
   const int piece = b / p.nchunk % p.split;
   const GnTile t = gn_tile(p, b / p.nchunk / p.split * p.nchunk + b % p.nchunk);
+  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes, c = t.c0 + lane * 8;
+  GnCh h;
+  gn_channels<Q8>(p, t.n, c, h);
   const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
   int sub = 64;
   while (sub > 1 && ng * sub > GN_T) sub >>= 1;
-  for (int i = threadIdx.x; i < ng * sub; i += GN_T) {
+  if (threadIdx.x < ng * sub) {
+    const int i = threadIdx.x / sub;
     double a, q;
-    gn_join(p, t.n, g0 + i / sub, i % sub, sub, a, q);
+    gn_join(p, t.n, g0 + i, threadIdx.x & (sub - 1), sub, a, q);
     const double m = (double)p.S * p.Cg;
-    if (i % sub == 0) {
-      const double rstd = p.stats[((long long)t.n * p.G + g0 + i / sub) * 2 + 1];
-      st[(i / sub) * 2] = rstd * (a / m);
-      st[(i / sub) * 2 + 1] = rstd * rstd * (q / m);
+    if ((threadIdx.x & (sub - 1)) == 0) {
+      const double rstd = p.stats[((long long)t.n * p.G + g0 + i) * 2 + 1];
+      st[i] = {rstd * (a / m), rstd * rstd * (q / m)};
     }
   }
   __syncthreads();
-  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes;
-  if (lane * V >= t.ct) return;
-  const int c = t.c0 + lane * V;
-  GnCh<V> h;
-  gn_channels<V, Q8>(p, t.n, c, h);
-  float m1[V], m2[V];  // dx = sc dz - m1 - d m2
-  GnGroup cg(c, p.Cg);
+  if (lane * 8 >= t.ct) return;
+  float m1[8], m2[8];  // dx = sc dz - m1 - d m2
+  {
+    int g[8];
+    gn_groups(p, c, g);
 #pragma unroll
-  for (int i = 0; i < V; ++i, cg.next(p.Cg)) {
-    m1[i] = (float)st[(cg.g - g0) * 2];
-    m2[i] = (float)st[(cg.g - g0) * 2 + 1];
+    for (int i = 0; i < 8; ++i) {
+      const double2 s = st[g[i] - g0];
+      m1[i] = (float)s.x;
+      m2[i] = (float)s.y;
+    }
   }
   const int r1 = min(p.S, min((t.k + 1) * p.crows, t.k * p.crows + (piece + 1) * p.arows));
   int r = t.k * p.crows + piece * p.arows + rl;
-  GnAt<E, V, Q8> at(p, t.n, r, c);
-  typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + ((long long)t.n * p.S + r) * p.C + c;
-  const auto write = [&](const GnRow<E, V, Q8> &w) {
-    float d[V], dz[V];
-    gn_row<E, V, ACT, Q8>(w, h, d, dz);
+  GnAt<E, Q8, TAIL> at(p, t.n, r, c);
+  typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + ((long long)t.n * p.S + r) * p.C;
+  const auto write = [&](const GnRow<E, Q8> &w) {
+    float d[8], dz[8];
+    gn_row<E, ACT, Q8>(w, h, d, dz);
 #pragma unroll
-    for (int i = 0; i < V; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
-    st_pack<E, V>(dx, put_pack<E, V>(dz));
+    for (int i = 0; i < 8; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
+    at.row.store(dx, put8<E>(dz));
     dx += (long long)RL * p.C;
   };
   for (; r + (U - 1) * RL < r1; r += U * RL) {
-    GnRow<E, V, Q8> w[U];
+    GnRow<E, Q8> w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
 #pragma unroll
@@ -514,29 +623,44 @@ __global__ __launch_bounds__(GN_T, V == 8 ? 4 : 8) void gn_bwd_dx_kernel(GnP p) 
 }
 
 // ---- host side
-// What a call runs is a function of the descriptor and the pointers' alignment.  The workspace holds for either alignment.
 static bool gn_desc_ok(const tbg_gn_desc *d) {
   return d && d->N >= 1 && d->S >= 1 && d->C >= 1 && d->G >= 1 && d->C % d->G == 0 && dt_valid(d->dtype) && d->act >= TBG_ACT_LINEAR &&
          d->act <= TBG_ACT_SILU && (d->per_sample == 0 || d->per_sample == 1) && d->eps > 0.f && d->xs >= d->C && d->xn >= 0 && d->ds >= d->C && d->dn >= 0;
 }
-// Row ranges: the sums launch has at most 32 a tile (64 where the samples and tiles are few), each joined by every block of the second
-// launch that needs it; that launch cuts them into pieces for about 8 blocks a CU, of 8 rows a lane or more.
-static int gn_geometry(const tbg_gn_desc *d, bool vec, bool backward, GnP &p) {
+static void gn_tiles(GnP &p, int CT) {
+  p.CT = CT;
+  p.ntile = (p.C + CT - 1) / CT;
+  p.lanes = CT / 8;
+  p.nslot = p.ntile + p.G - 1;
+}
+// One launch (forward): a tile of whole groups whose rows fit a block's registers.  Of those the narrowest: more blocks.
+static bool gn_whole_tile(GnP &p) {
+  for (int ct = 32; ct <= GN_CT; ct <<= 1)
+    if ((ct % p.Cg == 0 || ct >= p.C) && p.S <= (long long)GN_R * (GN_TW / (ct / 8))) {
+      gn_tiles(p, ct);
+      p.nchunk = p.split = 1;
+      p.crows = p.arows = p.S;
+      return true;
+    }
+  return false;
+}
+// Two launches.  Row ranges: the sums launch has at most 32 a tile (64 where the samples and tiles are few), each joined by every block of the
+// second launch that needs it; that launch cuts them into pieces for about 8 blocks a CU, of 8 rows a lane or more.
+static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   if (d->S > (1 << 30) || d->C > (1 << 24)) return TBG_ERANGE;
-  const int V = vec ? 8 : 1;
   p.N = d->N; p.S = d->S; p.C = d->C; p.G = d->G; p.Cg = d->C / d->G; p.affn = d->per_sample ? d->C : 0;
   p.nb = (d->C + A8_BLOCK - 1) / A8_BLOCK;
   p.xn = d->xn; p.xs = d->xs; p.dn = d->dn; p.ds = d->ds; p.eps = d->eps;
+  const long long count = d->per_sample ? (long long)d->N * d->C : d->C;
+  p.pblocks = (int)((count + GN_T / 8 - 1) / (GN_T / 8));
   // the tile (a power of two; a row's 8-bit block never spans two) that leaves the fewest lanes without channels
   const int padded = p.nb * A8_BLOCK;
-  p.CT = 0;
-  for (int ct = vec ? GN_CT : 64, best = 0; ct >= 32; ct >>= 1) {
+  int best = 0, tile = 0;
+  for (int ct = GN_CT; ct >= 32; ct >>= 1) {
     const int used = (int)(1000LL * padded / ((long long)(padded + ct - 1) / ct * ct));
-    if (used > best && (ct > 32 || padded == 32 || !p.CT)) { best = used; p.CT = ct; }
+    if (used > best && (ct > 32 || padded == 32)) { best = used; tile = ct; }
   }
-  p.ntile = (d->C + p.CT - 1) / p.CT;
-  p.lanes = p.CT / V;
-  p.nslot = p.ntile + p.G - 1;
+  gn_tiles(p, tile);
   const int RL = (backward ? GN_TB : GN_TS) / p.lanes, RA = GN_T / p.lanes;
   const long long tiles = (long long)p.N * p.ntile;
   long long want = 512 / tiles;
@@ -554,9 +678,8 @@ static int gn_geometry(const tbg_gn_desc *d, bool vec, bool backward, GnP &p) {
   if (split < 1) split = 1;
   p.arows = (int)(((p.crows + split - 1) / split + RA - 1) / RA * RA);
   p.split = (p.crows + p.arows - 1) / p.arows;
-  const long long count = d->per_sample ? (long long)d->N * d->C : d->C;
-  if (tiles * p.nchunk * p.split > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
-  p.pblocks = (int)((count + GN_T / 8 - 1) / (GN_T / 8));
+  if (!backward && !GN_NOWHOLE) gn_whole_tile(p);
+  if ((long long)p.N * p.ntile * p.nchunk * p.split > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
   return TBG_OK;
 }
 static long long gn_part_bytes(const GnP &p) { return (long long)p.N * p.nchunk * p.nslot * 2 * (long long)sizeof(double); }
@@ -564,56 +687,59 @@ static long long gn_pch_bytes(const GnP &p) { return (long long)p.N * p.nchunk *
 
 extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int backward) {
   if (!gn_desc_ok(d)) return TBG_EINVAL;
-  long long most = 0;
-  for (int vec = 0; vec < 2; ++vec) {
-    GnP p{};
-    if (const int rc = gn_geometry(d, vec != 0, backward != 0, p)) return rc;
-    const long long b = gn_part_bytes(p) + (backward ? gn_pch_bytes(p) : 0);
-    if (b > most) most = b;
-  }
-  return most;
+  GnP p{};
+  if (const int rc = gn_geometry(d, backward != 0, p)) return rc;
+  return gn_part_bytes(p) + (backward ? gn_pch_bytes(p) : 0);
 }
 
-template <class E, int V, int ACT>
+// the accumulators a lane needs: channels in runs of 8, 4, 2 or 1 within a group
+template <class E, int ACT, bool Q, bool TAIL>
 static int gn_run_fwd(const GnP &p, hipStream_t st) {
-  const auto sums = V == 1 || p.Cg % 8 == 0 ? gn_sums_kernel<E, V, 1>
-                    : p.Cg % 4 == 0 ? gn_sums_kernel<E, V, V == 8 ? 2 : 1>
-                    : p.Cg % 2 == 0 ? gn_sums_kernel<E, V, V == 8 ? 4 : 1> : gn_sums_kernel<E, V, V>;
-  const auto apply = p.q || p.yq ? gn_apply_kernel<E, V, ACT, true> : gn_apply_kernel<E, V, ACT, false>;
+  const int run = TAIL ? (p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1) : (p.Cg % 8 == 0 ? 8 : p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1);
+  constexpr int A8 = TAIL ? 2 : 1;
+  if (p.nchunk == 1 && p.crows == p.S) {
+    const auto whole = run == 8 ? gn_whole_kernel<E, A8, ACT, Q, TAIL> : run == 4 ? gn_whole_kernel<E, 2, ACT, Q, TAIL>
+                       : run == 2 ? gn_whole_kernel<E, 4, ACT, Q, TAIL> : gn_whole_kernel<E, 8, ACT, Q, TAIL>;
+    hipLaunchKernelGGL(whole, dim3(p.N * p.ntile), dim3(GN_TW), 0, st, p);
+    TBG_LAUNCH_CHECK();
+    return TBG_OK;
+  }
+  const auto sums = run == 8 ? gn_sums_kernel<E, A8, TAIL> : run == 4 ? gn_sums_kernel<E, 2, TAIL>
+                    : run == 2 ? gn_sums_kernel<E, 4, TAIL> : gn_sums_kernel<E, 8, TAIL>;
   hipLaunchKernelGGL(sums, dim3(p.N * p.ntile * p.nchunk), dim3(GN_TS), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL(apply, dim3(p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
+  hipLaunchKernelGGL((gn_apply_kernel<E, ACT, Q, TAIL>), dim3(p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
-template <class E, int V, int ACT, bool Q8>
+template <class E, int ACT, bool Q8, bool TAIL>
 static int gn_run_bwd(const GnP &p, hipStream_t st) {
-  hipLaunchKernelGGL((gn_bwd_sums_kernel<E, V, ACT, Q8>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
+  hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT, Q8, TAIL>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, V, ACT, Q8>), dim3(p.pblocks + p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
+  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, Q8, TAIL>), dim3(p.pblocks + p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
-template <class E, int V, int ACT>
+template <class E, int ACT, bool TAIL>
 static int gn_run(const GnP &p, bool backward, hipStream_t st) {
-  if (!backward) return gn_run_fwd<E, V, ACT>(p, st);
-  return p.q ? gn_run_bwd<E, V, ACT, true>(p, st) : gn_run_bwd<E, V, ACT, false>(p, st);
+  if (backward) return p.q ? gn_run_bwd<E, ACT, true, TAIL>(p, st) : gn_run_bwd<E, ACT, false, TAIL>(p, st);
+  return p.q || p.yq ? gn_run_fwd<E, ACT, true, TAIL>(p, st) : gn_run_fwd<E, ACT, false, TAIL>(p, st);
+}
+template <class E, bool TAIL>
+static int gn_run_act(const GnP &p, int act, bool backward, hipStream_t st) {
+  return act == TBG_ACT_LINEAR ? gn_run<E, TBG_ACT_LINEAR, TAIL>(p, backward, st)
+         : act == TBG_ACT_LRELU ? gn_run<E, TBG_ACT_LRELU, TAIL>(p, backward, st)
+                                : gn_run<E, TBG_ACT_SILU, TAIL>(p, backward, st);
 }
 template <class E>
-static int gn_run_type(const GnP &p, bool vec, int act, bool backward, hipStream_t st) {
-  if (vec)
-    return act == TBG_ACT_LINEAR ? gn_run<E, 8, TBG_ACT_LINEAR>(p, backward, st)
-           : act == TBG_ACT_LRELU ? gn_run<E, 8, TBG_ACT_LRELU>(p, backward, st)
-                                  : gn_run<E, 8, TBG_ACT_SILU>(p, backward, st);
-  return act == TBG_ACT_LINEAR ? gn_run<E, 1, TBG_ACT_LINEAR>(p, backward, st)
-         : act == TBG_ACT_LRELU ? gn_run<E, 1, TBG_ACT_LRELU>(p, backward, st)
-                                : gn_run<E, 1, TBG_ACT_SILU>(p, backward, st);
+static int gn_run_type(const GnP &p, int act, bool backward, hipStream_t st) {
+  return p.C % 8 ? gn_run_act<E, true>(p, act, backward, st) : gn_run_act<E, false>(p, act, backward, st);
 }
-static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool vec, bool backward, void *stream) {
+static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool backward, void *stream) {
   hipStream_t st = tbg_stream(stream);
-  return d->dtype == TBG_DT_F32 ? gn_run_type<ElF32>(p, vec, d->act, backward, st)
-         : d->dtype == TBG_DT_BF16 ? gn_run_type<ElBf16>(p, vec, d->act, backward, st)
-                                   : gn_run_type<ElF16>(p, vec, d->act, backward, st);
+  return d->dtype == TBG_DT_F32 ? gn_run_type<ElF32>(p, d->act, backward, st)
+         : d->dtype == TBG_DT_BF16 ? gn_run_type<ElBf16>(p, d->act, backward, st)
+                                   : gn_run_type<ElF16>(p, d->act, backward, st);
 }
 static bool gn_misaligned(const void *a, const void *b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) != 0; }
 
@@ -622,14 +748,13 @@ extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const flo
   if (!gn_desc_ok(d) || !x || !gamma || !beta || !y || !workspace || (q == nullptr) != (e == nullptr) || (yq == nullptr) != (ye == nullptr))
     return TBG_EINVAL;
   if (gn_misaligned(q, yq) || gn_misaligned(workspace, stats)) return TBG_EINVAL;
-  const bool vec = d->C % 8 == 0 && vec8_ok(x, d->dtype, d->xs, d->xn) && vec8_ok(y, d->dtype, d->C);
   GnP p{};
-  if (const int rc = gn_geometry(d, vec, false, p)) return rc;
+  if (const int rc = gn_geometry(d, false, p)) return rc;
   if (gn_part_bytes(p) > workspace_bytes) return TBG_EINVAL;
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = y; p.stats = stats; p.part = reinterpret_cast<double *>(workspace);
   p.q = reinterpret_cast<unsigned char *>(q); p.e = reinterpret_cast<unsigned char *>(e);
   p.yq = reinterpret_cast<unsigned char *>(yq); p.ye = reinterpret_cast<unsigned char *>(ye);
-  return gn_dispatch(d, p, vec, false, stream);
+  return gn_dispatch(d, p, false, stream);
 }
 
 extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const void *q, const void *e, const void *dy, const float *gamma,
@@ -639,9 +764,8 @@ extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const voi
       (x == nullptr) == (q == nullptr))
     return TBG_EINVAL;
   if (gn_misaligned(q, workspace) || gn_misaligned(stats, nullptr)) return TBG_EINVAL;
-  const bool vec = d->C % 8 == 0 && (!x || vec8_ok(x, d->dtype, d->xs, d->xn)) && vec8_ok(dy, d->dtype, d->ds, d->dn) && vec8_ok(dx, d->dtype, d->C);
   GnP p{};
-  if (const int rc = gn_geometry(d, vec, true, p)) return rc;
+  if (const int rc = gn_geometry(d, true, p)) return rc;
   if (gn_part_bytes(p) + gn_pch_bytes(p) > workspace_bytes) return TBG_EINVAL;
   p.x = x; p.dy = dy; p.gamma = gamma; p.beta = beta; p.y = dx; p.stats = const_cast<double *>(stats);
   p.q = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(q));
@@ -649,5 +773,5 @@ extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const voi
   p.part = reinterpret_cast<double *>(workspace);
   p.pch = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + gn_part_bytes(p));
   p.dgamma = dgamma; p.dbeta = dbeta;
-  return gn_dispatch(d, p, vec, true, stream);
+  return gn_dispatch(d, p, true, stream);
 }
