@@ -120,6 +120,7 @@ def test_empty_tensors(dev):
 SHAPES = [  # N, positions, C, groups
     (1, 1, 1, 1), (2, 1, 8, 8), (1, 1, 64, 2), (2, 3, 32, 32), (3, 5, 24, 8), (1, 7, 33, 11), (2, 17, 40, 5), (2, 100, 96, 3), (4, 64, 128, 32),
     (1, 300, 160, 5), (2, 33, 250, 10), (3, 65, 120, 8), (1, 40, 1024, 1), (1, 9, 2056, 2), (2, 1000, 64, 4), (5, 130, 256, 16), (1, 4097, 48, 6), (300, 2, 16, 2),
+    (2, 64, 256, 1), (1, 128, 384, 2), (3, 512, 64, 1), (1, 1024, 32, 4), (2, 1025, 40, 8), (1, 70, 136, 17), (2, 33, 7, 7), (2, 5, 5, 1), (1, 600, 100, 4),
 ]
 
 

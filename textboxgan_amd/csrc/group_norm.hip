@@ -28,16 +28,11 @@ struct GnP {
   int CT, ntile, lanes;                // channels a tile (a power of two), tiles, lanes a row
   int nchunk, crows, nslot;            // row ranges of the sums launch
   int split, arows;                    // the second launch's part of a row range: `split` pieces of arows rows
+  int whole;                           // forward in one launch
   int pblocks;                         // backward: first blocks of the second launch that sum dgamma / dbeta
   float eps;
 };
 
-#ifndef GN_NOWHOLE
-#define GN_NOWHOLE 0
-#endif
-#ifndef GN_BLOCKS
-#define GN_BLOCKS 2048
-#endif
 // threads a block: second launches, forward sums, backward sums, whole forward; most channels a tile; rows a lane of the whole forward keeps
 constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_TW = 512, GN_CT = 128, GN_R = 8;
 
@@ -107,12 +102,21 @@ __device__ __forceinline__ GnTile gn_tile(const GnP &p, int b) {
 __device__ __forceinline__ void gn_join(const GnP &p, int n, int g, int lane, int sub, double &a, double &b) {
   const int t0 = g * p.Cg / p.CT, t1 = ((g + 1) * p.Cg - 1) / p.CT, nt = t1 - t0 + 1;
   a = b = 0.0;
-  const double *base = p.part + (long long)n * p.nchunk * p.nslot * 2;
-  for (int i = lane; i < nt * p.nchunk; i += sub) {
-    const int k = i / nt, t = t0 + i - k * nt;
-    const double2 s = *reinterpret_cast<const double2 *>(base + ((long long)k * p.nslot + t + g) * 2);
-    a += s.x;
-    b += s.y;
+  const double *base = p.part + ((long long)n * p.nchunk * p.nslot + t0 + g) * 2;
+  if (nt == 1) {
+#pragma unroll 8
+    for (int k = lane; k < p.nchunk; k += sub) {  // (the loads of all ranges under way at once)
+      const double2 s = *reinterpret_cast<const double2 *>(base + (long long)k * p.nslot * 2);
+      a += s.x;
+      b += s.y;
+    }
+  } else {
+    for (int i = lane; i < nt * p.nchunk; i += sub) {
+      const int k = i / nt;
+      const double2 s = *reinterpret_cast<const double2 *>(base + ((long long)k * p.nslot + i - k * nt) * 2);
+      a += s.x;
+      b += s.y;
+    }
   }
   for (int off = sub >> 1; off > 0; off >>= 1) {
     a += __shfl_xor(a, off, 64);
@@ -227,6 +231,18 @@ __global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
     *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = gn_group_sums<A>(p, t, g, red);
 }
 
+// gamma and beta of a lane's channels, zeros beyond the last
+template <bool TAIL>
+__device__ __forceinline__ void gn_affine(const GnP &p, int n, int c, float (&ga)[8], float (&be)[8]) {
+  const Row8<ElF32, TAIL> row(c, p.C);
+  const Pack8<ElF32> a = row.load(p.gamma + (long long)n * p.affn), b = row.load(p.beta + (long long)n * p.affn);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    ga[i] = a.v[i];
+    be[i] = b.v[i];
+  }
+}
+
 // ---- forward: what a lane does to a row.  Q: checkpoints are written
 template <class E, int ACT, bool Q, bool TAIL>
 struct GnOut {
@@ -238,14 +254,9 @@ struct GnOut {
   float lo[8], be[8];  // LeakyReLU's kink: the scale's remainder, beta
 
   __device__ __forceinline__ GnOut(const GnP &p_, int c_) : p(p_), row(c_, p_.C), c(c_), in(c_ < p_.C) {}
-  // affine parameters (loaded before the statistics are waited for)
+  // affine parameters, 0 where there is no channel (loaded before the statistics are waited for)
   __device__ __forceinline__ void affine(int n) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long long at = (long long)n * p.affn + min(c + i, p.C - 1);
-      sc[i] = p.gamma[at];
-      sh[i] = p.beta[at];
-    }
+    if (in) gn_affine<TAIL>(p, n, c, sc, sh);
   }
   // st: mean, rstd of the groups from g0 on
   __device__ __forceinline__ void stats(const double *st, int g0) {
@@ -255,8 +266,7 @@ struct GnOut {
     for (int i = 0; i < 8; ++i) {
       const bool real = !TAIL || c + i < p.C;
       const double2 s = *reinterpret_cast<const double2 *>(st + (g[i] - g0) * 2);
-      const double ga = real ? (double)sc[i] : 0.0, b = real ? (double)sh[i] : 0.0;
-      const double scale = s.y * ga;
+      const double b = sh[i], scale = s.y * (double)sc[i];
       mu[i] = real ? (float)s.x : 0.f;
       be[i] = (float)b;
       sc[i] = (float)scale;
@@ -394,20 +404,19 @@ __global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
 struct GnCh {
   float mu[8], mlo[8], sc[8], lo[8], be[8], za[8], zb[8];  // mean, scale: and their remainders; za, zb: sc, be times -log2(e), for the exponential
 };
+// st: mean, rstd of the groups from g0 on; sc, be come as gamma, beta
 template <bool Q8>
-__device__ __forceinline__ void gn_channels(const GnP &p, int n, int c, GnCh &h) {
+__device__ __forceinline__ void gn_channels(const GnP &p, int c, const double2 *st, int g0, GnCh &h) {
   int g[8];
   gn_groups(p, c, g);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const double2 s = *reinterpret_cast<const double2 *>(p.stats + ((long long)n * p.G + g[i]) * 2);
-    const long long at = (long long)n * p.affn + min(c + i, p.C - 1);
+    const double2 s = st[g[i] - g0];
     h.mu[i] = Q8 ? 0.f : (float)s.x;
     h.mlo[i] = Q8 ? 0.f : (float)(s.x - (double)(float)s.x);
-    const double scale = s.y * (double)p.gamma[at];
+    const double scale = s.y * (double)h.sc[i];
     h.sc[i] = (float)scale;
     h.lo[i] = (float)(scale - (double)h.sc[i]);
-    h.be[i] = p.beta[at];
     h.za[i] = (float)(-1.44269504088896341 * scale);
     h.zb[i] = (float)(-1.44269504088896341 * (double)h.be[i]);
   }
@@ -472,15 +481,20 @@ template <class E, int ACT, bool Q8, bool TAIL>
 __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
   constexpr int U = 2, NW = GN_TB / 64;
   __shared__ float red[NW * GN_CT * 2];
+  __shared__ double2 st[GN_CT];  // mean, rstd of the tile's groups
   const GnTile t = gn_tile(p, blockIdx.x);
+  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg;
+  if (threadIdx.x <= g1 - g0) st[threadIdx.x] = *reinterpret_cast<const double2 *>(p.stats + ((long long)t.n * p.G + g0 + threadIdx.x) * 2);
   const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TB / p.lanes;
   const int r1 = min(p.S, (t.k + 1) * p.crows), c = t.c0 + lane * 8;
   float s1[8], s2[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) s1[i] = s2[i] = 0.f;
+  GnCh h;
+  if (lane * 8 < t.ct) gn_affine<TAIL>(p, t.n, c, h.sc, h.be);
+  __syncthreads();
   if (lane * 8 < t.ct) {
-    GnCh h;
-    gn_channels<Q8>(p, t.n, c, h);
+    gn_channels<Q8>(p, c, st, g0, h);
     const auto add = [&](const GnRow<E, Q8> &w) {
       float d[8], dz[8];
       gn_row<E, ACT, Q8>(w, h, d, dz);
@@ -519,12 +533,11 @@ __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
     float a = red[threadIdx.x];
 #pragma unroll
     for (int w = 1; w < NW; ++w) a += red[w * 2 * p.CT + threadIdx.x];
-    if (threadIdx.x & 1) a *= (float)p.stats[((long long)t.n * p.G + (t.c0 + (threadIdx.x >> 1)) / p.Cg) * 2 + 1];  // d -> xh
+    if (threadIdx.x & 1) a *= (float)st[(t.c0 + (threadIdx.x >> 1)) / p.Cg - g0].y;  // d -> xh
     red[threadIdx.x] = a;
     p.pch[(((long long)t.n * p.nchunk + t.k) * p.C + t.c0) * 2 + threadIdx.x] = a;
   }
   __syncthreads();
-  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg;
   for (int g = g0 + threadIdx.x; g <= g1; g += GN_TB) {
     const int a0 = max(g * p.Cg - t.c0, 0), a1 = min((g + 1) * p.Cg - t.c0, t.ct);
     double2 o = {0.0, 0.0};
@@ -541,30 +554,35 @@ __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
 template <class E, int ACT, bool Q8, bool TAIL>
 __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   constexpr int U = 2;
-  __shared__ double2 st[GN_CT];  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh)
+  __shared__ double2 sh[2 * GN_CT];
+  double2 *st = sh, *stats = sh + GN_CT;  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh); mean, rstd
   int b = blockIdx.x;
-  if (b < p.pblocks) {  // 8 lanes a channel: the row ranges (and samples, where the parameters are shared) in a fixed order
-    const long long idx = (long long)b * (GN_T / 8) + threadIdx.x / 8;
-    const int sub = threadIdx.x & 7;
-    const long long count = p.affn ? (long long)p.N * p.C : p.C;
+  if (b < p.pblocks) {  // 32 channels, 8 lanes each: the row ranges (and samples, where the parameters are shared) in a fixed order
+    static_assert(GN_T == 256 && 2 * GN_CT == GN_T, "a lane's sums in sh");
+    const int sub = threadIdx.x >> 5;
+    const long long idx = (long long)b * 32 + (threadIdx.x & 31), count = p.affn ? (long long)p.N * p.C : p.C;
+    double2 o = {0.0, 0.0};
     if (idx < count) {
       const int n = p.affn ? (int)(idx / p.C) : 0, c = (int)(idx % p.C);
       const long long len = (long long)(p.affn ? 1 : p.N) * p.nchunk;
-      double a = 0.0, q = 0.0;
+      const float *src = p.pch + ((long long)n * p.nchunk * p.C + c) * 2;
+#pragma unroll 8
       for (long long i = sub; i < len; i += 8) {
-        const float2 s = *reinterpret_cast<const float2 *>(p.pch + (((long long)n * p.nchunk + i) * p.C + c) * 2);
-        a += s.x;
-        q += s.y;
+        const float2 s = *reinterpret_cast<const float2 *>(src + i * p.C * 2);
+        o.x += s.x;
+        o.y += s.y;
       }
+    }
+    sh[threadIdx.x] = o;
+    __syncthreads();
+    if (threadIdx.x < 32 && idx < count) {
 #pragma unroll
-      for (int off = 4; off > 0; off >>= 1) {
-        a += __shfl_xor(a, off, 64);
-        q += __shfl_xor(q, off, 64);
+      for (int l = 1; l < 8; ++l) {
+        o.x += sh[l * 32 + threadIdx.x].x;
+        o.y += sh[l * 32 + threadIdx.x].y;
       }
-      if (sub == 0) {
-        p.dbeta[idx] = (float)a;
-        p.dgamma[idx] = (float)q;
-      }
+      p.dbeta[idx] = (float)o.x;
+      p.dgamma[idx] = (float)o.y;
     }
     return;
   }
@@ -573,7 +591,7 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   const GnTile t = gn_tile(p, b / p.nchunk / p.split * p.nchunk + b % p.nchunk);
   const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes, c = t.c0 + lane * 8;
   GnCh h;
-  gn_channels<Q8>(p, t.n, c, h);
+  if (lane * 8 < t.ct) gn_affine<TAIL>(p, t.n, c, h.sc, h.be);
   const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
   int sub = 64;
   while (sub > 1 && ng * sub > GN_T) sub >>= 1;
@@ -583,12 +601,14 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
     gn_join(p, t.n, g0 + i, threadIdx.x & (sub - 1), sub, a, q);
     const double m = (double)p.S * p.Cg;
     if ((threadIdx.x & (sub - 1)) == 0) {
-      const double rstd = p.stats[((long long)t.n * p.G + g0 + i) * 2 + 1];
+      stats[i] = *reinterpret_cast<const double2 *>(p.stats + ((long long)t.n * p.G + g0 + i) * 2);
+      const double rstd = stats[i].y;
       st[i] = {rstd * (a / m), rstd * rstd * (q / m)};
     }
   }
   __syncthreads();
   if (lane * 8 >= t.ct) return;
+  gn_channels<Q8>(p, c, stats, g0, h);
   float m1[8], m2[8];  // dx = sc dz - m1 - d m2
   {
     int g[8];
@@ -638,21 +658,22 @@ static bool gn_whole_tile(GnP &p) {
   for (int ct = 32; ct <= GN_CT; ct <<= 1)
     if ((ct % p.Cg == 0 || ct >= p.C) && p.S <= (long long)GN_R * (GN_TW / (ct / 8))) {
       gn_tiles(p, ct);
-      p.nchunk = p.split = 1;
+      p.whole = p.nchunk = p.split = 1;
       p.crows = p.arows = p.S;
       return true;
     }
   return false;
 }
 // Two launches.  Row ranges: the sums launch has at most 32 a tile (64 where the samples and tiles are few), each joined by every block of the
-// second launch that needs it; that launch cuts them into pieces for about 8 blocks a CU, of 8 rows a lane or more.
+// second launch that needs it; of 4 rows a lane or more, fewer where that leaves CUs idle.  The second launch cuts them into pieces for about
+// 8 blocks a CU, of 8 rows a lane or more, fewer for 2 blocks a CU.
 static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   if (d->S > (1 << 30) || d->C > (1 << 24)) return TBG_ERANGE;
   p.N = d->N; p.S = d->S; p.C = d->C; p.G = d->G; p.Cg = d->C / d->G; p.affn = d->per_sample ? d->C : 0;
   p.nb = (d->C + A8_BLOCK - 1) / A8_BLOCK;
   p.xn = d->xn; p.xs = d->xs; p.dn = d->dn; p.ds = d->ds; p.eps = d->eps;
   const long long count = d->per_sample ? (long long)d->N * d->C : d->C;
-  p.pblocks = (int)((count + GN_T / 8 - 1) / (GN_T / 8));
+  p.pblocks = (int)((count + 31) / 32);
   // the tile (a power of two; a row's 8-bit block never spans two) that leaves the fewest lanes without channels
   const int padded = p.nb * A8_BLOCK;
   int best = 0, tile = 0;
@@ -664,7 +685,10 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   const int RL = (backward ? GN_TB : GN_TS) / p.lanes, RA = GN_T / p.lanes;
   const long long tiles = (long long)p.N * p.ntile;
   long long want = 512 / tiles;
-  const long long cap = tiles < 8 ? 64 : 32, most = (p.S + 4LL * RL - 1) / (4LL * RL);
+  const long long cap = tiles < 8 ? 64 : 32, fill = 128 / tiles, rows_each = (p.S + RL - 1) / RL;
+  long long most = (p.S + 4LL * RL - 1) / (4LL * RL);
+  most = most > fill ? most : (rows_each < fill ? rows_each : fill);
+  if (most < 1) most = 1;
   want = want > cap ? cap : want;
   want = want > most ? most : want;
   if (want >= 8) want &= ~7LL;
@@ -672,13 +696,15 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   long long rows = (p.S + want - 1) / want;
   p.crows = (int)((rows + RL - 1) / RL * RL);
   p.nchunk = (int)((p.S + p.crows - 1LL) / p.crows);
-  long long split = GN_BLOCKS / (tiles * p.nchunk);
-  const long long least = p.crows / (8LL * RA);
+  long long split = 2048 / (tiles * p.nchunk);
+  long long least = p.crows / (8LL * RA);
+  const long long filled = 512 / (tiles * p.nchunk), pieces = p.crows / RA;
+  least = least > filled ? least : (pieces < filled ? pieces : filled);
   split = split > least ? least : split;
   if (split < 1) split = 1;
   p.arows = (int)(((p.crows + split - 1) / split + RA - 1) / RA * RA);
   p.split = (p.crows + p.arows - 1) / p.arows;
-  if (!backward && !GN_NOWHOLE) gn_whole_tile(p);
+  if (!backward) gn_whole_tile(p);
   if ((long long)p.N * p.ntile * p.nchunk * p.split > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
   return TBG_OK;
 }
@@ -697,7 +723,7 @@ template <class E, int ACT, bool Q, bool TAIL>
 static int gn_run_fwd(const GnP &p, hipStream_t st) {
   const int run = TAIL ? (p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1) : (p.Cg % 8 == 0 ? 8 : p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1);
   constexpr int A8 = TAIL ? 2 : 1;
-  if (p.nchunk == 1 && p.crows == p.S) {
+  if (p.whole) {
     const auto whole = run == 8 ? gn_whole_kernel<E, A8, ACT, Q, TAIL> : run == 4 ? gn_whole_kernel<E, 2, ACT, Q, TAIL>
                        : run == 2 ? gn_whole_kernel<E, 4, ACT, Q, TAIL> : gn_whole_kernel<E, 8, ACT, Q, TAIL>;
     hipLaunchKernelGGL(whole, dim3(p.N * p.ntile), dim3(GN_TW), 0, st, p);
