@@ -87,8 +87,11 @@ def test_entries_check_pointers_and_workspaces():
     assert fwd(p, p, p, p, None, p, None, None, None, p, 1 << 20, None) == -1        # values without scales
     assert fwd(p, p, p, p, None, None, None, p, None, p, 1 << 20, None) == -1
     assert fwd(p, p, p, p, None, odd, p, None, None, p, 1 << 20, None) == -1         # misaligned checkpoint
-    assert fwd(p, p, p, p, None, None, None, None, None, p, 8, None) == -1           # workspace too small
-    assert fwd(p, p, p, p, None, None, None, None, None, None, 1 << 20, None) == -1
+    big = C.byref(_desc(S=100000, xn=800000, dn=800000))                             # (one launch, for few positions, takes no workspace)
+    assert lib.tbg_group_norm_workspace_bytes(big, 0) > 8 and lib.tbg_group_norm_workspace_bytes(d, 0) == 0
+    assert lib.tbg_group_norm_fwd(big, p, p, p, p, None, None, None, None, None, p, 8, None) == -1         # workspace too small
+    assert lib.tbg_group_norm_fwd(big, p, p, p, p, None, None, None, None, None, None, 1 << 20, None) == -1
+    assert fwd(p, p, p, p, odd, None, None, None, None, p, 1 << 20, None) == -1      # misaligned statistics
     bwd = lambda *a: lib.tbg_group_norm_bwd(d, *a)
     assert bwd(p, p, p, p, p, p, p, p, p, p, p, 1 << 20, None) == -1                 # both the input and a checkpoint
     assert bwd(None, None, None, p, p, p, p, p, p, p, p, 1 << 20, None) == -1        # neither

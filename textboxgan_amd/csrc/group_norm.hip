@@ -708,7 +708,7 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   if ((long long)p.N * p.ntile * p.nchunk * p.split > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
   return TBG_OK;
 }
-static long long gn_part_bytes(const GnP &p) { return (long long)p.N * p.nchunk * p.nslot * 2 * (long long)sizeof(double); }
+static long long gn_part_bytes(const GnP &p) { return p.whole ? 0 : (long long)p.N * p.nchunk * p.nslot * 2 * (long long)sizeof(double); }
 static long long gn_pch_bytes(const GnP &p) { return (long long)p.N * p.nchunk * p.C * 2 * (long long)sizeof(float); }
 
 extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int backward) {
@@ -771,12 +771,12 @@ static bool gn_misaligned(const void *a, const void *b) { return ((reinterpret_c
 
 extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const float *gamma, const float *beta, void *y, double *stats,
                                   void *q, void *e, void *yq, void *ye, void *workspace, long long workspace_bytes, void *stream) {
-  if (!gn_desc_ok(d) || !x || !gamma || !beta || !y || !workspace || (q == nullptr) != (e == nullptr) || (yq == nullptr) != (ye == nullptr))
+  if (!gn_desc_ok(d) || !x || !gamma || !beta || !y || (q == nullptr) != (e == nullptr) || (yq == nullptr) != (ye == nullptr))
     return TBG_EINVAL;
   if (gn_misaligned(q, yq) || gn_misaligned(workspace, stats)) return TBG_EINVAL;
   GnP p{};
   if (const int rc = gn_geometry(d, false, p)) return rc;
-  if (gn_part_bytes(p) > workspace_bytes) return TBG_EINVAL;
+  if (gn_part_bytes(p) > (workspace ? workspace_bytes : 0)) return TBG_EINVAL;
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = y; p.stats = stats; p.part = reinterpret_cast<double *>(workspace);
   p.q = reinterpret_cast<unsigned char *>(q); p.e = reinterpret_cast<unsigned char *>(e);
   p.yq = reinterpret_cast<unsigned char *>(yq); p.ye = reinterpret_cast<unsigned char *>(ye);

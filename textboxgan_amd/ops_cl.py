@@ -48,24 +48,20 @@ class Act8(NamedTuple):
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _on:
-    """Run launches on the device of ``t`` (the current one as a rule: then nothing is switched), on its current stream."""
-    __slots__ = ("prev", "idx")
-
-    def __init__(self, t: torch.Tensor):
-        self.idx, self.prev = t.device.index, None
-
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.idx:
-            self.prev = cur
-            torch.cuda.set_device(self.idx)
-        return _raw_stream(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
-        return False
+def _call(name: str, t: torch.Tensor, *args):
+    """One C entry, on the device of ``t`` (the current one as a rule: then nothing is switched) and its current stream."""
+    fn = getattr(N.lib(), name)
+    idx, cur = t.device.index, torch.cuda.current_device()
+    if idx == cur:
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        torch.cuda.set_device(idx)
+        try:
+            rc = fn(*args, _raw_stream(idx))
+        finally:
+            torch.cuda.set_device(cur)
+    if rc:
+        N.check(rc, name)
 
 
 def _check(t, what: str, dtypes):
@@ -153,8 +149,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     q, e = _alloc8(rows, shape[-1], x.device)
     if rows:
         x, _, pitch = _rows(x)
-        with _on(x) as st:
-            N.check(N.lib().tbg_act8_pack(x.data_ptr(), _DTYPES[x.dtype], rows, shape[-1], pitch, q.data_ptr(), e.data_ptr(), st), "tbg_act8_pack")
+        _call("tbg_act8_pack", x, x.data_ptr(), _DTYPES[x.dtype], rows, shape[-1], pitch, q.data_ptr(), e.data_ptr())
     return Act8(q, e, shape, x.dtype)
 
 
@@ -167,9 +162,7 @@ def act8_unpack(a: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     _placed("act8_unpack", a.q, a.e)
     x = torch.empty(a.shape, device=a.q.device, dtype=dtype)
     if a.rows:
-        with _on(x) as st:
-            N.check(N.lib().tbg_act8_unpack(a.q.data_ptr(), a.e.data_ptr(), a.rows, a.shape[-1], x.data_ptr(), _DTYPES[dtype], a.shape[-1], st),
-                    "tbg_act8_unpack")
+        _call("tbg_act8_unpack", x, a.q.data_ptr(), a.e.data_ptr(), a.rows, a.shape[-1], x.data_ptr(), _DTYPES[dtype], a.shape[-1])
     return x
 
 
@@ -192,73 +185,86 @@ def act8_wgrad(a: Act8, dy: torch.Tensor, coef: float = 1.0, want_db: bool = Tru
     nbytes = N.lib().tbg_act8_wgrad_workspace_bytes(rows, cin, cout, dt)
     N.check(min(nbytes, 0), "tbg_act8_wgrad_workspace_bytes")
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    with _on(dy) as st:
-        N.check(N.lib().tbg_act8_wgrad(a.q.data_ptr(), a.e.data_ptr(), dy.data_ptr(), dt, rows, cin, cout, pitch, float(coef), dw.data_ptr(),
-                                       None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, st), "tbg_act8_wgrad")
+    _call("tbg_act8_wgrad", dy, a.q.data_ptr(), a.e.data_ptr(), dy.data_ptr(), dt, rows, cin, cout, pitch, float(coef), dw.data_ptr(),
+          None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return dw, db
 
 
 # ----------------------------------------------------------------------------------------
 # group norm + activation
 # ----------------------------------------------------------------------------------------
-def _gn_fwd(x, gamma, beta, groups, act, eps, want_stats, save8, sink):
-    shape = tuple(x.shape)
+_ptr = lambda t: None if t is None else t.data_ptr()
+_PLANS = {}  # arguments of a group norm call that follow from sizes, pitches and options alone: (reference to the descriptor, workspace bytes)
+
+
+def _gn_plan(backward: int, *fields):
+    key = (backward, fields)
+    plan = _PLANS.get(key)
+    if plan is None:
+        d = C.byref(N.GnDesc(*fields))
+        nbytes = N.lib().tbg_group_norm_workspace_bytes(d, backward)
+        N.check(min(nbytes, 0), "tbg_group_norm_workspace_bytes")
+        if len(_PLANS) >= 1024:
+            _PLANS.clear()
+        plan = _PLANS[key] = (d, nbytes)
+    return plan
+
+
+def _gn_fwd(x, gamma, beta, cfg, want_stats, save8, sink):
+    groups, act, eps = cfg
+    shape, dev, dtype = x.shape, x.device, x.dtype
     n, ch = shape[0], shape[-1]
-    dev = x.device
     x, xn, xs, pos = _samples(x)
-    y = torch.empty(shape, device=dev, dtype=x.dtype)
-    stats = torch.empty((n, groups, 2), device=dev, dtype=torch.float64) if want_stats else None
     rows = n * pos
+    d, nbytes = _gn_plan(0, xn, xs, xn, xs, n, pos, ch, groups, _DTYPES[dtype], act, gamma.dim() - 1, eps)
+    y = torch.empty(shape, device=dev, dtype=dtype)
+    stats = torch.empty((n, groups, 2), device=dev, dtype=torch.float64) if want_stats else None
     q, e = _alloc8(rows, ch, dev) if save8 else (None, None)
     yq, ye = _alloc8(rows, ch, dev) if sink else (None, None)
-    d = N.GnDesc(xn, xs, xn, xs, n, pos, ch, groups, _DTYPES[x.dtype], act, int(gamma.dim() == 2), eps)
-    nbytes = N.lib().tbg_group_norm_workspace_bytes(C.byref(d), 0)
-    N.check(min(nbytes, 0), "tbg_group_norm_workspace_bytes")
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    p = lambda t: None if t is None else t.data_ptr()
-    with _on(x) as st:
-        N.check(N.lib().tbg_group_norm_fwd(C.byref(d), x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), p(stats), p(q), p(e), p(yq),
-                                           p(ye), ws.data_ptr(), nbytes, st), "tbg_group_norm_fwd")
-    return y, stats, (q, e), Act8(yq, ye, shape, x.dtype) if sink else None
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    _call("tbg_group_norm_fwd", x, d, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), _ptr(stats), _ptr(q), _ptr(e), _ptr(yq),
+          _ptr(ye), _ptr(ws), nbytes)
+    return y, stats, q, e, Act8(yq, ye, tuple(shape), dtype) if sink else None
 
 
-def _gn_bwd(x, q, e, dy, gamma, beta, stats, groups, act, eps):
-    shape = tuple(dy.shape)
+def _gn_bwd(x, q, e, dy, gamma, beta, stats, cfg):
+    groups, act, eps = cfg
+    shape, dev, dtype = dy.shape, dy.device, dy.dtype
     n, ch = shape[0], shape[-1]
-    dev = dy.device
     dy, dn, ds, pos = _samples(dy)
     xn, xs = dn, ds
     if x is not None:
         x, xn, xs, _ = _samples(x)
-    dx = torch.empty(shape, device=dev, dtype=dy.dtype)
+    d, nbytes = _gn_plan(1, xn, xs, dn, ds, n, pos, ch, groups, _DTYPES[dtype], act, gamma.dim() - 1, eps)
+    dx = torch.empty(shape, device=dev, dtype=dtype)
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-    d = N.GnDesc(xn, xs, dn, ds, n, pos, ch, groups, _DTYPES[dy.dtype], act, int(gamma.dim() == 2), eps)
-    nbytes = N.lib().tbg_group_norm_workspace_bytes(C.byref(d), 1)
-    N.check(min(nbytes, 0), "tbg_group_norm_workspace_bytes")
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    p = lambda t: None if t is None else t.data_ptr()
-    with _on(dy) as st:
-        N.check(N.lib().tbg_group_norm_bwd(C.byref(d), p(x), p(q), p(e), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(),
-                                           dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), nbytes, st), "tbg_group_norm_bwd")
+    _call("tbg_group_norm_bwd", dy, d, _ptr(x), _ptr(q), _ptr(e), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), dx.data_ptr(),
+          dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), nbytes)
     return dx, dgamma, dbeta
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, beta, groups, act, eps, save8, sink, box):
-        y, stats, (q, e), y8 = _gn_fwd(x, gamma, beta, groups, act, eps, True, save8, sink)
-        ctx.save_for_backward(None if save8 else x, q, e, gamma, beta, stats)
-        ctx.cfgv = (groups, act, eps)
-        box.append(y8)
+    def forward(ctx, x, gamma, beta, cfg, save8, sink, box):
+        y, stats, q, e, y8 = _gn_fwd(x, gamma, beta, cfg, True, save8, sink)
+        if save8:
+            ctx.save_for_backward(gamma, beta, stats, q, e)
+        else:
+            ctx.save_for_backward(gamma, beta, stats, x)
+        ctx.cfg = cfg
+        if sink:
+            box.append(y8)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, q, e, gamma, beta, stats = ctx.saved_tensors
-        dx, dgamma, dbeta = _gn_bwd(x, q, e, dy, gamma, beta, stats, *ctx.cfgv)
+        gamma, beta, stats, *kept = ctx.saved_tensors
+        x, q, e = (None, *kept) if len(kept) == 2 else (kept[0], None, None)
+        dx, dgamma, dbeta = _gn_bwd(x, q, e, dy, gamma, beta, stats, ctx.cfg)
         need = ctx.needs_input_grad
-        return dx if need[0] else None, dgamma if need[1] else None, dbeta if need[2] else None, None, None, None, None, None, None
+        return dx if need[0] else None, dgamma if need[1] else None, dbeta if need[2] else None, None, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups: int, act: str = "linear", eps: float = 1e-5,
@@ -291,14 +297,13 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
         y = x * gamma.sum() * beta.sum() if grad else torch.empty(x.shape, device=x.device, dtype=x.dtype)
         y = y.to(x.dtype)
         return (y, Act8(*_alloc8(0, ch, x.device), tuple(x.shape), x.dtype)) if sink else y
-    gamma, beta = gamma.contiguous(), beta.contiguous()
+    gamma, beta, cfg = gamma.contiguous(), beta.contiguous(), (groups, ACTS[act], float(eps))
     if not grad:
-        y, _, _, y8 = _gn_fwd(x, gamma, beta, groups, ACTS[act], float(eps), False, False, sink)
-    else:
-        box = []
-        y = _GroupNormAct.apply(x, gamma, beta, groups, ACTS[act], float(eps), save == "act8", sink, box)
-        y8 = box[0]
-    return (y, y8) if sink else y
+        y, *_, y8 = _gn_fwd(x, gamma, beta, cfg, False, False, sink)
+        return (y, y8) if sink else y
+    box = []
+    y = _GroupNormAct.apply(x, gamma, beta, cfg, save == "act8", sink, box)
+    return (y, box[0]) if sink else y
 
 
 # ----------------------------------------------------------------------------------------
