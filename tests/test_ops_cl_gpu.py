@@ -267,7 +267,8 @@ def test_runs_repeat_bit_for_bit(dev):
 
 # ---------------------------------------------------------------------------------------- weight gradient
 WSHAPES = [(1, 1, 1), (1, 32, 8), (3, 33, 5), (31, 64, 64), (32, 65, 72), (100, 128, 128), (129, 200, 72), (500, 17, 300), (1000, 256, 256), (4099, 200, 72),
-           (2048, 512, 40), (777, 40, 512), (2000, 520, 264), (300, 1, 1000), (300, 1000, 1)]
+           (2048, 512, 40), (777, 40, 512), (2000, 520, 264), (300, 1, 1000), (300, 1000, 1),
+           (16400, 512, 512), (20011, 384, 264), (16400, 400, 512), (66000, 256, 144)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)

@@ -29,17 +29,45 @@ struct A8wP {
 
 constexpr int A8W_RB = 32, A8W_PAD = 32;  // rows a stage; elements between two LDS rows (the 4 rows x 64 B of two transposing reads: all 64 banks)
 
-// the bf16 terms of dy, largest first, by truncation: every remainder is exact and nothing overflows
+// the bf16 terms of 8 values of dy, largest first, by truncation: every remainder is exact and nothing overflows (an infinity leaves NaN behind)
 template <int NP>
-__device__ __forceinline__ void a8w_terms(float v, unsigned short (&t)[NP]) {
-  const bool fine = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
-  float rest = v;
+__device__ __forceinline__ void a8w_terms(const float (&v)[8], Pack8<ElBf16> (&w)[NP]) {
+  float rest[8];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const unsigned hi = __float_as_uint(rest) & 0xffff0000u;
-    t[i] = fine ? (unsigned short)(hi >> 16) : (i == 0 ? ElBf16::put(v) : (unsigned short)0);
-    rest -= __uint_as_float(hi);
+  for (int j = 0; j < 8; ++j) rest[j] = v[j];
+#pragma unroll
+  for (int m = 0; m < NP; ++m) {
+    unsigned u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * j + 1]), __float_as_uint(rest[2 * j]), 0x07060302u);
+    __builtin_memcpy(&w[m], u, 16);
+    if (m + 1 < NP) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rest[j] -= __uint_as_float(__float_as_uint(rest[j]) & 0xffff0000u);
+    }
   }
+}
+
+// a wave's products: entry (8 (r / 4) + 4 (lane / 32) + r % 4, lane % 32) of each 32 x 32 in register r
+template <int WM, int WN>
+__device__ __forceinline__ void a8w_store(const A8wP &p, const f32x16 (&acc)[WM][WN], int z, int k, int n, bool whole, int lane) {
+  float *out = p.out + (long long)z * p.cin * p.cout;
+  const float f = p.nsplit == 1 ? p.coef : 1.f;
+  const int kl = k + 4 * (lane >> 5), nl = n + (lane & 31);
+#pragma unroll
+  for (int i = 0; i < WM; ++i)
+#pragma unroll
+    for (int j = 0; j < WN; ++j) {
+      float *o = out + (long long)(kl + 32 * i) * p.cout + nl + 32 * j;
+      if (whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[(8 * (r >> 2) + (r & 3)) * (long long)p.cout] = f * acc[i][j][r];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kl + 32 * i + 8 * (r >> 2) + (r & 3) < p.cin && nl + 32 * j < p.cout) o[(8 * (r >> 2) + (r & 3)) * (long long)p.cout] = f * acc[i][j][r];
+      }
+    }
 }
 
 // KW x NW waves of WM x WN products of 32 x 32.  Three LDS buffers and one barrier a stage: while the block multiplies stage t it writes stage
@@ -139,13 +167,10 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
       if constexpr (NP == 1) {
         __builtin_memcpy(&w[0], &g.dv[i], 16);
       } else {
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          unsigned short t[NP];
-          a8w_terms<NP>(E::get(g.dv[i].v[j]), t);
-#pragma unroll
-          for (int m = 0; m < NP; ++m) w[m].v[j] = t[m];
-        }
+        for (int j = 0; j < 8; ++j) v[j] = E::get(g.dv[i].v[j]);
+        a8w_terms<NP>(v, w);
       }
 #pragma unroll
       for (int m = 0; m < NP; ++m) st8<ElBf16>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
@@ -234,24 +259,7 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
     __syncthreads();
   }
 
-  float *out = p.out + (long long)z * p.cin * p.cout;
-  const float f = p.nsplit == 1 ? p.coef : 1.f;
-  const bool whole = k0 + TK <= p.cin && n0 + TN <= p.cout;
-  const int kl = k0 + wk * 32 * WM + 4 * (lane >> 5), nl = n0 + wn * 32 * WN + (lane & 31);
-#pragma unroll
-  for (int i = 0; i < WM; ++i)
-#pragma unroll
-    for (int j = 0; j < WN; ++j) {
-      float *o = out + (long long)(kl + 32 * i) * p.cout + nl + 32 * j;
-      if (whole) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[(8 * (r >> 2) + (r & 3)) * (long long)p.cout] = f * acc[i][j][r];
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (kl + 32 * i + 8 * (r >> 2) + (r & 3) < p.cin && nl + 32 * j < p.cout) o[(8 * (r >> 2) + (r & 3)) * (long long)p.cout] = f * acc[i][j][r];
-      }
-    }
+  a8w_store<WM, WN>(p, acc, z, k0 + wk * 32 * WM, n0 + wn * 32 * WN, k0 + TK <= p.cin && n0 + TN <= p.cout, lane);
   if (do_db) {
     float *red = reinterpret_cast<float *>(smem);  // [T][8]; every wave is past its last operand read
 #pragma unroll
@@ -325,10 +333,15 @@ static int a8w_args(long long rows, int cin, int cout, int dtype) {
   return TBG_OK;
 }
 
+// partial sums: products of every split, then column sums of every split
+static long long a8w_workspace(const A8wGeo &g, int cin, int cout) {
+  return g.nsplit == 1 ? 0 : (long long)g.nsplit * ((long long)cin * cout + cout) * (long long)sizeof(float);
+}
+
 extern "C" long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int cout, int dtype) {
   if (const int rc = a8w_args(rows, cin, cout, dtype)) return rc;
   const A8wGeo g = a8w_geometry(rows, cin, cout, dtype);
-  return g.nsplit == 1 ? 0 : (long long)g.nsplit * ((long long)cin * cout + cout) * (long long)sizeof(float);
+  return a8w_workspace(g, cin, cout);
 }
 
 template <class E, int NP, int WM, int WN, int KW, int NW>
@@ -362,7 +375,7 @@ extern "C" int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int 
   if (ldy > (1LL << 26)) return TBG_ERANGE;
   const A8wGeo g = a8w_geometry(rows, cin, cout, dtype);
   if ((long long)(g.nsplit + 7) * g.tk * g.tn > 0x7fffffffLL) return TBG_ERANGE;
-  const long long kn = (long long)cin * cout, need = g.nsplit == 1 ? 0 : g.nsplit * (kn + cout) * (long long)sizeof(float);
+  const long long kn = (long long)cin * cout, need = a8w_workspace(g, cin, cout);
   if (need > workspace_bytes || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))) return TBG_EINVAL;
   A8wP p{};
   p.q = reinterpret_cast<const unsigned char *>(q); p.e = reinterpret_cast<const unsigned char *>(e); p.dy = dy;
