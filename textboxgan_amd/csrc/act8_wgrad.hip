@@ -273,15 +273,15 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
   }
 }
 
-// dw = coef sum of the splits' products, db = sum of theirs.  A lane takes V neighbouring entries; the 4 waves of a block every fourth split of
-// the same entries each, joined through LDS: the loads are what there is to wait for, and small products have few entries.
+// dw = coef sum of the splits' products, db = sum of theirs.  A lane takes V neighbouring entries; `ranks` lanes (4 to 64) take every ranks-th
+// split of the same entries each, joined through LDS: the loads are what there is to wait for, and small products have few entries.
 template <int V>
 __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, const float *dbws, float *dw, float *db, long long kn, int cout,
-                                                              int nsplit, float coef) {
+                                                              int nsplit, int ranks, float coef) {
   typedef float vec __attribute__((ext_vector_type(V)));
   __shared__ vec red[256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  long long i = ((long long)blockIdx.x * 64 + lane) * V;
+  const int wide = 256 / ranks, lane = threadIdx.x & (wide - 1), rank = threadIdx.x / wide;
+  long long i = ((long long)blockIdx.x * wide + lane) * V;
   const bool bias = i >= kn;
   if (bias) i -= kn;
   const bool live = !bias || (db && i < cout);
@@ -292,16 +292,18 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, c
   for (int j = 0; j < V; ++j) a[j] = 0.f;
   if (live) {
 #pragma unroll 8
-    for (int z = wave; z < nsplit; z += 4) a += *reinterpret_cast<const vec *>(src + z * len);
+    for (int z = rank; z < nsplit; z += ranks) a += *reinterpret_cast<const vec *>(src + z * len);
   }
   red[threadIdx.x] = a;
-  __syncthreads();
-  if (wave == 0 && live)
-    *reinterpret_cast<vec *>((bias ? db : dw) + i) = (bias ? 1.f : coef) * ((red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]));
+  for (int half = ranks >> 1; half > 0; half >>= 1) {
+    __syncthreads();
+    if (rank < half) red[threadIdx.x] += red[threadIdx.x + half * wide];
+  }
+  if (rank == 0 && live) *reinterpret_cast<vec *>((bias ? db : dw) + i) = (bias ? 1.f : coef) * red[threadIdx.x];
 }
 
 // Tile and row splits.  The tile: the largest that the channels fill (fewer re-reads of both operands, fewer operand reads an MFMA), made
-// smaller while the launch would have less than a block a CU with splits of 256 rows; the splits then fill the card once.
+// smaller while splits of 256 rows would leave a quarter of the CUs without a block; the splits then fill the card once.
 struct A8wGeo {
   int form, tk, tn, nsplit;
   long long rsplit;
@@ -316,7 +318,7 @@ static A8wGeo a8w_geometry(long long rows, int cin, int cout, int dtype) {
   for (g.form = cin > 128 && cout > 128 && dtype == TBG_DT_BF16 ? 0 : cin > 64 ? (cout > 64 ? 1 : 2) : (cout > 64 ? 3 : 4);; g.form = g.form == 0 ? 1 : 4) {
     g.tk = (cin + A8W_FORMS[g.form].tk - 1) / A8W_FORMS[g.form].tk;
     g.tn = (cout + A8W_FORMS[g.form].tn - 1) / A8W_FORMS[g.form].tn;
-    if ((long long)g.tk * g.tn * most >= 256 || g.form == 4) break;
+    if ((long long)g.tk * g.tn * most >= 192 || g.form == 4) break;
   }
   long long want = 256LL * A8W_FORMS[g.form].per_cu / ((long long)g.tk * g.tn);
   const long long cap = g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
@@ -392,8 +394,10 @@ extern "C" int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int 
   if (rc || g.nsplit == 1) return rc;
   const bool v4 = cout % 4 == 0 && ((reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(db)) & 15) == 0;
   const long long lanes = (kn + (db ? cout : 0) + (v4 ? 3 : 0)) / (v4 ? 4 : 1);
-  hipLaunchKernelGGL(v4 ? act8_wgrad_join_kernel<4> : act8_wgrad_join_kernel<1>, dim3((unsigned)((lanes + 63) / 64)), dim3(256), 0, st, ws,
-                     ws + g.nsplit * kn, dw, db, kn, cout, g.nsplit, coef);
+  int ranks = 4;  // more while the launch has less than a block a CU
+  while (ranks < 64 && ranks < g.nsplit && lanes * ranks < 256 * 256) ranks <<= 1;
+  hipLaunchKernelGGL(v4 ? act8_wgrad_join_kernel<4> : act8_wgrad_join_kernel<1>, dim3((unsigned)((lanes * ranks + 255) / 256)), dim3(256), 0, st, ws,
+                     ws + g.nsplit * kn, dw, db, kn, cout, g.nsplit, ranks, coef);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }

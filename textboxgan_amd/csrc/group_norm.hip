@@ -181,17 +181,26 @@ __device__ __forceinline__ void gn_block_sums(const GnP &p, double (&s1)[A], dou
   }
   __syncthreads();
 }
-// ... of the part of group g that lies in the tile
-template <int A>
-__device__ __forceinline__ double2 gn_group_sums(const GnP &p, const GnTile &t, int g, const double *red) {
-  constexpr int step = 8 / A;
-  const int a0 = max(g * p.Cg - t.c0, 0) / step, a1 = min((g + 1) * p.Cg - t.c0, t.ct) / step;
-  double2 o = {0.0, 0.0};
-  for (int c = a0; c < a1; ++c) {
-    o.x += red[c * 2];
-    o.y += red[c * 2 + 1];
+// sums over the part of each of the tile's ng groups (from g0 on) that lies in it, of red's pairs (one for each `step` channels), by as many
+// lanes a group as the block has; done(group - g0, sum) in one lane of each
+template <int T, class F>
+__device__ __forceinline__ void gn_group_sums(const GnP &p, const GnTile &t, int g0, int ng, int step, const double *red, F done) {
+  int sub = 64;
+  while (sub > 1 && ng * sub > T) sub >>= 1;
+  const int i = threadIdx.x / sub, l = threadIdx.x & (sub - 1);
+  if (i < ng) {
+    const int g = g0 + i, a0 = max(g * p.Cg - t.c0, 0) / step, a1 = min((g + 1) * p.Cg - t.c0, t.ct) / step;
+    double2 o = {0.0, 0.0};
+    for (int c = a0 + l; c < a1; c += sub) {
+      o.x += red[c * 2];
+      o.y += red[c * 2 + 1];
+    }
+    for (int off = sub >> 1; off > 0; off >>= 1) {
+      o.x += __shfl_xor(o.x, off, 64);
+      o.y += __shfl_xor(o.y, off, 64);
+    }
+    if (l == 0) done(i, o);
   }
-  return o;
 }
 __device__ __forceinline__ double2 gn_stats(const GnP &p, double a, double q) {  // mean, rstd
   const double m = (double)p.S * p.Cg, mean = a / m, var = q / m - mean * mean;
@@ -226,9 +235,10 @@ __global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
     }
   }
   gn_block_sums<A, GN_TS>(p, s1, s2, red);
-  const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg;
-  for (int g = g0 + threadIdx.x; g <= g1; g += GN_TS)
-    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = gn_group_sums<A>(p, t, g, red);
+  const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
+  gn_group_sums<GN_TS>(p, t, g0, ng, 8 / A, red, [&](int i, const double2 &o) {
+    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g0 + i) * 2) = o;
+  });
 }
 
 // gamma and beta of a lane's channels, zeros beyond the last
@@ -385,11 +395,10 @@ __global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
   }
   gn_block_sums<A, GN_TW>(p, s1, s2, red);
   const int g0 = t.c0 / p.Cg, ng = (t.ct + p.Cg - 1) / p.Cg;
-  if (threadIdx.x < ng) {
-    const double2 s = gn_group_sums<A>(p, t, g0 + threadIdx.x, red);
-    st[threadIdx.x] = gn_stats(p, s.x, s.y);
-    if (p.stats) *reinterpret_cast<double2 *>(p.stats + ((long long)t.n * p.G + g0 + threadIdx.x) * 2) = st[threadIdx.x];
-  }
+  gn_group_sums<GN_TW>(p, t, g0, ng, 8 / A, red, [&](int i, const double2 &o) {
+    st[i] = gn_stats(p, o.x, o.y);
+    if (p.stats) *reinterpret_cast<double2 *>(p.stats + ((long long)t.n * p.G + g0 + i) * 2) = st[i];
+  });
   __syncthreads();
   if (out.c >= p.nb * A8_BLOCK || (!Q && !out.in)) return;
   out.stats(reinterpret_cast<const double *>(st), g0);
@@ -481,6 +490,7 @@ template <class E, int ACT, bool Q8, bool TAIL>
 __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
   constexpr int U = 2, NW = GN_TB / 64;
   __shared__ float red[NW * GN_CT * 2];
+  __shared__ double gred[GN_CT * 2];  // times gamma
   __shared__ double2 st[GN_CT];  // mean, rstd of the tile's groups
   const GnTile t = gn_tile(p, blockIdx.x);
   const int g0 = t.c0 / p.Cg, g1 = (t.c0 + t.ct - 1) / p.Cg;
@@ -533,21 +543,15 @@ __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
     float a = red[threadIdx.x];
 #pragma unroll
     for (int w = 1; w < NW; ++w) a += red[w * 2 * p.CT + threadIdx.x];
-    if (threadIdx.x & 1) a *= (float)st[(t.c0 + (threadIdx.x >> 1)) / p.Cg - g0].y;  // d -> xh
-    red[threadIdx.x] = a;
+    const int j = threadIdx.x >> 1;
+    if (threadIdx.x & 1) a *= (float)st[(t.c0 + j) / p.Cg - g0].y;  // d -> xh
     p.pch[(((long long)t.n * p.nchunk + t.k) * p.C + t.c0) * 2 + threadIdx.x] = a;
+    gred[threadIdx.x] = (double)p.gamma[(long long)t.n * p.affn + t.c0 + j] * (double)a;
   }
   __syncthreads();
-  for (int g = g0 + threadIdx.x; g <= g1; g += GN_TB) {
-    const int a0 = max(g * p.Cg - t.c0, 0), a1 = min((g + 1) * p.Cg - t.c0, t.ct);
-    double2 o = {0.0, 0.0};
-    for (int j = a0; j < a1; ++j) {
-      const double ga = p.gamma[(long long)t.n * p.affn + t.c0 + j];
-      o.x = fma(ga, (double)red[j * 2], o.x);
-      o.y = fma(ga, (double)red[j * 2 + 1], o.y);
-    }
-    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g) * 2) = o;
-  }
+  gn_group_sums<GN_TB>(p, t, g0, g1 - g0 + 1, 1, gred, [&](int i, const double2 &o) {
+    *reinterpret_cast<double2 *>(p.part + (((long long)t.n * p.nchunk + t.k) * p.nslot + t.tile + g0 + i) * 2) = o;
+  });
 }
 
 // ---- backward, second launch: dx, and in its first blocks dgamma / dbeta
