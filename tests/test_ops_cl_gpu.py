@@ -206,6 +206,21 @@ def test_group_norm_far_from_zero(dev, act):
             check(dg, o["dgamma"], o["dgamma_amp"], SUMS, "dgamma")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_group_norm_of_extreme_values(dev, dtype):
+    """a position filled with the type's lowest value, and values at both ends of the type's range"""
+    for fill in (torch.finfo(dtype).min, torch.finfo(dtype).max / 4, torch.finfo(dtype).tiny):
+        x = values((2, 200, 64), dtype, dev, 18)
+        x[1, 7] = fill
+        if fill > 0:
+            x[0] = (x[0].double() / x[0].double().abs().max() * fill).to(dtype)
+        gamma, beta = affine(2, 64, False, dev)
+        with torch.no_grad():
+            y = ops_cl.group_norm_act(x, gamma, beta, 4, act="silu")
+        o = R.group_norm(x, gamma, beta, 4, "silu", 1e-5)
+        check(y, o["y"], o["y_amp"], ARITH, f"fill {fill}")
+
+
 def test_group_norm_of_constant_groups(dev):
     for dtype in TYPES:
         x = torch.full((2, 20, 32), 3.0, device=dev, dtype=dtype)
@@ -457,6 +472,28 @@ def test_captured_and_replayed(dev):
         for a, b in got:
             assert torch.equal(a, ye.detach()) and all(torch.equal(u, v) for u, v in zip(b, ge)), k
         assert torch.isfinite(other).all()
+
+
+def test_captured_weight_gradients(dev):
+    """every form of the weight gradient in a graph, replayed with new inputs between eager calls"""
+    cases = [(values((r, i), torch.float32, dev, 100 + k), values((r, o), t, dev, 110 + k)) for k, (r, i, o, t) in enumerate(
+        [(16400, 512, 512, torch.bfloat16), (9000, 256, 200, torch.float32), (5000, 70, 130, torch.float16), (40, 33, 7, torch.float32)])]
+    static = [(ops_cl.act8_pack(x), dy.clone()) for x, dy in cases]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out = [ops_cl.act8_wgrad(a, dy) for a, dy in static]
+    for k in range(3):
+        for (a, dy), (x, y) in zip(static, cases):
+            new = ops_cl.act8_pack(x * (1 + k))
+            a.q.copy_(new.q)
+            a.e.copy_(new.e)
+            dy.copy_(y * (2 - k))
+        g.replay()
+        want = [ops_cl.act8_wgrad(a, dy) for a, dy in static]
+        torch.cuda.synchronize()
+        for got, ref in zip(out, want):
+            assert all(torch.equal(u, v) for u, v in zip(got, ref)), k
 
 
 def test_on_another_stream(dev):

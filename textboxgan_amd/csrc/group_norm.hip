@@ -9,8 +9,8 @@
 // leaves partial sums per (sample, row range, tile, group), the second launch joins those of its groups in a fixed order (no atomics) and
 // writes the result.
 //
-// The statistics are 64-bit sums of x and x^2: one pass, and mean(x^2) - mean^2 loses nothing that matters for fp32 values of
-// |mean| = 10^5 standard deviations, nor for 16-bit ones, which do not resolve more than 2^11 of them.  The mean is used as fp32 + its remainder.
+// The statistics are 64-bit sums of x and x^2 (the card adds fp64 about as fast as unpacked fp32, so a streaming pass hardly notices): one pass,
+// mean(x^2) - mean^2 loses nothing that matters even where |mean| is 10^5 standard deviations, and no value of any type overflows.  The mean is used as fp32 + its remainder.
 #include "act8.h"
 
 struct GnP {
@@ -124,35 +124,14 @@ __device__ __forceinline__ void gn_join(const GnP &p, int n, int g, int lane, in
   }
 }
 
-// ---- forward: sums of x and x^2.  8 / A neighbouring channels share a group (A accumulators a lane).
-// 16-bit types: up to 8 values and squares are added in fp32 before they are in fp64 (values of 8 or 11 bits within 13 or 10 binades: the
-// first sum is exact; the second is off by 2^-24 at most, at random over the sums of a group)
-template <class E, int A, int ROWS>
-__device__ __forceinline__ void gn_add(const Pack8<E> *v, double (&s1)[A], double (&s2)[A]) {
+// ---- forward: sums of x and x^2, in fp64 from the first addition on.  8 / A neighbouring channels share a group (A accumulators a lane)
+template <class E, int A>
+__device__ __forceinline__ void gn_add(const Pack8<E> &v, double (&s1)[A], double (&s2)[A]) {
 #pragma unroll
-  for (int a = 0; a < A; ++a) {
-    if constexpr (E::BYTES == 2) {
-      float t1 = 0.f, t2 = 0.f;
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int i = a * 8 / A; i < (a + 1) * 8 / A; ++i) {
-          const float d = E::get(v[u].v[i]);
-          t1 += d;
-          t2 = fmaf(d, d, t2);
-        }
-      s1[a] += (double)t1;
-      s2[a] += (double)t2;
-    } else {
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int i = a * 8 / A; i < (a + 1) * 8 / A; ++i) {
-          const double d = E::get(v[u].v[i]);
-          s1[a] += d;
-          s2[a] = fma(d, d, s2[a]);
-        }
-    }
+  for (int i = 0; i < 8; ++i) {
+    const double d = E::get(v.v[i]);
+    s1[i * A / 8] += d;
+    s2[i * A / 8] = fma(d, d, s2[i * A / 8]);
   }
 }
 // a block's sums of each 8 / A channels of the tile, in red[2 c], red[2 c + 1]: rows of a wave by lane exchanges, the waves through LDS
@@ -209,7 +188,7 @@ __device__ __forceinline__ double2 gn_stats(const GnP &p, double a, double q) { 
 
 template <class E, int A, bool TAIL>
 __global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
-  constexpr int U = 4, B = A < U ? A : U;  // rows loaded at a time, rows added up before fp64
+  constexpr int U = 4;  // rows under way
   __shared__ double red[GN_TS / 64 * (GN_CT / 8) * A * 2];
   const GnTile t = gn_tile(p, blockIdx.x);
   const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TS / p.lanes;
@@ -227,12 +206,9 @@ __global__ __launch_bounds__(GN_TS) void gn_sums_kernel(GnP p) {
 #pragma unroll
       for (int u = 0; u < U; ++u, x += step) v[u] = row.load(x);
 #pragma unroll
-      for (int u = 0; u < U; u += B) gn_add<E, A, B>(v + u, s1, s2);
+      for (int u = 0; u < U; ++u) gn_add<E, A>(v[u], s1, s2);
     }
-    for (; r < r1; r += RL, x += step) {
-      const Pack8<E> v = row.load(x);
-      gn_add<E, A, 1>(&v, s1, s2);
-    }
+    for (; r < r1; r += RL, x += step) gn_add<E, A>(row.load(x), s1, s2);
   }
   gn_block_sums<A, GN_TS>(p, s1, s2, red);
   const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
@@ -391,7 +367,7 @@ __global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
   out.affine(t.n);
   if (out.in) {
 #pragma unroll
-    for (int u = 0; u < GN_R; ++u) gn_add<E, A, 1>(v + u, s1, s2);  // (rows that do not exist are zeros)
+    for (int u = 0; u < GN_R; ++u) gn_add<E, A>(v[u], s1, s2);  // (rows that do not exist are zeros)
   }
   gn_block_sums<A, GN_TW>(p, s1, s2, red);
   const int g0 = t.c0 / p.Cg, ng = (t.ct + p.Cg - 1) / p.Cg;
