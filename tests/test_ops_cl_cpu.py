@@ -43,6 +43,13 @@ BAD = native.TbgError
     (lambda: _gn(gamma=torch.ones(2, 8)), "have to be"),
     (lambda: _gn(gamma=torch.ones(3, 8), beta=torch.ones(3, 8)), "have to be"),
     (lambda: _gn(), "device tensors"),
+    (lambda: ops_cl.act8_unpack(ops_cl.Act8(torch.zeros(0, 0, dtype=torch.int8), torch.zeros(0, 0, dtype=torch.uint8), (), torch.float32)), "is wanted"),
+    (lambda: ops_cl.act8_pack(torch.zeros(1, 1).expand(1, 2 ** 32 + 8)), "channels, at most"),
+    (lambda: ops_cl.act8_wgrad(_a8((2, 2 ** 20 + 1)), torch.zeros(2, 8)), "channels, at most"),
+    (lambda: ops_cl.act8_wgrad(_a8((2, 8)), torch.zeros(1, 1).expand(2, 2 ** 32 + 1)), "channels, at most"),
+    (lambda: _gn(x=torch.zeros(1, 1, 8).expand(1, 2 ** 32 + 3, 8)), "positions, at most"),
+    (lambda: _gn(x=torch.zeros(1, 1, 8).expand(2 ** 32 + 3, 1, 8)), "samples, at most"),
+    (lambda: _gn(x=torch.zeros(1, 1, 1).expand(1, 1, 2 ** 32 + 8)), "channels, at most"),
     (lambda: ops_cl.dense_act8(torch.zeros(2, 8), torch.zeros(7, 4)), "do not fit"),
     (lambda: ops_cl.dense_act8(torch.zeros(2, 8), torch.zeros(8, 4, dtype=torch.float16)), "w: unsupported dtype"),
     (lambda: ops_cl.dense_act8(torch.zeros(2, 8), torch.zeros(8, 4), torch.zeros(5)), "bias"),
@@ -101,6 +108,11 @@ def test_entries_check_pointers_and_workspaces():
     assert lib.tbg_act8_pack(p, 0, 4, 8, 8, odd, p, None) == -1 and lib.tbg_act8_pack(None, 0, 4, 8, 8, p, p, None) == -1
     assert lib.tbg_act8_unpack(p, p, 0, 8, p, 0, 8, None) == -1 and lib.tbg_act8_unpack(p, None, 4, 8, p, 0, 8, None) == -1
     assert lib.tbg_act8_pack(p, 0, 1 << 38, 64, 64, p, p, None) == -2
+    # launches of 2^32 threads
+    for kw, backward in ((dict(N=1 << 24, S=1), 0), (dict(N=1 << 24, S=1), 1), (dict(N=1 << 13, S=1, C=1 << 17), 0), (dict(N=1 << 30, S=5), 1)):
+        wide = dict(xs=kw.get("C", 8), ds=kw.get("C", 8), **kw)
+        assert lib.tbg_group_norm_workspace_bytes(C.byref(_desc(**wide)), backward) == -2, kw
+    assert lib.tbg_act8_wgrad_workspace_bytes(1 << 10, 1 << 16, 1 << 15, 1) >= 0
     ws = lib.tbg_act8_wgrad_workspace_bytes(1 << 16, 256, 256, 1)
     assert ws > 0 and lib.tbg_act8_wgrad_workspace_bytes(1, 1, 1, 0) == 0
     assert lib.tbg_act8_wgrad_workspace_bytes(0, 1, 1, 0) == -1 and lib.tbg_act8_wgrad_workspace_bytes(1, 1, 1, 3) == -1

@@ -97,6 +97,23 @@ def test_pack_beyond_32_bit_offsets(dev):
         assert torch.equal(y[r].double(), R.unpack(q, e, x[r].shape))
 
 
+def test_pack_of_more_rows_than_a_launch_takes(dev):
+    """2^30 + 70 rows of one channel: 2^32 lanes and some"""
+    rows = (1 << 30) + 70
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    x = torch.ones((rows, 1), dtype=torch.float16, device=dev)
+    at = [0, 1, (1 << 29) - 1, 1 << 29, (1 << 30) - 1, 1 << 30, rows - 1]
+    for k, r in enumerate(at):
+        x[r] = k - 2.5
+    a = ops_cl.act8_pack(x)
+    q, e = R.pack(x[at])
+    assert torch.equal(a.q[at], q) and torch.equal(a.e[at], e)
+    assert int(a.q[:, 0].view(-1, 2).eq(64).sum()) >= rows - 2 * len(at)
+    back = ops_cl.act8_unpack(a)
+    assert torch.equal(back, x)
+
+
 def test_empty_tensors(dev):
     for shape in ((0, 40), (3, 0, 40)):
         x = torch.zeros(shape, device=dev, dtype=torch.bfloat16)
@@ -472,6 +489,46 @@ def test_captured_and_replayed(dev):
         for a, b in got:
             assert torch.equal(a, ye.detach()) and all(torch.equal(u, v) for u, v in zip(b, ge)), k
         assert torch.isfinite(other).all()
+
+
+def test_a_backward_pass_is_not_captured_over_an_eager_graph(dev):
+    """leaves that an eager graph of the default stream holds: the capture is refused while it lives, and works once it is gone"""
+    p = block_params(1, 64, 32, dev)
+    x, dy = values((1, 50, 64), torch.bfloat16, dev, 52), values((1, 50, 64), torch.bfloat16, dev, 53)
+    want = torch.autograd.grad(block(x, p), p, dy)
+    eager = block(x, p)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(native.TbgError, match="is alive"):
+        with torch.cuda.graph(g):
+            block(x, p)
+    with torch.no_grad():  # no backward pass: nothing to refuse
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = block(x, p)
+    g.replay()
+    assert torch.equal(y, eager.detach())
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        grads = torch.autograd.grad(block(x, p), p, dy)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_under_autocast(dev):
+    """types are the operands' own, whatever the caller's autocast"""
+    p = block_params(2, 64, 48, dev)
+    for dtype in (torch.float32, torch.bfloat16):
+        x, dy = values((2, 30, 64), dtype, dev, 54), values((2, 30, 64), dtype, dev, 55)
+        want_y = block(x, p)
+        want = torch.autograd.grad(want_y, p, dy)
+        with torch.autocast("cuda", dtype=torch.float16):
+            y = block(x, p)
+        got = torch.autograd.grad(y, p, dy)
+        assert y.dtype == dtype and torch.equal(y, want_y) and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_captured_weight_gradients(dev):

@@ -53,21 +53,25 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(const unsigned char *_
 static int act8_args(const void *x, const void *q, const void *e, int dtype, long long rows, int ch, long long ldx) {
   if (!x || !q || !e || !dt_valid(dtype) || rows < 1 || ch < 1 || ldx < ch) return TBG_EINVAL;
   if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return TBG_EINVAL;
-  if (ch > (1 << 24)) return TBG_ERANGE;
+  if (ch > (1 << 24) || rows > (1LL << 39) / ((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK)) return TBG_ERANGE;
   return TBG_OK;
 }
 
+// rows a launch: a grid holds less than 2^32 threads
+static long long act8_rows(unsigned cols) { return (1LL << 31) / cols; }
+
 template <class E>
 static int launch_pack(const void *x, long long rows, int ch, long long ldx, void *q, void *e, hipStream_t st) {
-  const unsigned padded = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK);
-  const unsigned cols = padded / 8;
-  const long long blocks = (rows * cols + 255) / 256;
-  if (rows > (1LL << 39) / padded || blocks > 0x7fffffffLL) return TBG_ERANGE;
-  auto *xp = reinterpret_cast<const typename E::type *>(x);
-  auto *qp = reinterpret_cast<unsigned char *>(q), *ep = reinterpret_cast<unsigned char *>(e);
-  hipLaunchKernelGGL((ch % 8 ? act8_pack_kernel<E, true> : act8_pack_kernel<E, false>), dim3((unsigned)blocks), dim3(256), 0, st, xp, rows, ch, ldx,
-                     qp, ep, cols);
-  TBG_LAUNCH_CHECK();
+  const unsigned cols = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * (A8_BLOCK / 8));
+  const long long most = act8_rows(cols);
+  for (long long r = 0; r < rows; r += most) {
+    const long long n = rows - r < most ? rows - r : most;
+    auto *xp = reinterpret_cast<const typename E::type *>(x) + r * ldx;
+    auto *qp = reinterpret_cast<unsigned char *>(q) + r * cols * 8, *ep = reinterpret_cast<unsigned char *>(e) + r * (cols / 4);
+    hipLaunchKernelGGL((ch % 8 ? act8_pack_kernel<E, true> : act8_pack_kernel<E, false>), dim3((unsigned)((n * cols + 255) / 256)), dim3(256), 0, st, xp,
+                       n, ch, ldx, qp, ep, cols);
+    TBG_LAUNCH_CHECK();
+  }
   return TBG_OK;
 }
 
@@ -75,13 +79,15 @@ template <class E>
 static int launch_unpack(const void *q, const void *e, long long rows, int ch, void *x, long long ldx, hipStream_t st) {
   const unsigned padded = (unsigned)((ch + A8_BLOCK - 1) / A8_BLOCK * A8_BLOCK);
   const unsigned cols = (ch + 7) / 8;
-  const long long blocks = (rows * cols + 255) / 256;
-  if (rows > (1LL << 39) / padded || blocks > 0x7fffffffLL) return TBG_ERANGE;
-  auto *xp = reinterpret_cast<typename E::type *>(x);
-  auto *qp = reinterpret_cast<const unsigned char *>(q), *ep = reinterpret_cast<const unsigned char *>(e);
-  hipLaunchKernelGGL((ch % 8 ? act8_unpack_kernel<E, true> : act8_unpack_kernel<E, false>), dim3((unsigned)blocks), dim3(256), 0, st, qp, ep, rows,
-                     ch, xp, ldx, cols, padded);
-  TBG_LAUNCH_CHECK();
+  const long long most = act8_rows(cols);
+  for (long long r = 0; r < rows; r += most) {
+    const long long n = rows - r < most ? rows - r : most;
+    auto *xp = reinterpret_cast<typename E::type *>(x) + r * ldx;
+    auto *qp = reinterpret_cast<const unsigned char *>(q) + r * padded, *ep = reinterpret_cast<const unsigned char *>(e) + r * (padded / A8_BLOCK);
+    hipLaunchKernelGGL((ch % 8 ? act8_unpack_kernel<E, true> : act8_unpack_kernel<E, false>), dim3((unsigned)((n * cols + 255) / 256)), dim3(256), 0, st,
+                       qp, ep, n, ch, xp, ldx, cols, padded);
+    TBG_LAUNCH_CHECK();
+  }
   return TBG_OK;
 }
 

@@ -376,7 +376,7 @@ extern "C" int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int 
   if (const int rc = a8w_args(rows, cin, cout, dtype)) return rc;
   if (ldy > (1LL << 26)) return TBG_ERANGE;
   const A8wGeo g = a8w_geometry(rows, cin, cout, dtype);
-  if ((long long)(g.nsplit + 7) * g.tk * g.tn > 0x7fffffffLL) return TBG_ERANGE;
+  if ((long long)(g.nsplit + 7) * g.tk * g.tn >= 1LL << 23) return TBG_ERANGE;  // a grid holds less than 2^32 threads
   const long long kn = (long long)cin * cout, need = a8w_workspace(g, cin, cout);
   if (need > workspace_bytes || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))) return TBG_EINVAL;
   A8wP p{};

@@ -10,7 +10,8 @@
 // writes the result.
 //
 // The statistics are 64-bit sums of x and x^2 (the card adds fp64 about as fast as unpacked fp32, so a streaming pass hardly notices): one pass,
-// mean(x^2) - mean^2 loses nothing that matters even where |mean| is 10^5 standard deviations, and no value of any type overflows.  The mean is used as fp32 + its remainder.
+// mean(x^2) - mean^2 loses nothing that matters even where |mean| is 10^5 standard deviations, and no value of any type overflows.  The mean
+// is used as fp32 + its remainder.
 #include "act8.h"
 
 struct GnP {
@@ -653,6 +654,7 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   p.nb = (d->C + A8_BLOCK - 1) / A8_BLOCK;
   p.xn = d->xn; p.xs = d->xs; p.dn = d->dn; p.ds = d->ds; p.eps = d->eps;
   const long long count = d->per_sample ? (long long)d->N * d->C : d->C;
+  if (count > 0x3fffffffLL) return TBG_ERANGE;
   p.pblocks = (int)((count + 31) / 32);
   // the tile (a power of two; a row's 8-bit block never spans two) that leaves the fewest lanes without channels
   const int padded = p.nb * A8_BLOCK;
@@ -685,7 +687,9 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   p.arows = (int)(((p.crows + split - 1) / split + RA - 1) / RA * RA);
   p.split = (p.crows + p.arows - 1) / p.arows;
   if (!backward) gn_whole_tile(p);
-  if ((long long)p.N * p.ntile * p.nchunk * p.split > 0x3fffffffLL || count > 0x3fffffffLL) return TBG_ERANGE;
+  // a grid holds less than 2^32 threads
+  const long long blocks = (long long)p.N * p.ntile * p.nchunk, threads = (1LL << 32) - 1;
+  if (blocks > threads / (p.whole ? GN_TW : backward ? GN_TB : GN_TS) || blocks * p.split + (backward ? p.pblocks : 0) > threads / GN_T) return TBG_ERANGE;
   return TBG_OK;
 }
 static long long gn_part_bytes(const GnP &p) { return p.whole ? 0 : (long long)p.N * p.nchunk * p.nslot * 2 * (long long)sizeof(double); }

@@ -12,6 +12,8 @@ pass read that form directly:
 * ``act8_wgrad``                        its weight and bias gradients, straight from the checkpoint
 
 Parameters and their gradients are fp32 in every mode, as in ``ops``.  First order: the backward passes are not themselves differentiable.
+Everything is enqueued on the current stream and can be captured into a graph; a backward pass is captured where no graph made on the default
+stream from the same leaves is alive (these functions refuse the leaves of one that they have seen).
 Inputs whose rows are not evenly spaced with contiguous channels are copied once (``contiguous()``); slices of wider tensors are not.
 """
 from __future__ import annotations
@@ -26,6 +28,7 @@ from . import native as N
 ACTS = {"linear": 0, "lrelu": 1, "silu": 2}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 BLOCK = 32
+MAX_CHANNELS, MAX_POSITIONS, MAX_SAMPLES, MAX_DENSE = 1 << 24, 1 << 30, 1 << 30, 1 << 20
 
 
 class Act8(NamedTuple):
@@ -69,6 +72,13 @@ def _check(t, what: str, dtypes):
         raise N.TbgError(f"{what}: a tensor is wanted, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise N.TbgError(f"{what}: unsupported dtype {t.dtype}")
+
+
+def _sizes(what: str, **most):
+    """sizes within what the C entries take (their integers are narrower than a tensor's sizes)"""
+    for name, (size, limit) in most.items():
+        if size > limit:
+            raise N.TbgError(f"{what}: {size} {name}, at most {limit} are taken")
 
 
 def _placed(what: str, *ts):
@@ -126,7 +136,10 @@ def _check8(a: Act8):
         raise N.TbgError(f"an Act8 checkpoint is wanted, got {type(a).__name__}")
     _check(a.q, "checkpoint values", (torch.int8,))
     _check(a.e, "checkpoint scales", (torch.uint8,))
-    ch = a.shape[-1]
+    ch = a.shape[-1] if len(a.shape) else 0
+    if ch < 1:
+        raise N.TbgError(f"a checkpoint of [..., channels] is wanted, got one of {tuple(a.shape)}")
+    _sizes("checkpoint", channels=(ch, MAX_CHANNELS))
     nb = (ch + BLOCK - 1) // BLOCK
     rows = 1
     for v in a.shape[:-1]:
@@ -143,6 +156,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     _check(x, "act8_pack", _DTYPES)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise N.TbgError(f"act8_pack: [..., channels] is wanted, got {tuple(x.shape)}")
+    _sizes("act8_pack", channels=(x.shape[-1], MAX_CHANNELS))
     _placed("act8_pack", x)
     shape, x = tuple(x.shape), x.detach()
     rows = x.numel() // shape[-1]
@@ -173,6 +187,7 @@ def act8_wgrad(a: Act8, dy: torch.Tensor, coef: float = 1.0, want_db: bool = Tru
     cin = a.shape[-1]
     if dy.dim() < 1 or dy.shape[-1] < 1 or tuple(dy.shape[:-1]) != tuple(a.shape[:-1]):
         raise N.TbgError(f"act8_wgrad: a gradient {tuple(dy.shape)} does not belong to a checkpoint of {tuple(a.shape)}")
+    _sizes("act8_wgrad", channels=(max(cin, dy.shape[-1]), MAX_DENSE))
     _placed("act8_wgrad", a.q, a.e, dy)
     cout, dev = dy.shape[-1], dy.device
     dy = dy.detach()
@@ -244,6 +259,21 @@ def _gn_bwd(x, q, e, dy, gamma, beta, stats, cfg):
     return dx, dgamma, dbeta
 
 
+def _leaves(what: str, y: torch.Tensor) -> torch.Tensor:
+    """y, an output just made.  The accumulation node of a leaf belongs to the stream of the graph that first used the leaf, for as long as that
+    graph lives.  A captured backward pass that reaches one of the default stream would end the capture, and the process, from the autograd
+    engine's thread: such a leaf is refused while its forward pass is captured."""
+    fn = y.grad_fn
+    if fn is not None:
+        for node, _ in fn.next_functions:
+            if type(node).__name__ == "AccumulateGrad":
+                idx = node.variable.device.index
+                if node.metadata.setdefault("tbg_stream", _raw_stream(idx)) == 0 and _raw_stream(idx) and torch.cuda.is_current_stream_capturing():
+                    raise N.TbgError(f"{what}: a graph that was made on the default stream from the same leaf {tuple(node.variable.shape)} is alive; "
+                                     "release its outputs before the backward pass is captured")
+    return y
+
+
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, cfg, save8, sink, box):
@@ -279,6 +309,7 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
     if x.dim() < 2 or x.shape[-1] < 1:
         raise N.TbgError(f"group_norm_act: [N, ..., channels] is wanted, got {tuple(x.shape)}")
     n, ch = x.shape[0], x.shape[-1]
+    _sizes("group_norm_act", samples=(n, MAX_SAMPLES), channels=(ch, MAX_CHANNELS), positions=(x.numel() // max(n * ch, 1), MAX_POSITIONS))
     if not isinstance(groups, int) or isinstance(groups, bool) or groups < 1 or ch % groups:
         raise N.TbgError(f"group_norm_act: {ch} channels do not divide into {groups} groups")
     if act not in ACTS:
@@ -302,7 +333,7 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
         y, *_, y8 = _gn_fwd(x, gamma, beta, cfg, False, False, sink)
         return (y, y8) if sink else y
     box = []
-    y = _GroupNormAct.apply(x, gamma, beta, cfg, save == "act8", sink, box)
+    y = _leaves("group_norm_act", _GroupNormAct.apply(x, gamma, beta, cfg, save == "act8", sink, box))
     return (y, box[0]) if sink else y
 
 
@@ -310,6 +341,9 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
 # dense (1x1) layer on an 8-bit checkpoint
 # ----------------------------------------------------------------------------------------
 def _dense_fwd(x, w, b, coef):
+    if torch.is_autocast_enabled("cuda"):  # y is in x's type whatever the caller's autocast
+        with torch.autocast("cuda", enabled=False):
+            return _dense_fwd(x, w, b, coef)
     y = x.reshape(-1, w.shape[0]) @ (w * coef).to(x.dtype)
     if b is not None:
         y = y + b.to(x.dtype)
@@ -362,5 +396,5 @@ def dense_act8(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = Non
     _placed("dense_act8", x, w, *(() if b is None else (b,)), *(() if x8 is None else (x8.q, x8.e)))
     coef = float(coef)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b)):
-        return _DenseAct8.apply(x, w, b, coef, None if x8 is None else x8.q, None if x8 is None else x8.e)
+        return _leaves("dense_act8", _DenseAct8.apply(x, w, b, coef, None if x8 is None else x8.q, None if x8 is None else x8.e))
     return _dense_fwd(x, w, b, coef)
