@@ -629,13 +629,16 @@ int tbg_demod_coefs_f32(const float *s, const float *w, float *wsq, float *d, in
  * group); act: 0 linear, 1 LeakyReLU(0.2) x sqrt2, 2 SiLU (z sigmoid(z)).  gamma, beta: [C], or [N][C] with per_sample = 1 (styles).
  * Forward writes y [N][S][C] contiguous; stats [N][G][2] = mean, rstd if not NULL; (q, e) = ACT8 of fl32(x - fl32(mean)) if not NULL,
  * for LeakyReLU moved by one step towards the value where rounding has put z on the other side of 0 (the backward pass takes its slope);
- * (yq, ye) = ACT8 of y as rounded to its type if not NULL (what a following layer keeps of its input).  Backward takes x or (q, e) --
+ * (yq, ye) = ACT8 of y as rounded to its type if not NULL (what a following layer keeps of its input).  Few positions take one launch and no
+ * workspace (0 bytes: NULL).  Backward takes x or (q, e) --
  * the other NULL --, dy and stats, and writes dx [N][S][C] contiguous, dgamma, dbeta (shaped like gamma): with a checkpoint,
  * xh = q 2^e rstd everywhere.  Sums are joined in a fixed order.  Checkpoints, stats and workspace are 16-byte aligned.
  *
  * tbg_act8_wgrad: gradients of a dense (1x1) layer y = coef x w + b, w [cin][cout], from the checkpoint of x:
  * dw[k][n] = coef sum_r x[r][k] dy[r][n], db[n] = sum_r dy[r][n] (db NULL: not wanted), fp32 accumulation on the bf16 matrix pipe: the
- * checkpoint is exact in bf16, dy is one (bf16), two (fp16) or three (fp32) bf16 terms.  dw, db contiguous.
+ * checkpoint is exact in bf16, dy is one (bf16), two (fp16) or three (fp32) bf16 terms (an infinity in fp16 or fp32 leaves NaN in its column of
+ * dw).  dw, db contiguous.
+ * TBG_ERANGE: more than 2^30 positions, 2^24 channels (2^20 of a dense layer), or a launch of 2^32 threads or more.
  * ---------------------------------------------------------------------------------------- */
 #define TBG_ACT_SILU 2
 typedef struct tbg_gn_desc {
