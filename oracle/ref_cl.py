@@ -6,6 +6,11 @@ import torch
 SQRT2 = math.sqrt(2.0)
 
 
+def pow2(k):
+    """2^k in float64, from its bits: a device's pow may be off in the last place"""
+    return ((k.long() + 1023) << 52).view(torch.float64)
+
+
 def pack(x):
     """x [..., C] (any float type) -> (q int8 [rows, 32 nb], e uint8 [rows, nb])."""
     ch = x.shape[-1]
@@ -17,13 +22,13 @@ def pack(x):
     m, k = torch.frexp(v.abs().amax(dim=2))          # amax = m 2^k, 1/2 <= m < 1: in the definition's terms 2m, k - 1
     e = (k - 1 - 6 + (128 * m >= 127.5).int()).clamp(-126, 121)
     e = torch.where(m == 0, -126, e)
-    q = torch.round(v * torch.pow(torch.tensor(2.0, dtype=torch.float64, device=x.device), -e.double())[..., None]).clamp(-127, 127)
+    q = torch.round(v * pow2(-e)[..., None]).clamp(-127, 127)
     return q.to(torch.int8).reshape(-1, nb * 32), torch.where(bad, 255, e + 127).to(torch.uint8)
 
 
 def unpack(q, e, shape):
     """the values, float64, in `shape`"""
-    s = torch.where(e == 255, math.nan, torch.pow(torch.tensor(2.0, dtype=torch.float64, device=q.device), e.double() - 127))
+    s = torch.where(e == 255, math.nan, pow2(e.int() - 127))
     v = (q.double().reshape(*e.shape, 32) * s[..., None]).reshape(q.shape[0], -1)
     return v[:, :shape[-1]].reshape(shape)
 
