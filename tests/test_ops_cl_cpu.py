@@ -109,7 +109,7 @@ def test_entries_check_pointers_and_workspaces():
     assert lib.tbg_act8_unpack(p, p, 0, 8, p, 0, 8, None) == -1 and lib.tbg_act8_unpack(p, None, 4, 8, p, 0, 8, None) == -1
     assert lib.tbg_act8_pack(p, 0, 1 << 38, 64, 64, p, p, None) == -2
     # launches of 2^32 threads
-    for kw, backward in ((dict(N=1 << 24, S=1), 0), (dict(N=1 << 24, S=1), 1), (dict(N=1 << 13, S=1, C=1 << 17), 0), (dict(N=1 << 30, S=5), 1)):
+    for kw, backward in ((dict(N=1 << 30, S=1, C=1024), 0), (dict(N=1 << 30, S=300, C=1024), 1), (dict(N=1 << 15, S=1, C=1 << 17), 0)):
         wide = dict(xs=kw.get("C", 8), ds=kw.get("C", 8), **kw)
         assert lib.tbg_group_norm_workspace_bytes(C.byref(_desc(**wide)), backward) == -2, kw
     assert lib.tbg_act8_wgrad_workspace_bytes(1 << 10, 1 << 16, 1 << 15, 1) >= 0

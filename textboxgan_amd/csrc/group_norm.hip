@@ -29,13 +29,16 @@ struct GnP {
   int CT, ntile, lanes;                // channels a tile (a power of two), tiles, lanes a row
   int nchunk, crows, nslot;            // row ranges of the sums launch
   int split, arows;                    // the second launch's part of a row range: `split` pieces of arows rows
-  int whole;                           // forward in one launch
-  int pblocks;                         // backward: first blocks of the second launch that sum dgamma / dbeta
+  int team;                            // one launch: lanes that share a tile of a sample (0: two launches)
+  int nteam, ng, per, slots;           // teams of a block; most groups of a tile; backward: samples a team takes in turn, blocks' partial sums a channel
+  int pblocks;                         // backward: first blocks of the second launch (one launch: blocks of one behind it) that sum dgamma / dbeta
   float eps;
 };
 
-// threads a block: second launches, forward sums, backward sums, whole forward; most channels a tile; rows a lane of the whole forward keeps
-constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_TW = 512, GN_CT = 128, GN_R = 8;
+// threads a block: second launches, forward sums, backward sums, one-launch forward; most channels a tile of two launches
+constexpr int GN_T = 256, GN_TS = 1024, GN_TB = 512, GN_TW = 512, GN_CT = 128;
+// rows that a lane of the one-launch forms keeps in registers, forward and backward
+constexpr int GN_R = 8, GN_RB = 4;
 
 template <int ACT>
 __device__ __forceinline__ float gn_act(float z) {
@@ -347,43 +350,105 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
   for (; r < r1; r += RL, x += xstep, y += ystep) out.write(out.in ? out.row.load(x) : zero, y, row0 + r);
 }
 
-// ---- forward in one launch, where the rows of a tile of whole groups fit a block's registers: x is read once
+// ---- one launch, where the rows of a tile of whole groups fit the registers of a team of lanes (a power of two, those of a row or more).  A
+// block's teams have the same tile of neighbouring samples, so that small samples leave no lanes idle and large ones get a whole block
+struct GnTeam {
+  int id, l, lane, rl, RL;         // team; lane of the team; of the row; row, rows at a time
+  int width, part, nparts;         // lanes that exchange rows' sums; then there are `nparts` sums of a channel left, this lane's among them
+  bool first;                      // has its part's sum
+  __device__ __forceinline__ GnTeam(const GnP &p) {
+    id = threadIdx.x / p.team;
+    l = threadIdx.x & (p.team - 1);
+    lane = l & (p.lanes - 1);
+    rl = l / p.lanes;
+    RL = p.team / p.lanes;
+    width = min(p.team, 64);
+    const int span = max(p.lanes, 64);
+    nparts = max(p.team / span, 1);
+    part = nparts > 1 ? l / span : 0;
+    first = (l & (width - 1)) < p.lanes;
+  }
+  // sums over a tile's groups of pairs (one for each `step` channels), done(group of the tile, sum) in one lane of each
+  template <class T, class F>
+  __device__ __forceinline__ void groups(const GnP &p, int ct, int ng, int step, const T *pairs, F done) const {
+    int sub = width;
+    while (sub > 1 && ng * sub > p.team) sub >>= 1;
+    const int k = l & (sub - 1);
+    for (int i = l / sub; i < ng; i += p.team / sub) {  // (more than one trip only where sub is 1)
+      const int a0 = i * p.Cg / step, a1 = min((i + 1) * p.Cg, ct) / step;
+      double2 o = {0.0, 0.0};
+      for (int c = a0 + k; c < a1; c += sub) {
+        o.x += pairs[c * 2];
+        o.y += pairs[c * 2 + 1];
+      }
+      for (int off = sub >> 1; off > 0; off >>= 1) {
+        o.x += __shfl_xor(o.x, off, 64);
+        o.y += __shfl_xor(o.y, off, 64);
+      }
+      if (k == 0) done(i, o);
+    }
+  }
+};
+
+// x is read once
 template <class E, int A, int ACT, bool Q, bool TAIL>
 __global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
-  __shared__ double red[GN_TW / 64 * (GN_CT / 8) * A * 2];
-  __shared__ double2 st[GN_CT];
-  const GnTile t = gn_tile(p, blockIdx.x);
-  const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_TW / p.lanes;
-  GnOut<E, ACT, Q, TAIL> out(p, t.c0 + lane * 8);
-  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + t.n * p.xn;
+  extern __shared__ __align__(16) char smem[];
+  const GnTeam w(p);
+  const int tile = blockIdx.x % p.ntile, n = blockIdx.x / p.ntile * p.nteam + w.id, c0 = tile * p.CT, ct = min(p.CT, p.C - c0), cols = p.lanes * A;
+  double *red = reinterpret_cast<double *>(smem) + w.id * w.nparts * cols * 2;  // [nparts][cols][2]
+  double2 *st = reinterpret_cast<double2 *>(smem) + p.nteam * w.nparts * cols + w.id * p.ng;
+  const bool live = n < p.N;
+  GnOut<E, ACT, Q, TAIL> out(p, c0 + w.lane * 8);
+  const typename E::type *x = reinterpret_cast<const typename E::type *>(p.x) + n * p.xn;
   Pack8<E> v[GN_R] = {};
   double s1[A], s2[A];
 #pragma unroll
   for (int i = 0; i < A; ++i) s1[i] = s2[i] = 0.0;
-  if (out.in) {
+  if (live && out.in) {
 #pragma unroll
     for (int u = 0; u < GN_R; ++u)
-      if (rl + u * RL < p.S) v[u] = out.row.load(x + (rl + u * RL) * p.xs);
+      if (w.rl + u * w.RL < p.S) v[u] = out.row.load(x + (w.rl + u * w.RL) * p.xs);
   }
-  out.affine(t.n);
-  if (out.in) {
+  if (live) out.affine(n);
+  if (live && out.in) {
 #pragma unroll
     for (int u = 0; u < GN_R; ++u) gn_add<E, A>(v[u], s1, s2);  // (rows that do not exist are zeros)
   }
-  gn_block_sums<A, GN_TW>(p, s1, s2, red);
-  const int g0 = t.c0 / p.Cg, ng = (t.ct + p.Cg - 1) / p.Cg;
-  gn_group_sums<GN_TW>(p, t, g0, ng, 8 / A, red, [&](int i, const double2 &o) {
+  for (int off = p.lanes; off < w.width; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      s1[i] += __shfl_xor(s1[i], off, 64);
+      s2[i] += __shfl_xor(s2[i], off, 64);
+    }
+  if (w.first)
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      red[(w.part * cols + w.lane * A + i) * 2] = s1[i];
+      red[(w.part * cols + w.lane * A + i) * 2 + 1] = s2[i];
+    }
+  __syncthreads();
+  if (w.nparts > 1) {
+    for (int j = w.l; j < 2 * cols; j += p.team) {
+      double a = red[j];
+      for (int k = 1; k < w.nparts; ++k) a += red[k * 2 * cols + j];
+      red[j] = a;
+    }
+    __syncthreads();
+  }
+  const int g0 = c0 / p.Cg;
+  w.groups(p, ct, (ct + p.Cg - 1) / p.Cg, 8 / A, red, [&](int i, const double2 &o) {
     st[i] = gn_stats(p, o.x, o.y);
-    if (p.stats) *reinterpret_cast<double2 *>(p.stats + ((long long)t.n * p.G + g0 + i) * 2) = st[i];
+    if (live && p.stats) *reinterpret_cast<double2 *>(p.stats + ((long long)n * p.G + g0 + i) * 2) = st[i];
   });
   __syncthreads();
-  if (out.c >= p.nb * A8_BLOCK || (!Q && !out.in)) return;
+  if (!live || out.c >= p.nb * A8_BLOCK || (!Q && !out.in)) return;
   out.stats(reinterpret_cast<const double *>(st), g0);
-  const long long row0 = (long long)t.n * p.S;
+  const long long row0 = (long long)n * p.S;
   typename E::type *y = reinterpret_cast<typename E::type *>(p.y) + row0 * p.C;
 #pragma unroll
   for (int u = 0; u < GN_R; ++u)
-    if (rl + u * RL < p.S) out.write(v[u], y + (long long)(rl + u * RL) * p.C, row0 + rl + u * RL);
+    if (w.rl + u * w.RL < p.S) out.write(v[u], y + (long long)(w.rl + u * w.RL) * p.C, row0 + w.rl + u * w.RL);
 }
 
 // ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd and z = sc d + be
@@ -414,6 +479,16 @@ struct GnRow {
   u32x2 q;
   unsigned e;
 };
+// (what is made of the operands before and after is made twice: it would fill the registers)
+template <class T>
+__device__ __forceinline__ void gn_opaque(T &v) {
+  static_assert(sizeof(T) % 4 == 0, "whole registers");
+  unsigned w[sizeof(T) / 4];
+  __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) asm volatile("" : "+v"(w[i]));
+  __builtin_memcpy(&v, w, sizeof(T));
+}
 // where a lane stands, and a step of `rows` rows
 template <class E, bool Q8, bool TAIL>
 struct GnAt {
@@ -531,6 +606,41 @@ __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
   });
 }
 
+// dgamma, dbeta of 32 channels from partial sums, by 8 lanes each of a block of GN_T: the row ranges (or blocks of the one-launch form, and the
+// samples, where the parameters are shared) in a fixed order
+__device__ __forceinline__ void gn_param_sums(const GnP &p, int b, double2 *sh) {
+  static_assert(GN_T == 256 && 2 * GN_CT == GN_T, "a lane's sums in sh");
+  const int sub = threadIdx.x >> 5;
+  const long long idx = (long long)b * 32 + (threadIdx.x & 31), count = p.affn ? (long long)p.N * p.C : p.C;
+  double2 o = {0.0, 0.0};
+  if (idx < count) {
+    const int n = p.affn ? (int)(idx / p.C) : 0, c = (int)(idx % p.C);
+    const long long len = p.team ? p.slots : (long long)(p.affn ? 1 : p.N) * p.nchunk;
+    const float *src = p.pch + ((long long)n * p.nchunk * p.C + c) * 2;
+#pragma unroll 8
+    for (long long i = sub; i < len; i += 8) {
+      const float2 s = *reinterpret_cast<const float2 *>(src + i * p.C * 2);
+      o.x += s.x;
+      o.y += s.y;
+    }
+  }
+  sh[threadIdx.x] = o;
+  __syncthreads();
+  if (threadIdx.x < 32 && idx < count) {
+#pragma unroll
+    for (int l = 1; l < 8; ++l) {
+      o.x += sh[l * 32 + threadIdx.x].x;
+      o.y += sh[l * 32 + threadIdx.x].y;
+    }
+    p.dbeta[idx] = (float)o.x;
+    p.dgamma[idx] = (float)o.y;
+  }
+}
+__global__ __launch_bounds__(GN_T) void gn_params_kernel(GnP p) {
+  __shared__ double2 sh[GN_T];
+  gn_param_sums(p, blockIdx.x, sh);
+}
+
 // ---- backward, second launch: dx, and in its first blocks dgamma / dbeta
 template <class E, int ACT, bool Q8, bool TAIL>
 __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
@@ -538,33 +648,8 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   __shared__ double2 sh[2 * GN_CT];
   double2 *st = sh, *stats = sh + GN_CT;  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh); mean, rstd
   int b = blockIdx.x;
-  if (b < p.pblocks) {  // 32 channels, 8 lanes each: the row ranges (and samples, where the parameters are shared) in a fixed order
-    static_assert(GN_T == 256 && 2 * GN_CT == GN_T, "a lane's sums in sh");
-    const int sub = threadIdx.x >> 5;
-    const long long idx = (long long)b * 32 + (threadIdx.x & 31), count = p.affn ? (long long)p.N * p.C : p.C;
-    double2 o = {0.0, 0.0};
-    if (idx < count) {
-      const int n = p.affn ? (int)(idx / p.C) : 0, c = (int)(idx % p.C);
-      const long long len = (long long)(p.affn ? 1 : p.N) * p.nchunk;
-      const float *src = p.pch + ((long long)n * p.nchunk * p.C + c) * 2;
-#pragma unroll 8
-      for (long long i = sub; i < len; i += 8) {
-        const float2 s = *reinterpret_cast<const float2 *>(src + i * p.C * 2);
-        o.x += s.x;
-        o.y += s.y;
-      }
-    }
-    sh[threadIdx.x] = o;
-    __syncthreads();
-    if (threadIdx.x < 32 && idx < count) {
-#pragma unroll
-      for (int l = 1; l < 8; ++l) {
-        o.x += sh[l * 32 + threadIdx.x].x;
-        o.y += sh[l * 32 + threadIdx.x].y;
-      }
-      p.dbeta[idx] = (float)o.x;
-      p.dgamma[idx] = (float)o.y;
-    }
+  if (b < p.pblocks) {
+    gn_param_sums(p, b, sh);
     return;
   }
   b -= p.pblocks;
@@ -623,6 +708,139 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   for (; r < r1; r += RL) write(at.next(p, RL));
 }
 
+// ---- backward in one launch (teams as in the forward one): x (or its checkpoint) and dy are read once.  The parameters' gradients are summed
+// over the `per` samples that a team takes in turn and the teams of the block; one block a tile: that is all of them, else a launch joins the blocks
+template <class E, int ACT, bool Q8, bool TAIL>
+__global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
+  constexpr int R = GN_RB;
+  extern __shared__ __align__(16) char smem[];
+  const GnTeam w(p);
+  const int tile = blockIdx.x % p.ntile, chunk = blockIdx.x / p.ntile, c0 = tile * p.CT, ct = min(p.CT, p.C - c0), c = c0 + w.lane * 8, g0 = c0 / p.Cg;
+  double2 *st = reinterpret_cast<double2 *>(smem) + w.id * p.ng;  // of the tile's groups: mean(sc dz), rstd^2 mean(sc dz d)
+  float *reds = reinterpret_cast<float *>(reinterpret_cast<double2 *>(smem) + p.nteam * p.ng);
+  float *red = reds + w.id * w.nparts * p.CT * 2;  // [nparts][CT][2]
+  const bool in = w.lane * 8 < ct;
+  float a1[8], a2[8];  // sums of dz, dz xh over the samples
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a1[i] = a2[i] = 0.f;
+  for (int k = 0; k < p.per; ++k) {
+    const long long at = ((long long)chunk * p.per + k) * p.nteam + w.id;
+    const bool live = at < p.N && in;
+    const int n = at < p.N ? (int)at : 0;
+    GnRow<E, Q8> row[R];
+    GnCh h;
+    float s1[8], s2[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s1[i] = s2[i] = 0.f;
+    if (live) {
+      GnAt<E, Q8, TAIL> from(p, n, w.rl, c);
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+        if (w.rl + u * w.RL < p.S) row[u] = from.next(p, w.RL);
+      gn_affine<TAIL>(p, n, c, h.sc, h.be);
+      gn_channels<Q8>(p, c, reinterpret_cast<const double2 *>(p.stats) + (long long)n * p.G, 0, h);
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+        if (w.rl + u * w.RL < p.S) {
+          float d[8], dz[8];
+          gn_row<E, ACT, Q8>(row[u], h, d, dz);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            s1[i] += dz[i];
+            s2[i] = fmaf(dz[i], d[i], s2[i]);
+          }
+        }
+    }
+    for (int off = p.lanes; off < w.width; off <<= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s1[i] += __shfl_xor(s1[i], off, 64);
+        s2[i] += __shfl_xor(s2[i], off, 64);
+      }
+    if (w.nparts > 1) {
+      if (w.first)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          red[(w.part * p.CT + w.lane * 8 + i) * 2] = s1[i];
+          red[(w.part * p.CT + w.lane * 8 + i) * 2 + 1] = s2[i];
+        }
+      __syncthreads();
+      if (w.rl == 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          for (int o = 1; o < w.nparts; ++o) {
+            s1[i] += red[(o * p.CT + w.lane * 8 + i) * 2];
+            s2[i] += red[(o * p.CT + w.lane * 8 + i) * 2 + 1];
+          }
+    }
+    if (w.rl == 0 && live) {  // the channels' sums: for the parameters, and times the scale for the groups
+      int g[8];
+      gn_groups(p, c, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float xh = s2[i] * (float)p.stats[((long long)n * p.G + g[i]) * 2 + 1];
+        if (p.affn) {
+          if (!TAIL || c + i < p.C) {
+            p.dbeta[(long long)n * p.C + c + i] = s1[i];
+            p.dgamma[(long long)n * p.C + c + i] = xh;
+          }
+        } else {
+          a1[i] += s1[i];
+          a2[i] += xh;
+        }
+        red[(w.lane * 8 + i) * 2] = h.sc[i] * s1[i];
+        red[(w.lane * 8 + i) * 2 + 1] = h.sc[i] * s2[i];
+      }
+    }
+    __syncthreads();
+    w.groups(p, ct, (ct + p.Cg - 1) / p.Cg, 1, red, [&](int i, const double2 &o) {
+      const double rstd = p.stats[((long long)n * p.G + g0 + i) * 2 + 1], m = (double)p.S * p.Cg;
+      st[i] = {o.x / m, rstd * rstd * (o.y / m)};
+    });
+    __syncthreads();
+    if (live) {
+      float m1[8], m2[8];  // dx = sc dz - m1 - d m2
+      int g[8];
+      gn_groups(p, c, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double2 m = st[g[i] - g0];
+        m1[i] = (float)m.x;
+        m2[i] = (float)m.y;
+      }
+      const Row8<E, TAIL> to(c, p.C);
+      typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + (long long)n * p.S * p.C;
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+        if (w.rl + u * w.RL < p.S) {
+          float d[8], dz[8];
+          gn_opaque(row[u].g);
+          if constexpr (Q8) gn_opaque(row[u].q);
+          else gn_opaque(row[u].x);
+          gn_row<E, ACT, Q8>(row[u], h, d, dz);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
+          to.store(dx + (long long)(w.rl + u * w.RL) * p.C, put8<E>(dz));
+        }
+    }
+  }
+  if (p.affn) return;
+  // (all reads of `reds` are before the last barrier)
+  if (w.rl == 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      reds[(w.id * p.CT + w.lane * 8 + i) * 2] = a1[i];
+      reds[(w.id * p.CT + w.lane * 8 + i) * 2 + 1] = a2[i];
+    }
+  __syncthreads();
+  for (int j = threadIdx.x; j < 2 * ct; j += GN_T) {
+    float a = reds[j];
+    for (int t = 1; t < p.nteam; ++t) a += reds[t * 2 * p.CT + j];
+    if (p.slots > 1) p.pch[((long long)chunk * p.C + c0) * 2 + j] = a;
+    else (j & 1 ? p.dgamma : p.dbeta)[c0 + (j >> 1)] = a;
+  }
+}
+
 // ---- host side
 static bool gn_desc_ok(const tbg_gn_desc *d) {
   return d && d->N >= 1 && d->S >= 1 && d->C >= 1 && d->G >= 1 && d->C % d->G == 0 && dt_valid(d->dtype) && d->act >= TBG_ACT_LINEAR &&
@@ -634,16 +852,47 @@ static void gn_tiles(GnP &p, int CT) {
   p.lanes = CT / 8;
   p.nslot = p.ntile + p.G - 1;
 }
-// One launch (forward): a tile of whole groups whose rows fit a block's registers.  Of those the narrowest: more blocks.
-static bool gn_whole_tile(GnP &p) {
-  for (int ct = 32; ct <= GN_CT; ct <<= 1)
-    if ((ct % p.Cg == 0 || ct >= p.C) && p.S <= (long long)GN_R * (GN_TW / (ct / 8))) {
-      gn_tiles(p, ct);
-      p.whole = p.nchunk = p.split = 1;
-      p.crows = p.arows = p.S;
-      return true;
+// channels in runs of 8, 4, 2 or 1 within a group (of the forward sums: 8 / run accumulators a lane)
+static int gn_run_length(const GnP &p) { return p.C % 8 == 0 && p.Cg % 8 == 0 ? 8 : p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1; }
+static size_t gn_team_lds(const GnP &p, bool backward) {
+  const int span = p.lanes > 64 ? p.lanes : 64, nparts = p.team > span ? p.team / span : 1;
+  return (size_t)p.nteam * (nparts * p.lanes * (backward ? 64 : 16 * (8 / gn_run_length(p))) + p.ng * 16);
+}
+// One launch: a tile of whole groups whose rows fit the registers of a block's lanes.  Few samples: the narrowest such tile and all of the
+// block's lanes.  Samples for more than the card's threads: tiles of up to GN_CT channels, as few lanes a sample as its rows need.
+static bool gn_one_launch(GnP &p, bool backward) {
+  const int T = backward ? GN_T : GN_TW, R = backward ? GN_RB : GN_R;
+  constexpr long long FULL = 256 * 1024;
+  constexpr size_t LDS = 40960;  // four blocks a CU
+  const GnP two = p;
+  const auto fits = [&](int ct, int team) {
+    if ((ct % p.Cg && ct < p.C) || ct / 8 > team || p.S > (long long)R * (team / (ct / 8))) return false;
+    gn_tiles(p, ct);
+    p.team = team;
+    p.nteam = T / team;
+    p.ng = p.G < ct / p.Cg ? p.G : ct / p.Cg;
+    return gn_team_lds(p, backward) <= LDS;
+  };
+  int ct = 32;
+  while (!fits(ct, T)) {
+    if (ct >= p.C || ct >= 8 * T) {
+      p = two;
+      return false;
     }
-  return false;
+    ct <<= 1;
+  }
+  while (ct < GN_CT && ct < p.C && (long long)p.N * p.ntile * T > FULL && fits(2 * ct, T)) ct <<= 1;
+  fits(ct, T);
+  int team = T;
+  while ((long long)p.N * p.ntile * team > FULL && fits(ct, team / 2)) team >>= 1;
+  fits(ct, team);
+  p.nchunk = p.split = 1;
+  p.crows = p.arows = p.S;
+  const long long blocks = (long long)p.N * p.ntile / p.nteam;
+  p.per = 1;
+  if (backward && blocks > 1024) p.per = (int)(blocks / 1024 < 64 ? blocks / 1024 : 64);
+  p.slots = (int)((p.N + (long long)p.nteam * p.per - 1) / (p.nteam * p.per));
+  return true;
 }
 // Two launches.  Row ranges: the sums launch has at most 32 a tile (64 where the samples and tiles are few), each joined by every block of the
 // second launch that needs it; of 4 rows a lane or more, fewer where that leaves CUs idle.  The second launch cuts them into pieces for about
@@ -686,14 +935,18 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   if (split < 1) split = 1;
   p.arows = (int)(((p.crows + split - 1) / split + RA - 1) / RA * RA);
   p.split = (p.crows + p.arows - 1) / p.arows;
-  if (!backward) gn_whole_tile(p);
+  const bool one = gn_one_launch(p, backward);
   // a grid holds less than 2^32 threads
-  const long long blocks = (long long)p.N * p.ntile * p.nchunk, threads = (1LL << 32) - 1;
-  if (blocks > threads / (p.whole ? GN_TW : backward ? GN_TB : GN_TS) || blocks * p.split + (backward ? p.pblocks : 0) > threads / GN_T) return TBG_ERANGE;
+  const long long blocks = (long long)(one ? p.slots : p.N) * p.ntile * p.nchunk, threads = (1LL << 32) - 1;
+  if (blocks > threads / (backward ? (one ? GN_T : GN_TB) : one ? GN_TW : GN_TS) || blocks * p.split + (backward ? p.pblocks : 0) > threads / GN_T)
+    return TBG_ERANGE;
   return TBG_OK;
 }
-static long long gn_part_bytes(const GnP &p) { return p.whole ? 0 : (long long)p.N * p.nchunk * p.nslot * 2 * (long long)sizeof(double); }
-static long long gn_pch_bytes(const GnP &p) { return (long long)p.N * p.nchunk * p.C * 2 * (long long)sizeof(float); }
+static long long gn_part_bytes(const GnP &p) { return p.team ? 0 : (long long)p.N * p.nchunk * p.nslot * 2 * (long long)sizeof(double); }
+static long long gn_pch_bytes(const GnP &p) {
+  if (p.team) return p.affn || p.slots == 1 ? 0 : (long long)p.slots * p.C * 2 * (long long)sizeof(float);
+  return (long long)p.N * p.nchunk * p.C * 2 * (long long)sizeof(float);
+}
 
 extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int backward) {
   if (!gn_desc_ok(d)) return TBG_EINVAL;
@@ -702,15 +955,14 @@ extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int ba
   return gn_part_bytes(p) + (backward ? gn_pch_bytes(p) : 0);
 }
 
-// the accumulators a lane needs: channels in runs of 8, 4, 2 or 1 within a group
 template <class E, int ACT, bool Q, bool TAIL>
 static int gn_run_fwd(const GnP &p, hipStream_t st) {
-  const int run = TAIL ? (p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1) : (p.Cg % 8 == 0 ? 8 : p.Cg % 4 == 0 ? 4 : p.Cg % 2 == 0 ? 2 : 1);
+  const int run = gn_run_length(p);
   constexpr int A8 = TAIL ? 2 : 1;
-  if (p.whole) {
+  if (p.team) {
     const auto whole = run == 8 ? gn_whole_kernel<E, A8, ACT, Q, TAIL> : run == 4 ? gn_whole_kernel<E, 2, ACT, Q, TAIL>
                        : run == 2 ? gn_whole_kernel<E, 4, ACT, Q, TAIL> : gn_whole_kernel<E, 8, ACT, Q, TAIL>;
-    hipLaunchKernelGGL(whole, dim3(p.N * p.ntile), dim3(GN_TW), 0, st, p);
+    hipLaunchKernelGGL(whole, dim3(p.slots * p.ntile), dim3(GN_TW), gn_team_lds(p, false), st, p);
     TBG_LAUNCH_CHECK();
     return TBG_OK;
   }
@@ -724,6 +976,15 @@ static int gn_run_fwd(const GnP &p, hipStream_t st) {
 }
 template <class E, int ACT, bool Q8, bool TAIL>
 static int gn_run_bwd(const GnP &p, hipStream_t st) {
+  if (p.team) {
+    hipLaunchKernelGGL((gn_bwd_whole_kernel<E, ACT, Q8, TAIL>), dim3(p.slots * p.ntile), dim3(GN_T), gn_team_lds(p, true), st, p);
+    TBG_LAUNCH_CHECK();
+    if (!p.affn && p.slots > 1) {
+      hipLaunchKernelGGL(gn_params_kernel, dim3(p.pblocks), dim3(GN_T), 0, st, p);
+      TBG_LAUNCH_CHECK();
+    }
+    return TBG_OK;
+  }
   hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT, Q8, TAIL>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
   TBG_LAUNCH_CHECK();
   hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, Q8, TAIL>), dim3(p.pblocks + p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
@@ -770,13 +1031,13 @@ extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const flo
 extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const void *q, const void *e, const void *dy, const float *gamma,
                                   const float *beta, const double *stats, void *dx, float *dgamma, float *dbeta, void *workspace,
                                   long long workspace_bytes, void *stream) {
-  if (!gn_desc_ok(d) || !dy || !gamma || !beta || !stats || !dx || !dgamma || !dbeta || !workspace || (q == nullptr) != (e == nullptr) ||
+  if (!gn_desc_ok(d) || !dy || !gamma || !beta || !stats || !dx || !dgamma || !dbeta || (q == nullptr) != (e == nullptr) ||
       (x == nullptr) == (q == nullptr))
     return TBG_EINVAL;
   if (gn_misaligned(q, workspace) || gn_misaligned(stats, nullptr)) return TBG_EINVAL;
   GnP p{};
   if (const int rc = gn_geometry(d, true, p)) return rc;
-  if (gn_part_bytes(p) + gn_pch_bytes(p) > workspace_bytes) return TBG_EINVAL;
+  if (gn_part_bytes(p) + gn_pch_bytes(p) > (workspace ? workspace_bytes : 0)) return TBG_EINVAL;
   p.x = x; p.dy = dy; p.gamma = gamma; p.beta = beta; p.y = dx; p.stats = const_cast<double *>(stats);
   p.q = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(q));
   p.e = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(e));

@@ -253,9 +253,9 @@ def _gn_bwd(x, q, e, dy, gamma, beta, stats, cfg):
     d, nbytes = _gn_plan(1, xn, xs, dn, ds, n, pos, ch, groups, _DTYPES[dtype], act, gamma.dim() - 1, eps)
     dx = torch.empty(shape, device=dev, dtype=dtype)
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     _call("tbg_group_norm_bwd", dy, d, _ptr(x), _ptr(q), _ptr(e), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), dx.data_ptr(),
-          dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), nbytes)
+          dgamma.data_ptr(), dbeta.data_ptr(), _ptr(ws), nbytes)
     return dx, dgamma, dbeta
 
 
