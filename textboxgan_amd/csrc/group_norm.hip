@@ -860,7 +860,7 @@ static size_t gn_team_lds(const GnP &p, bool backward) {
 }
 // One launch: a tile of whole groups whose rows fit the registers of a block's lanes.  Few samples: the narrowest such tile and all of the
 // block's lanes.  Samples for more than the card's threads: tiles of up to GN_CT channels, as few lanes a sample as its rows need.
-static bool gn_one_launch(GnP &p, bool backward) {
+static bool gn_one_launch(GnP &p, int least_ct, bool backward) {
   const int T = backward ? GN_T : GN_TW, R = backward ? GN_RB : GN_R;
   constexpr long long FULL = 256 * 1024;
   constexpr size_t LDS = 40960;  // four blocks a CU
@@ -873,7 +873,7 @@ static bool gn_one_launch(GnP &p, bool backward) {
     p.ng = p.G < ct / p.Cg ? p.G : ct / p.Cg;
     return gn_team_lds(p, backward) <= LDS;
   };
-  int ct = 32;
+  int ct = least_ct;
   while (!fits(ct, T)) {
     if (ct >= p.C || ct >= 8 * T) {
       p = two;
@@ -894,10 +894,10 @@ static bool gn_one_launch(GnP &p, bool backward) {
   p.slots = (int)((p.N + (long long)p.nteam * p.per - 1) / (p.nteam * p.per));
   return true;
 }
-// Two launches.  Row ranges: the sums launch has at most 32 a tile (64 where the samples and tiles are few), each joined by every block of the
+// Two launches.  Row ranges: the sums launch has at most 32 a tile (256 where samples and tiles are few), each joined by every block of the
 // second launch that needs it; of 4 rows a lane or more, fewer where that leaves CUs idle.  The second launch cuts them into pieces for about
 // 8 blocks a CU, of 8 rows a lane or more, fewer for 2 blocks a CU.
-static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
+static int gn_geometry(const tbg_gn_desc *d, bool backward, bool writes8, GnP &p) {
   if (d->S > (1 << 30) || d->C > (1 << 24)) return TBG_ERANGE;
   p.N = d->N; p.S = d->S; p.C = d->C; p.G = d->G; p.Cg = d->C / d->G; p.affn = d->per_sample ? d->C : 0;
   p.nb = (d->C + A8_BLOCK - 1) / A8_BLOCK;
@@ -905,18 +905,18 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   const long long count = d->per_sample ? (long long)d->N * d->C : d->C;
   if (count > 0x3fffffffLL) return TBG_ERANGE;
   p.pblocks = (int)((count + 31) / 32);
-  // the tile (a power of two; a row's 8-bit block never spans two) that leaves the fewest lanes without channels
-  const int padded = p.nb * A8_BLOCK;
-  int best = 0, tile = 0;
-  for (int ct = GN_CT; ct >= 32; ct >>= 1) {
+  // the tile (a power of two; where 8-bit blocks are written, none spans two) that leaves the fewest lanes without channels
+  const int padded = p.nb * A8_BLOCK, least_ct = p.C > 16 || writes8 ? A8_BLOCK : p.C > 8 ? 16 : 8;
+  int best = 0, tile = least_ct;
+  for (int ct = GN_CT; ct > A8_BLOCK && p.C > A8_BLOCK; ct >>= 1) {
     const int used = (int)(1000LL * padded / ((long long)(padded + ct - 1) / ct * ct));
-    if (used > best && (ct > 32 || padded == 32)) { best = used; tile = ct; }
+    if (used > best) { best = used; tile = ct; }
   }
   gn_tiles(p, tile);
   const int RL = (backward ? GN_TB : GN_TS) / p.lanes, RA = GN_T / p.lanes;
   const long long tiles = (long long)p.N * p.ntile;
   long long want = 512 / tiles;
-  const long long cap = tiles < 8 ? 64 : 32, fill = 128 / tiles, rows_each = (p.S + RL - 1) / RL;
+  const long long cap = tiles < 8 ? 256 : 32, fill = 128 / tiles, rows_each = (p.S + RL - 1) / RL;
   long long most = (p.S + 4LL * RL - 1) / (4LL * RL);
   most = most > fill ? most : (rows_each < fill ? rows_each : fill);
   if (most < 1) most = 1;
@@ -935,7 +935,7 @@ static int gn_geometry(const tbg_gn_desc *d, bool backward, GnP &p) {
   if (split < 1) split = 1;
   p.arows = (int)(((p.crows + split - 1) / split + RA - 1) / RA * RA);
   p.split = (p.crows + p.arows - 1) / p.arows;
-  const bool one = gn_one_launch(p, backward);
+  const bool one = gn_one_launch(p, least_ct, backward);
   // a grid holds less than 2^32 threads
   const long long blocks = (long long)(one ? p.slots : p.N) * p.ntile * p.nchunk, threads = (1LL << 32) - 1;
   if (blocks > threads / (backward ? (one ? GN_T : GN_TB) : one ? GN_TW : GN_TS) || blocks * p.split + (backward ? p.pblocks : 0) > threads / GN_T)
@@ -950,9 +950,11 @@ static long long gn_pch_bytes(const GnP &p) {
 
 extern "C" long long tbg_group_norm_workspace_bytes(const tbg_gn_desc *d, int backward) {
   if (!gn_desc_ok(d)) return TBG_EINVAL;
-  GnP p{};
-  if (const int rc = gn_geometry(d, backward != 0, p)) return rc;
-  return gn_part_bytes(p) + (backward ? gn_pch_bytes(p) : 0);
+  GnP p{}, w{};
+  if (const int rc = gn_geometry(d, backward != 0, false, p)) return rc;
+  if (backward) return gn_part_bytes(p) + gn_pch_bytes(p);
+  if (const int rc = gn_geometry(d, false, true, w)) return rc;  // (the form that writes checkpoints has wider tiles for few channels)
+  return gn_part_bytes(p) > gn_part_bytes(w) ? gn_part_bytes(p) : gn_part_bytes(w);
 }
 
 template <class E, int ACT, bool Q, bool TAIL>
@@ -1020,7 +1022,7 @@ extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const flo
     return TBG_EINVAL;
   if (gn_misaligned(q, yq) || gn_misaligned(workspace, stats)) return TBG_EINVAL;
   GnP p{};
-  if (const int rc = gn_geometry(d, false, p)) return rc;
+  if (const int rc = gn_geometry(d, false, q || yq, p)) return rc;
   if (gn_part_bytes(p) > (workspace ? workspace_bytes : 0)) return TBG_EINVAL;
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = y; p.stats = stats; p.part = reinterpret_cast<double *>(workspace);
   p.q = reinterpret_cast<unsigned char *>(q); p.e = reinterpret_cast<unsigned char *>(e);
@@ -1036,7 +1038,7 @@ extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const voi
     return TBG_EINVAL;
   if (gn_misaligned(q, workspace) || gn_misaligned(stats, nullptr)) return TBG_EINVAL;
   GnP p{};
-  if (const int rc = gn_geometry(d, true, p)) return rc;
+  if (const int rc = gn_geometry(d, true, false, p)) return rc;
   if (gn_part_bytes(p) + gn_pch_bytes(p) > (workspace ? workspace_bytes : 0)) return TBG_EINVAL;
   p.x = x; p.dy = dy; p.gamma = gamma; p.beta = beta; p.y = dx; p.stats = const_cast<double *>(stats);
   p.q = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(q));
