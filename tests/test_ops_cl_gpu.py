@@ -185,7 +185,7 @@ def test_group_norm_forward_and_gradients(dev, dtype, act, save):
 def test_group_norm_of_many_small_samples(dev, dtype, per_sample, save):
     """samples that share blocks, some of them taken in turn"""
     for i, (n, s, ch, groups) in enumerate([(700, 1, 256, 8), (1100, 3, 33, 11), (5000, 1, 40, 5), (601, 20, 64, 2), (20000, 1, 32, 1), (2100, 4, 100, 4),
-                                            (17001, 2, 256, 8), (700, 7, 1000, 8), (70001, 1, 24, 3), (1030, 9, 520, 1), (800, 3, 130, 130), (3000, 60, 32, 2)]):
+                                            (17001, 2, 256, 8), (700, 7, 1000, 8), (70001, 1, 24, 3), (1030, 9, 520, 1), (800, 3, 130, 130), (3000, 60, 32, 2), (4200, 200, 32, 2)]):
         what = f"{n}x{s}x{ch} groups {groups}"
         x = values((n, s, ch), dtype, dev, 110 + i)
         gamma, beta = affine(n, ch, per_sample, dev)

@@ -860,6 +860,10 @@ static size_t gn_team_lds(const GnP &p, bool backward) {
 }
 // One launch: a tile of whole groups whose rows fit the registers of a block's lanes.  Few samples: the narrowest such tile and all of the
 // block's lanes.  Samples for more than the card's threads: tiles of up to GN_CT channels, as few lanes a sample as its rows need.
+// Forward (bf16, SiLU, us of kernels, one launch / two): 1 x 64 x 256 channels 8.4 / 10.0, 32 x 16 x 64 7.0 / 9.8, 128 x 64 x 512 14.5 / 17.6, 512 x 32
+// x 512 18 / 37, 65536 x 1 x 256 55 / 4800; a few blocks of full registers 11.1 / 9.6 (1 x 1024 x 32), where the launch saved is worth the rest.
+// Backward: one launch where it makes the parameters' gradients whole as well (1 x 64 x 256 9.1 / 10.9) or where samples are many (512 x 32 x 512 27 / 39,
+// 65536 x 1 x 256 84 / 1390); between, a second launch would join them (32 x 64 x 512 14.4 / 13.4, 4 x 128 x 256 13.3 / 11.5).
 static bool gn_one_launch(GnP &p, int least_ct, bool backward) {
   const int T = backward ? GN_T : GN_TW, R = backward ? GN_RB : GN_R;
   constexpr long long FULL = 256 * 1024;
@@ -880,6 +884,10 @@ static bool gn_one_launch(GnP &p, int least_ct, bool backward) {
       return false;
     }
     ct <<= 1;
+  }
+  if (backward && !p.affn && p.N > 1 && (long long)p.N * p.ntile * T < 4 * FULL) {
+    p = two;
+    return false;
   }
   while (ct < GN_CT && ct < p.C && (long long)p.N * p.ntile * T > FULL && fits(2 * ct, T)) ct <<= 1;
   fits(ct, T);
