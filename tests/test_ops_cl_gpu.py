@@ -5,8 +5,9 @@ Tolerances.  A result rounded to type t is off by at most eps(t) / 2 of its valu
 fp64): an element goes through at most 16 roundings of 2^-24, each relative to the magnitude of the terms it is made of (`*_amp`), plus the
 exponential's 2^-20: ARITH = 2^-19 of the magnitude.  Sums over positions are accumulated by lanes over at most 64 values in these tests,
 then joined in a tree: at most 64 + 32 more roundings of the sum of magnitudes, 2^-17.  Weight gradients: every product is exact in fp32 and
-the matrix pipe adds 8 or more products at a time; the tests' chains are at most 2^4 long in additions that round by 2^-24 of the sum of
-magnitudes; truncating additions would double that: 2^-18."""
+the matrix pipe adds 8 or more products at a time; the tests' chains are at most 2^6 long (512 rows in two terms, 16 rows at a time) in additions
+that are off by 2^-23 of the partial sum if they truncate, and partial sums of magnitudes grow to the whole over the chain, half of it on
+average: 2^6 2^-1 2^-23 = 2^-18."""
 import pytest
 import torch
 
