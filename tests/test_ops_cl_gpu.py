@@ -546,6 +546,18 @@ def test_a_backward_pass_is_not_captured_over_an_eager_graph(dev):
         assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
+def test_checkpoints_are_no_part_of_a_graph(dev):
+    """operands that want gradients, contiguous and not"""
+    x, dy = values((40, 96), torch.float32, dev, 56).requires_grad_(), values((40, 64), torch.float32, dev, 57).requires_grad_()
+    for xs, ds in ((x, dy), (x[:, 1:34], dy[:, 3:20]), (x.t()[:40].t(), dy.t()[:8].t())):
+        a = ops_cl.act8_pack(xs)
+        dw, db = ops_cl.act8_wgrad(a, ds)
+        y = ops_cl.act8_unpack(a)
+        assert not any(t.requires_grad for t in (a.q, a.e, dw, db, y))
+        w, b = ops_cl.act8_wgrad(ops_cl.act8_pack(xs.detach().contiguous()), ds.detach().contiguous())
+        assert torch.equal(dw, w) and torch.equal(db, b)
+
+
 def test_under_autocast(dev):
     """types are the operands' own, whatever the caller's autocast"""
     p = block_params(2, 64, 48, dev)

@@ -74,11 +74,10 @@ def _check(t, what: str, dtypes):
         raise N.TbgError(f"{what}: unsupported dtype {t.dtype}")
 
 
-def _sizes(what: str, **most):
+def _most(what: str, size: int, limit: int, name: str):
     """sizes within what the C entries take (their integers are narrower than a tensor's sizes)"""
-    for name, (size, limit) in most.items():
-        if size > limit:
-            raise N.TbgError(f"{what}: {size} {name}, at most {limit} are taken")
+    if size > limit:
+        raise N.TbgError(f"{what}: {size} {name}, at most {limit} are taken")
 
 
 def _placed(what: str, *ts):
@@ -139,7 +138,7 @@ def _check8(a: Act8):
     ch = a.shape[-1] if len(a.shape) else 0
     if ch < 1:
         raise N.TbgError(f"a checkpoint of [..., channels] is wanted, got one of {tuple(a.shape)}")
-    _sizes("checkpoint", channels=(ch, MAX_CHANNELS))
+    _most("checkpoint", ch, MAX_CHANNELS, "channels")
     nb = (ch + BLOCK - 1) // BLOCK
     rows = 1
     for v in a.shape[:-1]:
@@ -156,13 +155,13 @@ def act8_pack(x: torch.Tensor) -> Act8:
     _check(x, "act8_pack", _DTYPES)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise N.TbgError(f"act8_pack: [..., channels] is wanted, got {tuple(x.shape)}")
-    _sizes("act8_pack", channels=(x.shape[-1], MAX_CHANNELS))
+    _most("act8_pack", x.shape[-1], MAX_CHANNELS, "channels")
     _placed("act8_pack", x)
-    shape, x = tuple(x.shape), x.detach()
+    shape = tuple(x.shape)
     rows = x.numel() // shape[-1]
     q, e = _alloc8(rows, shape[-1], x.device)
     if rows:
-        x, _, pitch = _rows(x)
+        x, _, pitch = _rows(x.detach() if x.requires_grad else x)
         _call("tbg_act8_pack", x, x.data_ptr(), _DTYPES[x.dtype], rows, shape[-1], pitch, q.data_ptr(), e.data_ptr())
     return Act8(q, e, shape, x.dtype)
 
@@ -187,15 +186,14 @@ def act8_wgrad(a: Act8, dy: torch.Tensor, coef: float = 1.0, want_db: bool = Tru
     cin = a.shape[-1]
     if dy.dim() < 1 or dy.shape[-1] < 1 or tuple(dy.shape[:-1]) != tuple(a.shape[:-1]):
         raise N.TbgError(f"act8_wgrad: a gradient {tuple(dy.shape)} does not belong to a checkpoint of {tuple(a.shape)}")
-    _sizes("act8_wgrad", channels=(max(cin, dy.shape[-1]), MAX_DENSE))
+    _most("act8_wgrad", max(cin, dy.shape[-1]), MAX_DENSE, "channels")
     _placed("act8_wgrad", a.q, a.e, dy)
     cout, dev = dy.shape[-1], dy.device
-    dy = dy.detach()
     if not a.rows:
         return torch.zeros((cin, cout), device=dev), torch.zeros(cout, device=dev) if want_db else None
     dw = torch.empty((cin, cout), device=dev, dtype=torch.float32)
     db = torch.empty(cout, device=dev, dtype=torch.float32) if want_db else None
-    dy, rows, pitch = _rows(dy)
+    dy, rows, pitch = _rows(dy.detach() if dy.requires_grad else dy)
     dt = _DTYPES[dy.dtype]
     nbytes = N.lib().tbg_act8_wgrad_workspace_bytes(rows, cin, cout, dt)
     N.check(min(nbytes, 0), "tbg_act8_wgrad_workspace_bytes")
@@ -309,7 +307,9 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
     if x.dim() < 2 or x.shape[-1] < 1:
         raise N.TbgError(f"group_norm_act: [N, ..., channels] is wanted, got {tuple(x.shape)}")
     n, ch = x.shape[0], x.shape[-1]
-    _sizes("group_norm_act", samples=(n, MAX_SAMPLES), channels=(ch, MAX_CHANNELS), positions=(x.numel() // max(n * ch, 1), MAX_POSITIONS))
+    _most("group_norm_act", n, MAX_SAMPLES, "samples")
+    _most("group_norm_act", ch, MAX_CHANNELS, "channels")
+    _most("group_norm_act", x.numel() // max(n * ch, 1), MAX_POSITIONS, "positions")
     if not isinstance(groups, int) or isinstance(groups, bool) or groups < 1 or ch % groups:
         raise N.TbgError(f"group_norm_act: {ch} channels do not divide into {groups} groups")
     if act not in ACTS:
