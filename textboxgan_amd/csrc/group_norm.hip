@@ -12,6 +12,9 @@
 // The statistics are 64-bit sums of x and x^2 (the card adds fp64 about as fast as unpacked fp32, so a streaming pass hardly notices): one pass,
 // mean(x^2) - mean^2 loses nothing that matters even where |mean| is 10^5 standard deviations, and no value of any type overflows.  The mean
 // is used as fp32 + its remainder.
+//
+// Measured (us): 32 x 16384 x 128 bf16, SiLU, 8-bit checkpoint: sums 35 (3.8 TB/s), second launch 67-69 (337 MB: 4.9-5.0), backward sums 56-58 and
+// second launch 63-65 (203 and 337 MB: 3.5, 5.2), whose two quarter-rate instructions a value are 34 us of vector time; 16 x 16384 x 128 forward 14 + 26.
 #include "act8.h"
 
 struct GnP {
