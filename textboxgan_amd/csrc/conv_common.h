@@ -30,6 +30,7 @@ typedef __bf16 bf16x2p __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2v __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void split3_pair(float a, float b, unsigned &h, unsigned &m, unsigned &l) {
+#pragma clang fp contract(off)  // a value that the caller multiplies is split as rounded, wherever this is inlined
   const f32x2v v = {a, b};
   const unsigned hu = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2p));
   const f32x2v hf = {__builtin_bit_cast(float, hu << 16), __builtin_bit_cast(float, hu & 0xffff0000u)};

@@ -27,6 +27,12 @@
 
 #include "conv_common.h"  // (split3 / bf16 unit helpers of the unit-sink form; includes common.h)
 
+// scaled value, noise and bias, each rounded: the same bits in every kernel that ends in them
+__device__ __forceinline__ float fir_terms(float a, float sc, float nz, float str, float bias) {
+#pragma clang fp contract(off)
+  return a * sc + nz * str + bias;
+}
+
 struct UpfirdnP {
   const float *x, *k, *kx, *ky, *in_scale;  // k: 2-D [kH][kW] or NULL; kx/ky: 1-D factors or NULL
   float *y;
@@ -209,7 +215,7 @@ __global__ __launch_bounds__(256) void upfirdn2d_tile_kernel(const UpfirdnP p) {
     float res[NOX];
 #pragma unroll
     for (int n = 0; n < NOX; ++n) {
-      float v = out[ny][n] * sc + nz[n] * str + bias;
+      float v = fir_terms(out[ny][n], sc, nz[n], str, bias);
       if (p.has_epi) v = (lrelu ? (v > 0.f ? v : v * slope) : v) * gain;
       res[n] = v;
     }
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(256) void fir_units_kernel(const FirUnitsP p) {
           float a = 0.f;
 #pragma unroll
           for (int t = 0; t < 4; ++t) a += h[ny + t][n] * kfy[t];
-          float v = a * sc + nz[n] * str + bias;
+          float v = fir_terms(a, sc, nz[n], str, bias);
           v = (lrelu ? (v > 0.f ? v : v * slope) : v) * gain;
           res[ny][n] = X0 + n < p.Wt ? v : 0.f;
         }
