@@ -203,6 +203,26 @@ def test_group_norm_of_many_small_samples(dev, dtype, per_sample, save):
         assert torch.equal(y2, y) and torch.equal(y8.q, q) and torch.equal(y8.e, e), what
 
 
+@pytest.mark.parametrize("ch", [128, 250])
+def test_group_norm_of_a_large_tensor(dev, ch):
+    """more than the card's caches hold (results are written past them): sample by sample against the definition"""
+    n, s = 3, 38400000 // ch
+    x = values((n, s, ch), torch.bfloat16, dev, 58)
+    gamma, beta = affine(n, ch, True, dev)
+    dy = values((n, s, ch), torch.bfloat16, dev, 59, 0.3)
+    (y, y8), dx, dg, db = train(x, gamma, beta, 2, dy, act="silu", save="act8", sink=True)
+    for i in range(n):
+        o = R.group_norm(x[i:i + 1], gamma[i:i + 1], beta[i:i + 1], 2, "silu", 1e-5, dy[i:i + 1], "act8")
+        check(y[i:i + 1].detach(), o["y"], o["y_amp"], ARITH, f"{i} y")
+        # (a lane's chain: 300000 rows over at most 32 row ranges of 32 rows at a time are 300 values, 5 times the 64 of SUMS, joined as there)
+        check(dx[i:i + 1], o["dx"], o["dx_amp"], 5 * SUMS, f"{i} dx")
+        check(dg[i:i + 1], o["dgamma"], o["dgamma_amp"], 5 * SUMS, f"{i} dgamma")
+        check(db[i:i + 1], o["dbeta"], o["dbeta_amp"], 5 * SUMS, f"{i} dbeta")
+        del o
+        q, e = R.pack(y[i].detach())
+        assert torch.equal(y8.q.view(n, s, -1)[i], q) and torch.equal(y8.e.view(n, s, -1)[i], e)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_group_norm_sink_is_the_outputs_checkpoint(dev, dtype):
     for n, s, ch, groups in SHAPES:

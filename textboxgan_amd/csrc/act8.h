@@ -54,15 +54,21 @@ __device__ __forceinline__ Pack8<E> ld8(const typename E::type *p) {
   }
   return r;
 }
-template <class E>
+// PAST: written past the caches, whose other lines stay
+template <bool PAST, class T, class V>
+__device__ __forceinline__ void st_vec(T *p, const V &v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <class E, bool PAST = false>
 __device__ __forceinline__ void st8(typename E::type *p, const Pack8<E> &r) {
   if constexpr (E::BYTES == 2) {
     u32x4 w;
     __builtin_memcpy(&w, &r, 16);
-    *reinterpret_cast<u32x4_any *>(p) = w;
+    st_vec<PAST>(reinterpret_cast<u32x4_any *>(p), w);
   } else {
-    reinterpret_cast<f32x4_any *>(p)[0] = f32x4{r.v[0], r.v[1], r.v[2], r.v[3]};
-    reinterpret_cast<f32x4_any *>(p)[1] = f32x4{r.v[4], r.v[5], r.v[6], r.v[7]};
+    st_vec<PAST>(reinterpret_cast<f32x4_any *>(p), f32x4{r.v[0], r.v[1], r.v[2], r.v[3]});
+    st_vec<PAST>(reinterpret_cast<f32x4_any *>(p) + 1, f32x4{r.v[4], r.v[5], r.v[6], r.v[7]});
   }
 }
 // moved down by k elements (k the same in all lanes), zeros above
@@ -118,9 +124,10 @@ struct Row8 {
     }
     return r;
   }
+  template <bool PAST = false>
   __device__ __forceinline__ void store(typename E::type *row, const Pack8<E> &r) const {
     if (!TAIL || left == 8) {
-      st8<E>(row + off, r);
+      st8<E, PAST>(row + off, r);
     } else {
       typename E::type *to = row + (C & ~7);
 #pragma unroll
@@ -183,6 +190,7 @@ __device__ __forceinline__ void a8_round(const float (&x)[8], unsigned code, flo
 }
 __device__ __forceinline__ float a8_scale(unsigned code) { return __uint_as_float(code == A8_NAN ? 0x7fc00000u : code << 23); }
 // what a8_round has left -> bytes
+template <bool PAST = false>
 __device__ __forceinline__ void a8_store(unsigned char *q, unsigned code, const float (&t)[8]) {
   u32x2 w;
 #pragma unroll
@@ -191,7 +199,7 @@ __device__ __forceinline__ void a8_store(unsigned char *q, unsigned code, const 
     const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(t[4 * k + 3]), __float_as_uint(t[4 * k + 2]), 0x04000c0cu);
     w[k] = code == A8_NAN ? 0u : lo | hi;
   }
-  *reinterpret_cast<u32x2 *>(q) = w;
+  st_vec<PAST>(reinterpret_cast<u32x2 *>(q), w);
 }
 // one value of eight packed bytes, in steps
 __device__ __forceinline__ float a8_value(const u32x2 &w, int i) { return (float)(int)(signed char)(w[i >> 2] >> (8 * (i & 3)) & 0xff); }

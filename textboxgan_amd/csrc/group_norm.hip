@@ -13,8 +13,8 @@
 // mean(x^2) - mean^2 loses nothing that matters even where |mean| is 10^5 standard deviations, and no value of any type overflows.  The mean
 // is used as fp32 + its remainder.
 //
-// Measured (us): 32 x 16384 x 128 bf16, SiLU, 8-bit checkpoint: sums 35 (3.8 TB/s), second launch 67-69 (337 MB: 4.9-5.0), backward sums 56-58 and
-// second launch 63-65 (203 and 337 MB: 3.5, 5.2), whose two quarter-rate instructions a value are 34 us of vector time; 16 x 16384 x 128 forward 14 + 26.
+// Measured (us): 32 x 16384 x 128 bf16, SiLU, 8-bit checkpoint: sums 28 (4.8 TB/s), second launch 69 (337 MB: 4.9), backward sums 49 and second
+// launch 62 (203 and 337 MB: 4.1, 5.4), whose two quarter-rate instructions a value are 34 us of vector time; 16 x 16384 x 128 forward 14 + 26.
 #include "act8.h"
 
 struct GnP {
@@ -32,6 +32,7 @@ struct GnP {
   int CT, ntile, lanes;                // channels a tile (a power of two), tiles, lanes a row
   int nchunk, crows, nslot;            // row ranges of the sums launch
   int split, arows;                    // the second launch's part of a row range: `split` pieces of arows rows
+  bool past;                           // second launches write past the caches (rows of whole 8 channels)
   int team;                            // one launch: lanes that share a tile of a sample (0: two launches)
   int nteam, ng, per, slots;           // teams of a block; most groups of a tile; backward: samples a team takes in turn, blocks' partial sums a channel
   int pblocks;                         // backward: first blocks of the second launch (one launch: blocks of one behind it) that sum dgamma / dbeta
@@ -237,7 +238,7 @@ __device__ __forceinline__ void gn_affine(const GnP &p, int n, int c, float (&ga
 }
 
 // ---- forward: what a lane does to a row.  Q: checkpoints are written
-template <class E, int ACT, bool Q, bool TAIL>
+template <class E, int ACT, bool Q, bool TAIL, bool PAST = false>
 struct GnOut {
   const GnP &p;
   Row8<E, TAIL> row;
@@ -282,7 +283,7 @@ struct GnOut {
       for (int i = 0; i < 8; ++i)
         if (f[i] != g[i]) k[i] = fminf(fmaxf(k[i] + (v[i] > kept[i] ? 1.f : -1.f), A8_MAGIC - 127.f), A8_MAGIC + 127.f);
     }
-    a8_store(q + r * p.nb * A8_BLOCK + c, code, k);
+    a8_store<PAST>(q + r * p.nb * A8_BLOCK + c, code, k);
     if ((c & (A8_BLOCK - 1)) == 0) e[r * p.nb + c / A8_BLOCK] = (unsigned char)code;
   }
   // v: channels of row r (of all samples' rows; zeros where there are none), y: where the row goes
@@ -294,7 +295,7 @@ struct GnOut {
       o[i] = gn_act<ACT>(fmaf(d[i], sc[i], sh[i]));
     }
     const Pack8<E> w = put8<E>(o);
-    if (!Q || in) row.store(y, w);
+    if (!Q || in) row.template store<PAST>(y, w);
     if constexpr (Q) {
       if (p.q) {
         if (!in) {
@@ -312,14 +313,14 @@ struct GnOut {
   }
 };
 
-template <class E, int ACT, bool Q, bool TAIL>
+template <class E, int ACT, bool Q, bool TAIL, bool PAST>
 __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
   constexpr int U = 4;
   __shared__ double2 st[GN_CT];  // mean, rstd of the tile's groups
   const int piece = blockIdx.x / p.nchunk % p.split;
   const GnTile t = gn_tile(p, blockIdx.x / p.nchunk / p.split * p.nchunk + blockIdx.x % p.nchunk);
   const int lane = threadIdx.x & (p.lanes - 1), rl = threadIdx.x / p.lanes, RL = GN_T / p.lanes;
-  GnOut<E, ACT, Q, TAIL> out(p, t.c0 + lane * 8);
+  GnOut<E, ACT, Q, TAIL, PAST> out(p, t.c0 + lane * 8);
   out.affine(t.n);
   const int g0 = t.c0 / p.Cg, ng = (t.c0 + t.ct - 1) / p.Cg - g0 + 1;
   int sub = 64;
@@ -645,7 +646,7 @@ __global__ __launch_bounds__(GN_T) void gn_params_kernel(GnP p) {
 }
 
 // ---- backward, second launch: dx, and in its first blocks dgamma / dbeta
-template <class E, int ACT, bool Q8, bool TAIL>
+template <class E, int ACT, bool Q8, bool TAIL, bool PAST>
 __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   constexpr int U = 2;
   __shared__ double2 sh[2 * GN_CT];
@@ -698,7 +699,7 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
     gn_row<E, ACT, Q8>(w, h, d, dz);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
-    at.row.store(dx, put8<E>(dz));
+    at.row.template store<PAST>(dx, put8<E>(dz));
     dx += (long long)RL * p.C;
   };
   for (; r + (U - 1) * RL < r1; r += U * RL) {
@@ -983,7 +984,8 @@ static int gn_run_fwd(const GnP &p, hipStream_t st) {
                     : run == 2 ? gn_sums_kernel<E, 4, TAIL> : gn_sums_kernel<E, 8, TAIL>;
   hipLaunchKernelGGL(sums, dim3(p.N * p.ntile * p.nchunk), dim3(GN_TS), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((gn_apply_kernel<E, ACT, Q, TAIL>), dim3(p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
+  const auto apply = !TAIL && p.past ? gn_apply_kernel<E, ACT, Q, TAIL, !TAIL> : gn_apply_kernel<E, ACT, Q, TAIL, false>;
+  hipLaunchKernelGGL(apply, dim3(p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
@@ -1000,7 +1002,8 @@ static int gn_run_bwd(const GnP &p, hipStream_t st) {
   }
   hipLaunchKernelGGL((gn_bwd_sums_kernel<E, ACT, Q8, TAIL>), dim3(p.N * p.ntile * p.nchunk), dim3(GN_TB), 0, st, p);
   TBG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((gn_bwd_dx_kernel<E, ACT, Q8, TAIL>), dim3(p.pblocks + p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
+  const auto second = !TAIL && p.past ? gn_bwd_dx_kernel<E, ACT, Q8, TAIL, !TAIL> : gn_bwd_dx_kernel<E, ACT, Q8, TAIL, false>;
+  hipLaunchKernelGGL(second, dim3(p.pblocks + p.N * p.ntile * p.nchunk * p.split), dim3(GN_T), 0, st, p);
   TBG_LAUNCH_CHECK();
   return TBG_OK;
 }
@@ -1025,6 +1028,12 @@ static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool backward, void *
          : d->dtype == TBG_DT_BF16 ? gn_run_type<ElBf16>(p, d->act, backward, st)
                                    : gn_run_type<ElF16>(p, d->act, backward, st);
 }
+// Calls that move more than the 256 MB of the card's memory-side cache write past the caches: the lines that they would leave to be written back
+// slow the next launch's reads.  32 x 16384 x 128 bf16 with 8-bit checkpoint (337 MB a direction): forward sums 33.8 -> 28.3, backward sums 55.9 ->
+// 48.4 us; smaller calls leave their results to the next reader (unpacking a 69 MB checkpoint takes 17.4 us, 19.3 if it was written past them).
+static bool gn_past(const tbg_gn_desc *d, int bytes) {
+  return (double)d->N * d->S * d->C * bytes > 256e6;
+}
 static bool gn_misaligned(const void *a, const void *b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) != 0; }
 
 extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const float *gamma, const float *beta, void *y, double *stats,
@@ -1035,6 +1044,7 @@ extern "C" int tbg_group_norm_fwd(const tbg_gn_desc *d, const void *x, const flo
   GnP p{};
   if (const int rc = gn_geometry(d, false, q || yq, p)) return rc;
   if (gn_part_bytes(p) > (workspace ? workspace_bytes : 0)) return TBG_EINVAL;
+  p.past = gn_past(d, 2 * dt_bytes(d->dtype) + (q != nullptr) + (yq != nullptr));
   p.x = x; p.gamma = gamma; p.beta = beta; p.y = y; p.stats = stats; p.part = reinterpret_cast<double *>(workspace);
   p.q = reinterpret_cast<unsigned char *>(q); p.e = reinterpret_cast<unsigned char *>(e);
   p.yq = reinterpret_cast<unsigned char *>(yq); p.ye = reinterpret_cast<unsigned char *>(ye);
@@ -1051,6 +1061,7 @@ extern "C" int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const voi
   GnP p{};
   if (const int rc = gn_geometry(d, true, false, p)) return rc;
   if (gn_part_bytes(p) + gn_pch_bytes(p) > (workspace ? workspace_bytes : 0)) return TBG_EINVAL;
+  p.past = gn_past(d, 2 * dt_bytes(d->dtype) + (q ? 1 : dt_bytes(d->dtype)));
   p.x = x; p.dy = dy; p.gamma = gamma; p.beta = beta; p.y = dx; p.stats = const_cast<double *>(stats);
   p.q = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(q));
   p.e = const_cast<unsigned char *>(reinterpret_cast<const unsigned char *>(e));
