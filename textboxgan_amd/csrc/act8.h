@@ -41,14 +41,20 @@ template <class E>
 struct Pack8 {
   typename E::type v[8];
 };
-template <class E>
+// PAST: read past the caches, which keep other lines
+template <bool PAST, class V, class T>
+__device__ __forceinline__ V ld_vec(const T *p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <class E, bool PAST = false>
 __device__ __forceinline__ Pack8<E> ld8(const typename E::type *p) {
   Pack8<E> r;
   if constexpr (E::BYTES == 2) {
-    const u32x4 w = *reinterpret_cast<const u32x4_any *>(p);
+    const u32x4 w = ld_vec<PAST, u32x4>(reinterpret_cast<const u32x4_any *>(p));
     __builtin_memcpy(&r, &w, 16);
   } else {
-    const f32x4 a = reinterpret_cast<const f32x4_any *>(p)[0], b = reinterpret_cast<const f32x4_any *>(p)[1];
+    const f32x4 a = ld_vec<PAST, f32x4>(reinterpret_cast<const f32x4_any *>(p)), b = ld_vec<PAST, f32x4>(reinterpret_cast<const f32x4_any *>(p) + 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { r.v[i] = a[i]; r.v[4 + i] = b[i]; }
   }
@@ -110,8 +116,9 @@ struct Row8 {
       off = C >= 8 ? C - 8 : 0;
     }
   }
+  template <bool PAST = false>
   __device__ __forceinline__ Pack8<E> load(const typename E::type *row) const {
-    if constexpr (!TAIL) return ld8<E>(row + off);
+    if constexpr (!TAIL) return ld8<E, PAST>(row + off);
     Pack8<E> r;
     if (C >= 8) {
       r = ld8<E>(row + off);

@@ -347,7 +347,7 @@ __global__ __launch_bounds__(GN_T) void gn_apply_kernel(GnP p) {
   for (; r + (U - 1) * RL < r1; r += U * RL) {
     Pack8<E> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u, x += xstep) v[u] = out.in ? out.row.load(x) : zero;
+    for (int u = 0; u < U; ++u, x += xstep) v[u] = out.in ? out.row.template load<PAST>(x) : zero;
 #pragma unroll
     for (int u = 0; u < U; ++u, y += ystep) out.write(v[u], y, row0 + r + u * RL);
   }
@@ -506,18 +506,19 @@ struct GnAt {
     q = p.q + at * p.nb * A8_BLOCK + c;
     e = p.e + at * p.nb + c / A8_BLOCK;
   }
+  template <bool PAST = false>
   __device__ __forceinline__ GnRow<E, Q8> next(const GnP &p, int rows) {
     GnRow<E, Q8> w;
     if constexpr (Q8) {
       w.e = *e;
-      w.q = *reinterpret_cast<const u32x2 *>(q);
+      w.q = ld_vec<PAST, u32x2>(reinterpret_cast<const u32x2 *>(q));
       q += (long long)rows * p.nb * A8_BLOCK;
       e += (long long)rows * p.nb;
     } else {
-      w.x = row.load(x);
+      w.x = row.template load<PAST>(x);
       x += rows * p.xs;
     }
-    w.g = row.load(g);
+    w.g = row.template load<PAST>(g);
     g += rows * p.ds;
     return w;
   }
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   for (; r + (U - 1) * RL < r1; r += U * RL) {
     GnRow<E, Q8> w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
+    for (int u = 0; u < U; ++u) w[u] = at.template next<PAST>(p, RL);
 #pragma unroll
     for (int u = 0; u < U; ++u) write(w[u]);
   }
@@ -1028,9 +1029,10 @@ static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool backward, void *
          : d->dtype == TBG_DT_BF16 ? gn_run_type<ElBf16>(p, d->act, backward, st)
                                    : gn_run_type<ElF16>(p, d->act, backward, st);
 }
-// Calls that move more than the 256 MB of the card's memory-side cache write past the caches: the lines that they would leave to be written back
-// slow the next launch's reads.  32 x 16384 x 128 bf16 with 8-bit checkpoint (337 MB a direction): forward sums 33.8 -> 28.3, backward sums 55.9 ->
-// 48.4 us; smaller calls leave their results to the next reader (unpacking a 69 MB checkpoint takes 17.4 us, 19.3 if it was written past them).
+// Calls that move more than the 256 MB of the card's memory-side cache read (for the second and last time) and write past the caches: lines that
+// are left to be written back slow the next launch's reads, and what the first launch has read stays for the second.  32 x 16384 x 128 bf16 with 8-bit
+// checkpoint (337 MB a direction): sums 33.8 -> 27.1, second launch 66 -> 54, backward sums 55.9 -> 48, second launch 63 -> 56 us.  Smaller calls
+// leave their results to the next reader (unpacking a 69 MB checkpoint takes 17.4 us, 19.3 if it was written past them).
 static bool gn_past(const tbg_gn_desc *d, int bytes) {
   return (double)d->N * d->S * d->C * bytes > 256e6;
 }
