@@ -13,8 +13,8 @@
 // mean(x^2) - mean^2 loses nothing that matters even where |mean| is 10^5 standard deviations, and no value of any type overflows.  The mean
 // is used as fp32 + its remainder.
 //
-// Measured (us): 32 x 16384 x 128 bf16, SiLU, 8-bit checkpoint: sums 28 (4.8 TB/s), second launch 69 (337 MB: 4.9), backward sums 49 and second
-// launch 62 (203 and 337 MB: 4.1, 5.4), whose two quarter-rate instructions a value are 34 us of vector time; 16 x 16384 x 128 forward 14 + 26.
+// Measured (us): 32 x 16384 x 128 bf16, SiLU, 8-bit checkpoint: sums 27 (5.0 TB/s), second launch 54-58 (337 MB: 5.8-6.2), backward sums 48-52
+// and second launch 56 (203 and 337 MB: 3.9-4.2, 6.0), whose two quarter-rate instructions a value are 34 us of vector time; 16 x 16384 x 128 forward 14 + 26.
 #include "act8.h"
 
 struct GnP {
