@@ -621,7 +621,8 @@ int tbg_demod_coefs_f32(const float *s, const float *w, float *wsq, float *d, in
  * scale 2^e: for a largest magnitude m 2^k (1 <= m < 2), e = k - 6, one more where 64 m >= 127.5, held in [-126, 121]; a value is
  * kept as q = x / 2^e rounded to the nearest integer (ties to even) within +-127, i.e. to amax / 127 or better; values of blocks below
  * 2^-120 are kept to 2^-127.  The scale being a power of two, q 2^e has 7 significant bits: exact in bf16, fp32.  A block that holds an
- * infinity or NaN comes back as NaN.  Storage: q int8 [rows][32 nb] (padding zero), e uint8 [rows][nb] = e + 127 (255: NaN block),
+ * infinity or NaN comes back as NaN.  Read as fp16, a value beyond +-65504 by at most half a step 2^e / 2 comes back as +-65504 (fp16's own largest
+ * values are kept as 65536), one further out as an infinity.  Storage: q int8 [rows][32 nb] (padding zero), e uint8 [rows][nb] = e + 127 (255: NaN block),
  * nb = ceil(C / 32); q 16-byte aligned.
  * tbg_act8_pack: x [rows][ldx] -> q, e.   tbg_act8_unpack: q, e -> x.
  *

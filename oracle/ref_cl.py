@@ -33,6 +33,16 @@ def unpack(q, e, shape):
     return v[:, :shape[-1]].reshape(shape)
 
 
+def unpack_as(q, e, shape, dtype):
+    """the values in `dtype`.  fp16 does not hold 65536 = 64 2^10, to which its own largest values are rounded: a kept value beyond +-65504 that
+    may stand for one of the type's (it lies within half a step of them) is the nearest of them"""
+    v = unpack(q, e, shape)
+    if dtype == torch.float16:
+        half = torch.where(e == 255, 0.0, pow2(e.int() - 127) / 2).repeat_interleave(32, dim=1)[:, :shape[-1]].reshape(shape)
+        v = torch.where(v.abs() - half <= 65504, v.clamp(-65504, 65504), v)
+    return v.to(dtype)
+
+
 def round_trip(x):
     return unpack(*pack(x), x.shape)
 

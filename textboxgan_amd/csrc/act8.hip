@@ -49,6 +49,13 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(const unsigned char *_
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = a8_value(w, i) * scale;
+  if constexpr (__is_same(E, ElF16)) {
+    // the largest values of fp16 itself (65280 .. 65504) are kept as 64 2^10 = 65536, which the type does not hold: a value that lies within half
+    // a step of the type's range is its end, values further out round to infinities (a NaN's comparison is false)
+    const float most = 65504.f + 0.5f * scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fabsf(v[i]) <= most ? fminf(fmaxf(v[i], -65504.f), 65504.f) : v[i];
+  }
   Row8<E, TAIL>(c, ch).store(x + row * ldx, put8<E>(v));
 }
 

@@ -167,7 +167,8 @@ def act8_pack(x: torch.Tensor) -> Act8:
 
 
 def act8_unpack(a: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """The values a checkpoint stands for, in the checkpointed tensor's shape and (unless ``dtype`` says otherwise) type."""
+    """The values a checkpoint stands for, in the checkpointed tensor's shape and (unless ``dtype`` says otherwise) type.  In fp16, values that
+    lie beyond the type's range by no more than half a step come back as its end (what fp16 holds from 65280 on is kept as 65536)."""
     _check8(a)
     dtype = a.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
