@@ -4,7 +4,7 @@ import torch
 
 from oracle import ref_cl as R
 from textboxgan_amd import ops_cl
-from test_ops_cl_gpu import values
+from test_ops_cl_gpu import ARITH, SUMS, affine, check, ids, train, values
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,29 @@ def test_fp16_output_checkpoint_stays_finite(dev):
     assert fine.any() and (y[fine] >= 65280).any()
     assert torch.isfinite(back[fine]).all() and torch.isnan(back[~fine]).all()
     assert ((back.double() - y.double())[fine].abs() <= 65504 / 127.5).all()
+
+
+# ---------------------------------------------------------------------------------------- group norm
+@pytest.mark.parametrize("save", ["input", "act8"])
+@pytest.mark.parametrize("act", ["linear", "lrelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+def test_gradients_over_the_whole_range(dev, dtype, act, save):
+    """one launch, a block of its own for every sample, and two launches; all groups of one size, and neighbouring groups far apart"""
+    for i, (n, s, ch, groups) in enumerate([(1, 40, 64, 4), (3, 30, 48, 12), (3, 700, 64, 4), (2, 1500, 40, 10), (2, 900, 35, 7)]):
+        for k in (-60, 60, 73, 100, 120):
+            for mixed in (False, True):
+                what = f"{n}x{s}x{ch} groups {groups} 2^{k} mixed {mixed}"
+                x = values((n, s, ch), torch.float32, dev, 210 + i, 0.2)
+                size = torch.full((ch,), 2.0 ** k, device=dev)
+                if mixed:
+                    size = torch.where(torch.arange(ch, device=dev) // (ch // groups) % 2 == 0, size, 1.0)
+                x = (x * size).to(dtype)
+                gamma, beta = affine(n, ch, i % 2 == 1, dev)
+                dy = values((n, s, ch), dtype, dev, 220 + i, 0.3)
+                eps = 1e-5 if k > 0 else 2.0 ** -130
+                y, dx, dg, db = train(x, gamma, beta, groups, dy, act=act, save=save, eps=eps)
+                o = R.group_norm(x, gamma, beta, groups, act, eps, dy, save)
+                check(y, o["y"], o["y_amp"], ARITH, f"{what} y")
+                check(dg, o["dgamma"], o["dgamma_amp"], SUMS, f"{what} dgamma")
+                check(db, o["dbeta"], o["dbeta_amp"], SUMS, f"{what} dbeta")
+                check(dx, o["dx"], o["dx_amp"], SUMS, f"{what} dx")

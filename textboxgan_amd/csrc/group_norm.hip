@@ -455,26 +455,44 @@ __global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
     if (w.rl + u * w.RL < p.S) out.write(v[u], y + (long long)(w.rl + u * w.RL) * p.C, row0 + w.rl + u * w.RL);
 }
 
-// ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd and z = sc d + be
+// ---- backward.  With d = x - mean (or its checkpoint), xh = d rstd and z = sc d + be.  Sums and dx take d times the power of two next to rstd (an
+// exact product): xh but for a factor of 1 to 2, so that neither dz d nor rstd^2 leaves the range that x and dx themselves are in.
+__device__ __forceinline__ float gn_power(double rstd) { return fmaxf(__uint_as_float(__float_as_uint((float)rstd) & 0x7f800000u), 0x1p-126f); }
+__device__ __forceinline__ double gn_factor(double rstd, float power) { return rstd * (double)__uint_as_float(0x7f000000u - __float_as_uint(power)); }
+// Two launches do without it where rstd is within 2^+-32
+__device__ __forceinline__ bool gn_far(double rstd) { return (unsigned)__double2hiint(rstd) - ((1023u - 32u) << 20) > 64u << 20; }
+__device__ __forceinline__ float gn_far_power(double rstd) { return gn_far(rstd) ? gn_power(rstd) : 1.f; }
 struct GnCh {
   float mu[8], mlo[8], sc[8], lo[8], be[8], za[8], zb[8];  // mean, scale: and their remainders; za, zb: sc, be times -log2(e), for the exponential
+  bool far;                                                // one of the wave's rstd is beyond 2^+-32
 };
 // st: mean, rstd of the groups from g0 on; sc, be come as gamma, beta
 template <bool Q8>
 __device__ __forceinline__ void gn_channels(const GnP &p, int c, const double2 *st, int g0, GnCh &h) {
   int g[8];
   gn_groups(p, c, g);
+  bool far = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const double2 s = st[g[i] - g0];
     h.mu[i] = Q8 ? 0.f : (float)s.x;
     h.mlo[i] = Q8 ? 0.f : (float)(s.x - (double)(float)s.x);
+    far |= gn_far(s.y);
     const double scale = s.y * (double)h.sc[i];
     h.sc[i] = (float)scale;
     h.lo[i] = (float)(scale - (double)h.sc[i]);
     h.za[i] = (float)(-1.44269504088896341 * scale);
     h.zb[i] = (float)(-1.44269504088896341 * (double)h.be[i]);
   }
+  h.far = __any(far);
+}
+// the channels' powers of two
+template <bool ALL>
+__device__ __forceinline__ void gn_powers(const GnP &p, int c, const double2 *st, int g0, float (&pw)[8]) {
+  int g[8];
+  gn_groups(p, c, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) pw[i] = ALL ? gn_power(st[g[i] - g0].y) : gn_far_power(st[g[i] - g0].y);
 }
 // a row's operands as they lie in memory
 template <class E, bool Q8>
@@ -562,25 +580,32 @@ __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
   __syncthreads();
   if (lane * 8 < t.ct) {
     gn_channels<Q8>(p, c, st, g0, h);
-    const auto add = [&](const GnRow<E, Q8> &w) {
+    const auto add = [&](const GnRow<E, Q8> &w, auto pw) {
       float d[8], dz[8];
       gn_row<E, ACT, Q8>(w, h, d, dz);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         s1[i] += dz[i];
-        s2[i] = fmaf(dz[i], d[i], s2[i]);
+        s2[i] = fmaf(dz[i], pw(d[i], i), s2[i]);
       }
     };
     int r = t.k * p.crows + rl;
     GnAt<E, Q8, TAIL> at(p, t.n, r, c);
-    for (; r + (U - 1) * RL < r1; r += U * RL) {
-      GnRow<E, Q8> w[U];
+    if (h.far) {  // (a loop of its own: that of ordinary values does without the registers)
+      float pw[8];
+      gn_powers<false>(p, c, st, g0, pw);
+      for (; r < r1; r += RL) add(at.next(p, RL), [&](float d, int i) { return d * pw[i]; });
+    } else {
+      const auto one = [](float d, int) { return d; };
+      for (; r + (U - 1) * RL < r1; r += U * RL) {
+        GnRow<E, Q8> w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
+        for (int u = 0; u < U; ++u) w[u] = at.next(p, RL);
 #pragma unroll
-      for (int u = 0; u < U; ++u) add(w[u]);
+        for (int u = 0; u < U; ++u) add(w[u], one);
+      }
+      for (; r < r1; r += RL) add(at.next(p, RL), one);
     }
-    for (; r < r1; r += RL) add(at.next(p, RL));
   }
   for (int off = p.lanes; off < 64; off <<= 1)
 #pragma unroll
@@ -601,7 +626,10 @@ __global__ __launch_bounds__(GN_TB, 4) void gn_bwd_sums_kernel(GnP p) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) a += red[w * 2 * p.CT + threadIdx.x];
     const int j = threadIdx.x >> 1;
-    if (threadIdx.x & 1) a *= (float)st[(t.c0 + j) / p.Cg - g0].y;  // d -> xh
+    if (threadIdx.x & 1) {  // -> xh
+      const double rstd = st[(t.c0 + j) / p.Cg - g0].y;
+      a *= (float)gn_factor(rstd, gn_far_power(rstd));
+    }
     p.pch[(((long long)t.n * p.nchunk + t.k) * p.C + t.c0) * 2 + threadIdx.x] = a;
     gred[threadIdx.x] = (double)p.gamma[(long long)t.n * p.affn + t.c0 + j] * (double)a;
   }
@@ -651,7 +679,7 @@ template <class E, int ACT, bool Q8, bool TAIL, bool PAST>
 __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   constexpr int U = 2;
   __shared__ double2 sh[2 * GN_CT];
-  double2 *st = sh, *stats = sh + GN_CT;  // of the tile's groups: rstd mean(gamma dz), rstd^2 mean(gamma dz xh); mean, rstd
+  double2 *st = sh, *stats = sh + GN_CT;  // of the tile's groups: rstd mean(gamma dz), rstd (times its factor) mean(gamma dz xh); mean, rstd
   int b = blockIdx.x;
   if (b < p.pblocks) {
     gn_param_sums(p, b, sh);
@@ -674,7 +702,7 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
     if ((threadIdx.x & (sub - 1)) == 0) {
       stats[i] = *reinterpret_cast<const double2 *>(p.stats + ((long long)t.n * p.G + g0 + i) * 2);
       const double rstd = stats[i].y;
-      st[i] = {rstd * (a / m), rstd * rstd * (q / m)};
+      st[i] = {rstd * (a / m), rstd * gn_factor(rstd, gn_far_power(rstd)) * (q / m)};
     }
   }
   __syncthreads();
@@ -695,22 +723,29 @@ __global__ __launch_bounds__(GN_T, 4) void gn_bwd_dx_kernel(GnP p) {
   int r = t.k * p.crows + piece * p.arows + rl;
   GnAt<E, Q8, TAIL> at(p, t.n, r, c);
   typename E::type *dx = reinterpret_cast<typename E::type *>(p.y) + ((long long)t.n * p.S + r) * p.C;
-  const auto write = [&](const GnRow<E, Q8> &w) {
+  const auto write = [&](const GnRow<E, Q8> &w, auto pw) {
     float d[8], dz[8];
     gn_row<E, ACT, Q8>(w, h, d, dz);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
+    for (int i = 0; i < 8; ++i) dz[i] = fmaf(-pw(d[i], i), m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
     at.row.template store<PAST>(dx, put8<E>(dz));
     dx += (long long)RL * p.C;
   };
+  if (h.far) {
+    float pw[8];
+    gn_powers<false>(p, c, stats, g0, pw);
+    for (; r < r1; r += RL) write(at.template next<PAST>(p, RL), [&](float d, int i) { return d * pw[i]; });
+    return;
+  }
+  const auto one = [](float d, int) { return d; };
   for (; r + (U - 1) * RL < r1; r += U * RL) {
     GnRow<E, Q8> w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = at.template next<PAST>(p, RL);
 #pragma unroll
-    for (int u = 0; u < U; ++u) write(w[u]);
+    for (int u = 0; u < U; ++u) write(w[u], one);
   }
-  for (; r < r1; r += RL) write(at.next(p, RL));
+  for (; r < r1; r += RL) write(at.next(p, RL), one);
 }
 
 // ---- backward in one launch (teams as in the forward one): x (or its checkpoint) and dy are read once.  The parameters' gradients are summed
@@ -721,7 +756,7 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
   extern __shared__ __align__(16) char smem[];
   const GnTeam w(p);
   const int tile = blockIdx.x % p.ntile, chunk = blockIdx.x / p.ntile, c0 = tile * p.CT, ct = min(p.CT, p.C - c0), c = c0 + w.lane * 8, g0 = c0 / p.Cg;
-  double2 *st = reinterpret_cast<double2 *>(smem) + w.id * p.ng;  // of the tile's groups: mean(sc dz), rstd^2 mean(sc dz d)
+  double2 *st = reinterpret_cast<double2 *>(smem) + w.id * p.ng;  // of the tile's groups: mean(sc dz), mean(sc dz d) times rstd's factor squared
   float *reds = reinterpret_cast<float *>(reinterpret_cast<double2 *>(smem) + p.nteam * p.ng);
   float *red = reds + w.id * w.nparts * p.CT * 2;  // [nparts][CT][2]
   const bool in = w.lane * 8 < ct;
@@ -734,7 +769,7 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
     const int n = at < p.N ? (int)at : 0;
     GnRow<E, Q8> row[R];
     GnCh h;
-    float s1[8], s2[8];
+    float pw[8], s1[8], s2[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) s1[i] = s2[i] = 0.f;
     if (live) {
@@ -744,6 +779,7 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
         if (w.rl + u * w.RL < p.S) row[u] = from.next(p, w.RL);
       gn_affine<TAIL>(p, n, c, h.sc, h.be);
       gn_channels<Q8>(p, c, reinterpret_cast<const double2 *>(p.stats) + (long long)n * p.G, 0, h);
+      gn_powers<true>(p, c, reinterpret_cast<const double2 *>(p.stats) + (long long)n * p.G, 0, pw);
 #pragma unroll
       for (int u = 0; u < R; ++u)
         if (w.rl + u * w.RL < p.S) {
@@ -752,7 +788,7 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             s1[i] += dz[i];
-            s2[i] = fmaf(dz[i], d[i], s2[i]);
+            s2[i] = fmaf(dz[i], pw[i] * d[i], s2[i]);
           }
         }
     }
@@ -783,7 +819,7 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
       gn_groups(p, c, g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float xh = s2[i] * (float)p.stats[((long long)n * p.G + g[i]) * 2 + 1];
+        const float xh = s2[i] * (float)gn_factor(p.stats[((long long)n * p.G + g[i]) * 2 + 1], pw[i]);
         if (p.affn) {
           if (!TAIL || c + i < p.C) {
             p.dbeta[(long long)n * p.C + c + i] = s1[i];
@@ -799,8 +835,8 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
     }
     __syncthreads();
     w.groups(p, ct, (ct + p.Cg - 1) / p.Cg, 1, red, [&](int i, const double2 &o) {
-      const double rstd = p.stats[((long long)n * p.G + g0 + i) * 2 + 1], m = (double)p.S * p.Cg;
-      st[i] = {o.x / m, rstd * rstd * (o.y / m)};
+      const double rstd = p.stats[((long long)n * p.G + g0 + i) * 2 + 1], f = gn_factor(rstd, gn_power(rstd)), m = (double)p.S * p.Cg;
+      st[i] = {o.x / m, f * f * (o.y / m)};
     });
     __syncthreads();
     if (live) {
@@ -824,7 +860,7 @@ __global__ __launch_bounds__(GN_T, 2) void gn_bwd_whole_kernel(GnP p) {
           else gn_opaque(row[u].x);
           gn_row<E, ACT, Q8>(row[u], h, d, dz);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dz[i] = fmaf(-d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
+          for (int i = 0; i < 8; ++i) dz[i] = fmaf(-pw[i] * d[i], m2[i], fmaf(dz[i], h.sc[i], -m1[i]));
           to.store(dx + (long long)(w.rl + u * w.RL) * p.C, put8<E>(dz));
         }
     }
