@@ -1,7 +1,10 @@
 """Channels-last layers at the ends of their types' ranges and next to callers' modes (no GPU)."""
+import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle import ref_cl as R
+from textboxgan_amd import native, ops_cl
 
 
 def test_the_format_read_as_fp16():
@@ -15,3 +18,51 @@ def test_the_format_read_as_fp16():
     assert ((v.double() - x.double()).abs() <= torch.clamp(x.double().abs() / 127.5, min=2.0 ** -25)).all()
     far = torch.tensor([[66560.0], [-70000.0], [3e38]])  # what no fp16 value can have been stays beyond its range
     assert torch.isinf(R.unpack_as(*R.pack(far), far.shape, torch.float16)).all()
+
+
+def a8(shape, dtype=torch.float32):
+    rows, nb = shape[0], (shape[-1] + 31) // 32
+    return ops_cl.Act8(torch.zeros(rows, nb * 32, dtype=torch.int8), torch.zeros(rows, nb, dtype=torch.uint8), shape, dtype)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", range(3))
+def test_a_group_norm_refuses_forward_mode(which, grad):
+    """no result that has lost its tangent: refused before anything runs, whether or not reverse mode is on as well"""
+    ops = [torch.ones(2, 3, 8), torch.ones(8), torch.zeros(8)]
+    with forward_ad.dual_level():
+        ops[which] = forward_ad.make_dual(ops[which], torch.ones_like(ops[which]))
+        if grad:
+            ops[0].requires_grad_()
+        with pytest.raises(native.TbgError, match="forward-mode"):
+            ops_cl.group_norm_act(*ops, 2)
+        with torch.no_grad(), pytest.raises(native.TbgError, match="forward-mode"):
+            ops_cl.group_norm_act(*ops, 2)
+        with pytest.raises(native.TbgError, match="device tensors"):  # (no operand has a tangent)
+            ops_cl.group_norm_act(torch.ones(2, 3, 8), torch.ones(8), torch.zeros(8), 2)
+
+
+def test_backward_passes_refuse_forward_mode(monkeypatch):
+    """a dual output gradient: the kernels would answer with its value alone"""
+    monkeypatch.setattr(ops_cl, "_gn_fwd", lambda x, *a: (x.detach().clone(), torch.zeros(1), None, None, None))
+    x, w = torch.ones(4, 8, requires_grad=True), torch.ones(8, 8)
+    y = ops_cl._GroupNormAct.apply(x, torch.ones(8), torch.zeros(8), (2, 0, 1e-5), False, False, [])
+    z = ops_cl._DenseAct8.apply(x, w, None, 1.0, None, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(4, 8), torch.ones(4, 8))
+        for out in (y, z):
+            with pytest.raises(native.TbgError, match="forward-mode"):
+                torch.autograd.grad(out, x, dual, retain_graph=True)
+        with pytest.raises(native.TbgError, match="forward-mode"):
+            ops_cl.act8_wgrad(a8((4, 40)), dual)
+    assert torch.equal(torch.autograd.grad(z, x, torch.ones(4, 8))[0], torch.full((4, 8), 8.0))
+
+
+def test_a_dense_layer_without_reverse_mode_keeps_tangents(monkeypatch):
+    monkeypatch.setattr(ops_cl, "_placed", lambda *a: None)
+    x, w, t = torch.randn(4, 8), torch.randn(8, 3), torch.randn(4, 8)
+    with forward_ad.dual_level():
+        y = ops_cl.dense_act8(forward_ad.make_dual(x, t), w, coef=0.5)
+        assert torch.allclose(forward_ad.unpack_dual(y).tangent, 0.5 * t @ w, atol=1e-6)
+        with pytest.raises(RuntimeError, match="jvp"):  # (torch's own refusal of a function that has none)
+            ops_cl.dense_act8(forward_ad.make_dual(x, t), w.clone().requires_grad_(), x8=a8((4, 8)))

@@ -11,7 +11,8 @@ pass read that form directly:
 * ``dense_act8``                        dense (1x1) layer whose input is kept in 8 bits only
 * ``act8_wgrad``                        its weight and bias gradients, straight from the checkpoint
 
-Parameters and their gradients are fp32 in every mode, as in ``ops``.  First order: the backward passes are not themselves differentiable.
+Parameters and their gradients are fp32 in every mode, as in ``ops``.  First order, reverse mode: the backward passes are not themselves
+differentiable, and dual tensors of forward-mode differentiation are refused (``dense_act8`` without reverse-mode gradients takes them).
 Everything is enqueued on the current stream and can be captured into a graph; a backward pass is captured where no graph made on the default
 stream from the same leaves is alive (these functions refuse the leaves of one that they have seen).
 Inputs whose rows are not evenly spaced with contiguous channels are copied once (``contiguous()``); slices of wider tensors are not.
@@ -22,6 +23,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native as N
 
@@ -72,6 +74,12 @@ def _check(t, what: str, dtypes):
         raise N.TbgError(f"{what}: a tensor is wanted, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise N.TbgError(f"{what}: unsupported dtype {t.dtype}")
+
+
+def _no_tangents(what: str, *ts):
+    """no operand is a dual tensor of forward-mode differentiation: the kernels would drop its tangent without a word"""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise N.TbgError(f"{what}: forward-mode derivatives are not implemented (an operand is a dual tensor)")
 
 
 def _most(what: str, size: int, limit: int, name: str):
@@ -188,6 +196,7 @@ def act8_wgrad(a: Act8, dy: torch.Tensor, coef: float = 1.0, want_db: bool = Tru
     if dy.dim() < 1 or dy.shape[-1] < 1 or tuple(dy.shape[:-1]) != tuple(a.shape[:-1]):
         raise N.TbgError(f"act8_wgrad: a gradient {tuple(dy.shape)} does not belong to a checkpoint of {tuple(a.shape)}")
     _most("act8_wgrad", max(cin, dy.shape[-1]), MAX_DENSE, "channels")
+    _no_tangents("act8_wgrad", dy)
     _placed("act8_wgrad", a.q, a.e, dy)
     cout, dev = dy.shape[-1], dy.device
     if not a.rows:
@@ -289,6 +298,7 @@ class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_tangents("group_norm_act backward", dy)
         gamma, beta, stats, *kept = ctx.saved_tensors
         x, q, e = (None, *kept) if len(kept) == 2 else (kept[0], None, None)
         dx, dgamma, dbeta = _gn_bwd(x, q, e, dy, gamma, beta, stats, ctx.cfg)
@@ -323,6 +333,7 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
     _check(beta, "group_norm_act: beta", (torch.float32,))
     if tuple(gamma.shape) not in ((ch,), (n, ch)) or gamma.shape != beta.shape:
         raise N.TbgError(f"group_norm_act: gamma {tuple(gamma.shape)} and beta {tuple(beta.shape)} have to be ({ch},) or ({n}, {ch}) alike")
+    _no_tangents("group_norm_act", x, gamma, beta)
     _placed("group_norm_act", x, gamma, beta)
     grad = torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad)
     if x.numel() == 0:
@@ -365,6 +376,7 @@ class _DenseAct8(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_tangents("dense_act8 backward", dy)
         q, e, w = ctx.saved_tensors
         shape, dtype, coef = ctx.cfgv
         need = ctx.needs_input_grad
