@@ -66,3 +66,14 @@ def test_a_dense_layer_without_reverse_mode_keeps_tangents(monkeypatch):
         assert torch.allclose(forward_ad.unpack_dual(y).tangent, 0.5 * t @ w, atol=1e-6)
         with pytest.raises(RuntimeError, match="jvp"):  # (torch's own refusal of a function that has none)
             ops_cl.dense_act8(forward_ad.make_dual(x, t), w.clone().requires_grad_(), x8=a8((4, 8)))
+
+
+def test_a_data_gradient_inside_autocast():
+    """the product of the backward pass runs in its operands' type, as that of the forward pass does"""
+    x, w = torch.randn(40, 72, requires_grad=True), torch.randn(72, 30)
+    dy = torch.randn(40, 30)
+    want = torch.autograd.grad(ops_cl._DenseAct8.apply(x, w, None, 0.5, None, None), x, dy)[0]
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = ops_cl._DenseAct8.apply(x, w, None, 0.5, None, None)
+        got = torch.autograd.grad(y, x, dy)[0]
+    assert y.dtype == got.dtype == torch.float32 and torch.equal(got, want)

@@ -1,10 +1,10 @@
-"""-m gpu: channels-last layers at the ends of their types' ranges, against their definitions in 64 bits (oracle/ref_cl.py).  Tolerances are those of test_ops_cl_gpu.py."""
+"""-m gpu: channels-last layers at the ends of their types' ranges and next to callers' modes, against their definitions in 64 bits (oracle/ref_cl.py).  Tolerances are those of test_ops_cl_gpu.py."""
 import pytest
 import torch
 
 from oracle import ref_cl as R
 from textboxgan_amd import ops_cl
-from test_ops_cl_gpu import ARITH, SUMS, affine, check, ids, train, values
+from test_ops_cl_gpu import ARITH, SUMS, TYPES, affine, check, ids, train, values
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,19 @@ def test_gradients_over_the_whole_range(dev, dtype, act, save):
                 check(dg, o["dgamma"], o["dgamma_amp"], SUMS, f"{what} dgamma")
                 check(db, o["dbeta"], o["dbeta_amp"], SUMS, f"{what} dbeta")
                 check(dx, o["dx"], o["dx_amp"], SUMS, f"{what} dx")
+
+
+# ---------------------------------------------------------------------------------------- callers' modes
+def test_backward_inside_autocast(dev):
+    """the gradients of a dense layer do not hang on an autocast region around the backward pass"""
+    for dtype in TYPES:
+        x = values((50, 72), dtype, dev, 230).requires_grad_()
+        w = (0.1 * values((72, 40), torch.float32, dev, 231)).requires_grad_()
+        b = values((40,), torch.float32, dev, 232).requires_grad_()
+        dy = values((50, 40), dtype, dev, 233)
+        want = torch.autograd.grad(ops_cl.dense_act8(x, w, b, coef=0.5), (x, w, b), dy)
+        for low in (torch.float16, torch.bfloat16):
+            with torch.autocast("cuda", dtype=low):
+                y = ops_cl.dense_act8(x, w, b, coef=0.5)
+                got = torch.autograd.grad(y, (x, w, b), dy)
+            assert all(torch.equal(u, v) and u.dtype == v.dtype for u, v in zip(got, want)), (dtype, low)

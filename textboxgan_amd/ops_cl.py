@@ -20,6 +20,7 @@ Inputs whose rows are not evenly spaced with contiguous channels are copied once
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -352,14 +353,29 @@ def group_norm_act(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, gro
 # ----------------------------------------------------------------------------------------
 # dense (1x1) layer on an 8-bit checkpoint
 # ----------------------------------------------------------------------------------------
+def _own_types(fn):
+    """fn(tensor, ...) outside the caller's autocast: its products run in the types of its operands"""
+    @functools.wraps(fn)
+    def call(t, *args):
+        kind = t.device.type
+        if not torch.is_autocast_enabled(kind):
+            return fn(t, *args)
+        with torch.autocast(kind, enabled=False):
+            return fn(t, *args)
+    return call
+
+
+@_own_types
 def _dense_fwd(x, w, b, coef):
-    if torch.is_autocast_enabled("cuda"):  # y is in x's type whatever the caller's autocast
-        with torch.autocast("cuda", enabled=False):
-            return _dense_fwd(x, w, b, coef)
     y = x.reshape(-1, w.shape[0]) @ (w * coef).to(x.dtype)
     if b is not None:
         y = y + b.to(x.dtype)
     return y.reshape(*x.shape[:-1], w.shape[1])
+
+
+@_own_types
+def _dense_dx(dy, w, coef, shape, dtype):
+    return (dy.reshape(-1, w.shape[1]) @ (w * coef).to(dtype).t()).reshape(shape)
 
 
 class _DenseAct8(torch.autograd.Function):
@@ -382,7 +398,7 @@ class _DenseAct8(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0]:
-            dx = (dy.reshape(-1, w.shape[1]) @ (w * coef).to(dtype).t()).reshape(shape)
+            dx = _dense_dx(dy, w, coef, shape, dtype)
         if need[1]:
             dw, db = act8_wgrad(Act8(q, e, shape, dtype), dy, coef, need[2])
         elif need[2]:
