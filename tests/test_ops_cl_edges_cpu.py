@@ -1,10 +1,14 @@
 """Channels-last layers at the ends of their types' ranges and next to callers' modes (no GPU)."""
+import os
+import re
+import subprocess
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from oracle import ref_cl as R
-from textboxgan_amd import native, ops_cl
+from textboxgan_amd import build, native, ops_cl
 
 
 def test_the_format_read_as_fp16():
@@ -77,3 +81,21 @@ def test_a_data_gradient_inside_autocast():
         y = ops_cl._DenseAct8.apply(x, w, None, 0.5, None, None)
         got = torch.autograd.grad(y, x, dy)[0]
     assert y.dtype == got.dtype == torch.float32 and torch.equal(got, want)
+
+
+def test_rows_are_moved_at_their_own_alignment(tmp_path):
+    """the 8-channel loads and stores of the channels-last kernels promise the compiler no more than a row's element alignment (rows begin at any
+    element), and the header compiles without a word about it"""
+    src = tmp_path / "rows.hip"
+    src.write_text('#include "act8.h"\n' + "\n".join(f"""
+__global__ void copy_{e}_{past}(const {e}::type *x, {e}::type *y) {{
+  const Pack8<{e}> r = ld8<{e}, {past}>(x + threadIdx.x * 9);
+  st8<{e}, {past}>(y + threadIdx.x * 9, r);
+}}""" for e in ("ElF32", "ElBf16", "ElF16") for past in ("false", "true")) + "\n")
+    out = tmp_path / "rows.ll"
+    run = subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), *build.FLAGS, "-I", build.CSRC, "--cuda-device-only", "-S", "-emit-llvm", str(src),
+                          "-o", str(out)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
+    assert "aligned" not in run.stderr, run.stderr
+    moves = re.findall(r"(?:load|store) <4 x (i32|float)>.*align (\d+)", out.read_text())
+    assert len(moves) == 2 * 2 * (2 + 1 + 1) and all(int(a) <= (4 if t == "float" else 2) for t, a in moves), moves

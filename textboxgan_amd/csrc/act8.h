@@ -33,7 +33,8 @@ struct ElF16 {
   }
 };
 
-// 8 neighbouring channels of a row, moved in 16-byte pieces wherever the row begins: the card takes them at any address
+// 8 neighbouring channels of a row, moved in 16-byte pieces wherever the row begins: the card takes them at any address.  The alignment belongs to
+// the typedef and not to the vector type, so a template's deduced parameter would lose it: the functions below name their pointers' types.
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
@@ -42,8 +43,18 @@ struct Pack8 {
   typename E::type v[8];
 };
 // PAST: read past the caches, which keep other lines
-template <bool PAST, class V, class T>
-__device__ __forceinline__ V ld_vec(const T *p) {
+template <bool PAST>
+__device__ __forceinline__ u32x4 ld_vec(const u32x4_any *p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool PAST>
+__device__ __forceinline__ f32x4 ld_vec(const f32x4_any *p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool PAST>
+__device__ __forceinline__ u32x2 ld_vec(const u32x2 *p) {
   if constexpr (PAST) return __builtin_nontemporal_load(p);
   else return *p;
 }
@@ -51,18 +62,28 @@ template <class E, bool PAST = false>
 __device__ __forceinline__ Pack8<E> ld8(const typename E::type *p) {
   Pack8<E> r;
   if constexpr (E::BYTES == 2) {
-    const u32x4 w = ld_vec<PAST, u32x4>(reinterpret_cast<const u32x4_any *>(p));
+    const u32x4 w = ld_vec<PAST>(reinterpret_cast<const u32x4_any *>(p));
     __builtin_memcpy(&r, &w, 16);
   } else {
-    const f32x4 a = ld_vec<PAST, f32x4>(reinterpret_cast<const f32x4_any *>(p)), b = ld_vec<PAST, f32x4>(reinterpret_cast<const f32x4_any *>(p) + 1);
+    const f32x4 a = ld_vec<PAST>(reinterpret_cast<const f32x4_any *>(p)), b = ld_vec<PAST>(reinterpret_cast<const f32x4_any *>(p + 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i) { r.v[i] = a[i]; r.v[4 + i] = b[i]; }
   }
   return r;
 }
 // PAST: written past the caches, whose other lines stay
-template <bool PAST, class T, class V>
-__device__ __forceinline__ void st_vec(T *p, const V &v) {
+template <bool PAST>
+__device__ __forceinline__ void st_vec(u32x4_any *p, u32x4 v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <bool PAST>
+__device__ __forceinline__ void st_vec(f32x4_any *p, f32x4 v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <bool PAST>
+__device__ __forceinline__ void st_vec(u32x2 *p, u32x2 v) {
   if constexpr (PAST) __builtin_nontemporal_store(v, p);
   else *p = v;
 }
@@ -74,8 +95,14 @@ __device__ __forceinline__ void st8(typename E::type *p, const Pack8<E> &r) {
     st_vec<PAST>(reinterpret_cast<u32x4_any *>(p), w);
   } else {
     st_vec<PAST>(reinterpret_cast<f32x4_any *>(p), f32x4{r.v[0], r.v[1], r.v[2], r.v[3]});
-    st_vec<PAST>(reinterpret_cast<f32x4_any *>(p) + 1, f32x4{r.v[4], r.v[5], r.v[6], r.v[7]});
+    st_vec<PAST>(reinterpret_cast<f32x4_any *>(p + 4), f32x4{r.v[4], r.v[5], r.v[6], r.v[7]});
   }
+}
+// 8 bf16 values to LDS, at a multiple of 16 bytes
+__device__ __forceinline__ void st8_lds(unsigned short *p, const Pack8<ElBf16> &r) {
+  u32x4 w;
+  __builtin_memcpy(&w, &r, 16);
+  *reinterpret_cast<u32x4 *>(p) = w;
 }
 // moved down by k elements (k the same in all lanes), zeros above
 template <class E>

@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = a8_value(g.xq[i], j) * s;
-      st8<ElBf16>(buf + (xrow + XR * i) * PK + xc, put8<ElBf16>(v));
+      st8_lds(buf + (xrow + XR * i) * PK + xc, put8<ElBf16>(v));
     }
 #pragma unroll
     for (int i = 0; i < DN; ++i) {
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
         a8w_terms<NP>(v, w);
       }
 #pragma unroll
-      for (int m = 0; m < NP; ++m) st8<ElBf16>(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
+      for (int m = 0; m < NP; ++m) st8_lds(buf + A8W_RB * PK + (m * A8W_RB + drow + DR * i) * PN + dc, w[m]);
     }
   };
   auto column_sums = [&](const Regs &g) {

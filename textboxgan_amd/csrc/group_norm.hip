@@ -529,7 +529,7 @@ struct GnAt {
     GnRow<E, Q8> w;
     if constexpr (Q8) {
       w.e = *e;
-      w.q = ld_vec<PAST, u32x2>(reinterpret_cast<const u32x2 *>(q));
+      w.q = ld_vec<PAST>(reinterpret_cast<const u32x2 *>(q));
       q += (long long)rows * p.nb * A8_BLOCK;
       e += (long long)rows * p.nb;
     } else {
