@@ -442,12 +442,8 @@ __device__ __forceinline__ void dense_fwd_body(const DenseP &p, const int bx, co
 #pragma unroll
         for (int r = 0; r < DN_RT; ++r) {
           const float4 xv = *reinterpret_cast<const float4 *>(&xs[r * KP + k0 + j]);
-          // One of the first two products is rounded by itself, the other is fused: which one is spelled out, so that the results do not
-          // hang on the compiler's choice.  (The recorded ones come from a build that took them in this pattern; random-weight training
-          // steps in bf16 answer to a style's last bit.)
-          const bool second = ((r ^ (r >> 3) ^ (j >= 40)) & 1) != 0;
-          const float first = second ? fmaf(xv.x, wv[j], xv.y * wv[j + 1]) : fmaf(xv.y, wv[j + 1], xv.x * wv[j]);
-          acc[r] += fmaf(xv.w, wv[j + 3], fmaf(xv.z, wv[j + 2], first));
+          // (one order for all rows and columns, spelled out: a row's result does not depend on its place in the batch, nor on the compiler)
+          acc[r] += fmaf(xv.w, wv[j + 3], fmaf(xv.z, wv[j + 2], fmaf(xv.x, wv[j], xv.y * wv[j + 1])));
         }
       }
     }
