@@ -99,3 +99,10 @@ __global__ void copy_{e}_{past}(const {e}::type *x, {e}::type *y) {{
     assert "aligned" not in run.stderr, run.stderr
     moves = re.findall(r"(?:load|store) <4 x (i32|float)>.*align (\d+)", out.read_text())
     assert len(moves) == 2 * 2 * (2 + 1 + 1) and all(int(a) <= (4 if t == "float" else 2) for t, a in moves), moves
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_checkpoint_of_another_type_is_refused(dtype):
+    for other in (torch.float32, torch.bfloat16, torch.float16):
+        with pytest.raises(native.TbgError, match="device tensors" if other == dtype else "is not one of"):
+            ops_cl.dense_act8(torch.zeros(2, 40, dtype=dtype), torch.zeros(40, 4), x8=a8((2, 40), other))

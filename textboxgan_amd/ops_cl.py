@@ -420,8 +420,8 @@ def dense_act8(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = Non
             raise N.TbgError(f"dense_act8: bias {tuple(b.shape)}, ({w.shape[1]},) is wanted")
     if x8 is not None:
         _check8(x8)
-        if tuple(x8.shape) != tuple(x.shape):
-            raise N.TbgError(f"dense_act8: a checkpoint of {tuple(x8.shape)} is not one of the input {tuple(x.shape)}")
+        if tuple(x8.shape) != tuple(x.shape) or x8.dtype != x.dtype:
+            raise N.TbgError(f"dense_act8: a checkpoint of {tuple(x8.shape)} {x8.dtype} is not one of the input {tuple(x.shape)} {x.dtype}")
     _placed("dense_act8", x, w, *(() if b is None else (b,)), *(() if x8 is None else (x8.q, x8.e)))
     coef = float(coef)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b)):
