@@ -106,3 +106,15 @@ def test_a_checkpoint_of_another_type_is_refused(dtype):
     for other in (torch.float32, torch.bfloat16, torch.float16):
         with pytest.raises(native.TbgError, match="device tensors" if other == dtype else "is not one of"):
             ops_cl.dense_act8(torch.zeros(2, 40, dtype=dtype), torch.zeros(40, 4), x8=a8((2, 40), other))
+
+
+@pytest.mark.parametrize("dtype, terms", [(0, 3), (1, 1), (2, 2)])
+@pytest.mark.parametrize("cin, cout, tk, tn, regs", [(128, 128, 128, 128, 2), (256, 256, 128, 128, 2), (128, 64, 128, 64, 2), (64, 128, 64, 128, 2), (64, 64, 64, 64, 4)])
+def test_weight_gradients_fill_the_card_once(dtype, terms, cin, cout, tk, tn, regs):
+    """many rows are split over as many blocks as 256 CUs hold at once (by registers, and by the 160 KB of LDS that three buffers of 32 rows share)"""
+    if dtype == 1 and cin == cout == 256:
+        tk, tn, regs = 256, 256, 1  # (bf16 has a wider tile)
+    lds = 3 * 32 * (tk + 32 + terms * (tn + 32)) * 2
+    rows = 1 << 20
+    splits, left = divmod(native.lib().tbg_act8_wgrad_workspace_bytes(rows, cin, cout, dtype), (cin + 1) * cout * 4)
+    assert left == 0 and splits * -(-cin // tk) * -(-cout // tn) == 256 * min(regs, 160 * 1024 // lds)

@@ -303,7 +303,10 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, c
 }
 
 // Tile and row splits.  The tile: the largest that the channels fill (fewer re-reads of both operands, fewer operand reads an MFMA), made
-// smaller while splits of 256 rows would leave a quarter of the CUs without a block; the splits then fill the card once.  Measured, us of kernels:
+// smaller while splits of 256 rows would leave a quarter of the CUs without a block; the splits then fill the card once: as many blocks a CU as its
+// registers and its 160 KB of LDS hold (the three buffers take 60 KB for 128 x 128 of one term, 120 KB of three).  Calls, us, with the splits of one
+// round of blocks / of two: fp32 65536 x 256 x 256 44 / 50, 262144 x 64 x 64 24 / 30, 262144 x 512 x 512 512 / 520; fp16 36 / 43, 20.6 / 26.6, but
+// 262144 x 512 x 512 407 / 391.  Measured, us of kernels:
 // 262144 x 512 x 512 bf16 158 + 12 (join) with 256 x 256 tiles, 200 with 128 x 128; fp32 (three terms: 256 x 256 tiles do not fit the registers)
 // 16384 x 256 x 256 20 + 4 with 128 x 128 tiles.  Few rows (512, fp32 256) are not split: the second launch and the partial sums cost what the split
 // saves (512 x 512 x 512 bf16 10.1 / 10.0, 256 rows 7.2 / 9.0, 512 x 64 x 64 8.6 / 7.2) and a call takes 13.4 instead of 17.8 us of the host.
@@ -312,9 +315,10 @@ struct A8wGeo {
   long long rsplit;
 };
 struct A8wForm {
-  int tk, tn, per_cu;
+  int tk, tn, per_cu;  // blocks that a CU's registers take
 };
 static constexpr A8wForm A8W_FORMS[] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 2}, {64, 128, 2}, {64, 64, 4}};
+static constexpr long long a8w_lds(int tk, int tn, int terms) { return 3LL * A8W_RB * (tk + A8W_PAD + terms * (tn + A8W_PAD)) * 2; }
 static A8wGeo a8w_geometry(long long rows, int cin, int cout, int dtype) {
   A8wGeo g;
   const long long most = (rows + 8 * A8W_RB - 1) / (8 * A8W_RB);
@@ -323,7 +327,9 @@ static A8wGeo a8w_geometry(long long rows, int cin, int cout, int dtype) {
     g.tn = (cout + A8W_FORMS[g.form].tn - 1) / A8W_FORMS[g.form].tn;
     if ((long long)g.tk * g.tn * most >= 192 || g.form == 4) break;
   }
-  long long want = 256LL * A8W_FORMS[g.form].per_cu / ((long long)g.tk * g.tn);
+  const A8wForm &f = A8W_FORMS[g.form];
+  const long long fits = 160 * 1024 / a8w_lds(f.tk, f.tn, dtype == TBG_DT_F32 ? 3 : dtype == TBG_DT_F16 ? 2 : 1);
+  long long want = 256LL * (f.per_cu < fits ? f.per_cu : fits) / ((long long)g.tk * g.tn);
   const long long cap = rows <= (dtype == TBG_DT_F32 ? 256 : 512) ? 1 : g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
   if (want > cap) want = cap;
   if (want < 1) want = 1;
@@ -351,7 +357,7 @@ extern "C" long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int
 
 template <class E, int NP, int WM, int WN, int KW, int NW>
 static int a8w_launch(const A8wP &p, bool vec, hipStream_t st) {
-  constexpr size_t lds = 3 * (size_t)A8W_RB * (32 * WM * KW + A8W_PAD + NP * (32 * WN * NW + A8W_PAD)) * 2;
+  constexpr size_t lds = a8w_lds(32 * WM * KW, 32 * WN * NW, NP);
   const unsigned blocks = (unsigned)((p.nsplit + 7) / 8 * 8 * p.tk * p.tn);
   const auto kern = vec ? act8_wgrad_kernel<E, NP, WM, WN, KW, NW, true> : act8_wgrad_kernel<E, NP, WM, WN, KW, NW, false>;
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
