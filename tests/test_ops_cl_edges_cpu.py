@@ -118,3 +118,11 @@ def test_weight_gradients_fill_the_card_once(dtype, terms, cin, cout, tk, tn, re
     rows = 1 << 20
     splits, left = divmod(native.lib().tbg_act8_wgrad_workspace_bytes(rows, cin, cout, dtype), (cin + 1) * cout * 4)
     assert left == 0 and splits * -(-cin // tk) * -(-cout // tn) == 256 * min(regs, 160 * 1024 // lds)
+
+
+@pytest.mark.parametrize("dtype, narrow, wide", [(0, 256, 192), (1, 512, 384), (2, 512, 256)])
+def test_weight_gradients_of_few_rows_take_one_launch(dtype, narrow, wide):
+    """up to where a second launch pays: less rows where the product is so wide that the call is not the host's"""
+    space = native.lib().tbg_act8_wgrad_workspace_bytes
+    for rows, cin, cout in ((narrow, 512, 512), (narrow, 64, 64), (narrow, 512, 1023), (wide, 512, 1024), (wide, 1024, 1024)):
+        assert space(rows, cin, cout, dtype) == 0 < space(rows + 1, cin, cout, dtype), (rows, cin, cout)

@@ -308,14 +308,21 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, c
 // round of blocks / of two: fp32 65536 x 256 x 256 44 / 50, 262144 x 64 x 64 24 / 30, 262144 x 512 x 512 512 / 520; fp16 36 / 43, 20.6 / 26.6, but
 // 262144 x 512 x 512 407 / 391.  Measured, us of kernels:
 // 262144 x 512 x 512 bf16 158 + 12 (join) with 256 x 256 tiles, 200 with 128 x 128; fp32 (three terms: 256 x 256 tiles do not fit the registers)
-// 16384 x 256 x 256 20 + 4 with 128 x 128 tiles.  Few rows (512, fp32 256) are not split: the second launch and the partial sums cost what the split
-// saves (512 x 512 x 512 bf16 10.1 / 10.0, 256 rows 7.2 / 9.0, 512 x 64 x 64 8.6 / 7.2) and a call takes 13.4 instead of 17.8 us of the host.
+// 16384 x 256 x 256 20 + 4 with 128 x 128 tiles.
+// Few rows are not split: a second launch and its partial sums cost the GPU 2-3 us and the host 4 (a call 12.3 / 16.4 us, whichever of the two is
+// longer).  Us of the GPU alone, whole / split:
+//   64 x 64     bf16 384 rows 6.7 / 6.6, 512 8.0 / 6.6, 1024 13.1 / 6.7; fp16 256 6.3 / 7.1, 512 9.5 / 7.1; fp32 256 6.9 / 7.4, 512 10.8 / 7.4
+//   512 x 512   bf16 384 8.1 / 9.0, 512 9.5 / 9.4, 640 10.9 / 10.4; fp16 384 10.5 / 9.9, 512 12.7 / 10.2; fp32 256 9.2 / 9.7, 384 11.7 / 10.4
+//   512 x 1024  bf16 384 11.5 / 13.2, 512 13.5 / 14.6; fp16 256 14.6 / 14.8, 384 18.4 / 15.7; fp32 192 14.0 / 14.7, 256 16.3 / 15.9
+//   1024 x 1024 bf16 384 19.2 / 18.9, 512 22.9 / 20.7; fp16 192 22.2 / 22.7, 256 25.9 / 24.2, 512 40.6 / 31.5; fp32 128 20.9 / 20.7, 256 30.0 / 26.3
+// Products of fewer than 2^19 entries, whose calls are the host's, are whole up to 512 (fp32: 256) rows: what a captured graph loses there, 2.5 us at
+// most, is less than the 4 that a call gains.  Larger ones are whole where the kernels are about even: 384 (fp16 256, fp32 192) rows.
 struct A8wGeo {
   int form, tk, tn, nsplit;
   long long rsplit;
 };
 struct A8wForm {
-  int tk, tn, per_cu;  // blocks that a CU's registers take
+  int tk, tn, per_cu;  // blocks a CU, as far as the registers go
 };
 static constexpr A8wForm A8W_FORMS[] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 2}, {64, 128, 2}, {64, 64, 4}};
 static constexpr long long a8w_lds(int tk, int tn, int terms) { return 3LL * A8W_RB * (tk + A8W_PAD + terms * (tn + A8W_PAD)) * 2; }
@@ -330,7 +337,9 @@ static A8wGeo a8w_geometry(long long rows, int cin, int cout, int dtype) {
   const A8wForm &f = A8W_FORMS[g.form];
   const long long fits = 160 * 1024 / a8w_lds(f.tk, f.tn, dtype == TBG_DT_F32 ? 3 : dtype == TBG_DT_F16 ? 2 : 1);
   long long want = 256LL * (f.per_cu < fits ? f.per_cu : fits) / ((long long)g.tk * g.tn);
-  const long long cap = rows <= (dtype == TBG_DT_F32 ? 256 : 512) ? 1 : g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
+  const bool wide = (long long)cin * cout >= 1 << 19;
+  const long long whole = dtype == TBG_DT_F32 ? (wide ? 192 : 256) : !wide ? 512 : dtype == TBG_DT_F16 ? 256 : 384;
+  const long long cap = rows <= whole ? 1 : g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
   if (want > cap) want = cap;
   if (want < 1) want = 1;
   g.rsplit = ((rows + want - 1) / want + A8W_RB - 1) / A8W_RB * A8W_RB;
