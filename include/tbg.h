@@ -633,7 +633,7 @@ int tbg_demod_coefs_f32(const float *s, const float *w, float *wsq, float *d, in
  * (yq, ye) = ACT8 of y as rounded to its type if not NULL (what a following layer keeps of its input).  Few positions take one launch and no
  * workspace (0 bytes: NULL).  Backward takes x or (q, e) --
  * the other NULL --, dy and stats, and writes dx [N][S][C] contiguous, dgamma, dbeta (shaped like gamma): with a checkpoint,
- * xh = q 2^e rstd everywhere.  Sums are joined in a fixed order.  Checkpoints, stats and workspace are 16-byte aligned.
+ * xh = q 2^e rstd everywhere.  x - mean is taken in fp32 (infinite where that distance is).  Sums are joined in a fixed order.  Checkpoints, stats and workspace are 16-byte aligned.
  *
  * tbg_act8_wgrad: gradients of a dense (1x1) layer y = coef x w + b, w [cin][cout], from the checkpoint of x:
  * dw[k][n] = coef sum_r x[r][k] dy[r][n], db[n] = sum_r dy[r][n] (db NULL: not wanted), fp32 accumulation on the bf16 matrix pipe: the

@@ -459,7 +459,8 @@ __global__ __launch_bounds__(GN_TW) void gn_whole_kernel(GnP p) {
 // exact product): xh but for a factor of 1 to 2, so that neither dz d nor rstd^2 leaves the range that x and dx themselves are in.
 __device__ __forceinline__ float gn_power(double rstd) { return fmaxf(__uint_as_float(__float_as_uint((float)rstd) & 0x7f800000u), 0x1p-126f); }
 __device__ __forceinline__ double gn_factor(double rstd, float power) { return rstd * (double)__uint_as_float(0x7f000000u - __float_as_uint(power)); }
-// Two launches do without it where rstd is within 2^+-32
+// Two launches do without it where rstd is within 2^+-32, whose loops have no registers left (LeakyReLU from a whole input with a channel tail keeps 8-12
+// of them in scratch as it is); in one launch it costs 0-8 % (512 x 32 x 512 bf16 SiLU 26.6 -> 28.7 us, linear 23.9 -> 24.4).
 __device__ __forceinline__ bool gn_far(double rstd) { return (unsigned)__double2hiint(rstd) - ((1023u - 32u) << 20) > 64u << 20; }
 __device__ __forceinline__ float gn_far_power(double rstd) { return gn_far(rstd) ? gn_power(rstd) : 1.f; }
 struct GnCh {
@@ -903,7 +904,7 @@ static size_t gn_team_lds(const GnP &p, bool backward) {
 // block's lanes.  Samples for more than the card's threads: tiles of up to GN_CT channels, as few lanes a sample as its rows need.
 // Forward (bf16, SiLU, us of kernels, one launch / two): 1 x 64 x 256 channels 8.4 / 10.0, 32 x 16 x 64 7.0 / 9.8, 128 x 64 x 512 14.5 / 17.6, 512 x 32
 // x 512 18 / 37, 65536 x 1 x 256 55 / 4800; a few blocks of full registers 11.1 / 9.6 (1 x 1024 x 32), where the launch saved is worth the rest.
-// Backward: one launch where it makes the parameters' gradients whole as well (1 x 64 x 256 9.1 / 10.9) or where samples are many (512 x 32 x 512 27 / 39,
+// Backward: one launch where it makes the parameters' gradients whole as well (1 x 64 x 256 9.0 / 12.7) or where samples are many (512 x 32 x 512 29 / 43,
 // 65536 x 1 x 256 84 / 1390); between, a second launch would join them (32 x 64 x 512 14.4 / 13.4, 4 x 128 x 256 13.3 / 11.5).
 static bool gn_one_launch(GnP &p, int least_ct, bool backward) {
   const int T = backward ? GN_T : GN_TW, R = backward ? GN_RB : GN_R;
@@ -1068,7 +1069,8 @@ static int gn_dispatch(const tbg_gn_desc *d, const GnP &p, bool backward, void *
 // Calls that move more than the 256 MB of the card's memory-side cache read (for the second and last time) and write past the caches: lines that
 // are left to be written back slow the next launch's reads, and what the first launch has read stays for the second.  32 x 16384 x 128 bf16 with 8-bit
 // checkpoint (337 MB a direction): sums 33.8 -> 27.1, second launch 66 -> 54, backward sums 55.9 -> 48, second launch 63 -> 56 us.  Smaller calls
-// leave their results to the next reader (unpacking a 69 MB checkpoint takes 17.4 us, 19.3 if it was written past them).
+// leave their results to the next reader (unpacking a 69 MB checkpoint takes 17.4 us, 19.3 if it was written past them).  Rows of other than whole 8
+// channels have no such form: their last lanes move single elements.
 static bool gn_past(const tbg_gn_desc *d, int bytes) {
   return (double)d->N * d->S * d->C * bytes > 256e6;
 }
