@@ -639,6 +639,7 @@ int tbg_demod_coefs_f32(const float *s, const float *w, float *wsq, float *d, in
  * dw[k][n] = coef sum_r x[r][k] dy[r][n], db[n] = sum_r dy[r][n] (db NULL: not wanted), fp32 accumulation on the bf16 matrix pipe: the
  * checkpoint is exact in bf16, dy is one (bf16), two (fp16) or three (fp32) bf16 terms (an infinity in fp16 or fp32 leaves NaN in its column of
  * dw).  dw, db contiguous.
+ * tbg_column_sums: out[c] = sum_r x[r][c] in fp32 (the bias gradient where the weight is frozen and its input not kept); workspace as above.
  * TBG_ERANGE: more than 2^30 positions, 2^24 channels (2^20 of a dense layer), or a launch of 2^32 threads or more.
  * ---------------------------------------------------------------------------------------- */
 #define TBG_ACT_SILU 2
@@ -660,6 +661,9 @@ int tbg_group_norm_bwd(const tbg_gn_desc *d, const void *x, const void *q, const
 long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int cout, int dtype);
 int tbg_act8_wgrad(const void *q, const void *e, const void *dy, int dtype, long long rows, int cin, int cout, long long ldy, float coef,
                    float *dw, float *db, void *workspace, long long workspace_bytes, void *stream);
+long long tbg_column_sums_workspace_bytes(long long rows, int cols, int dtype);
+int tbg_column_sums(const void *x, int dtype, long long rows, int cols, long long ldx, float *out, void *workspace, long long workspace_bytes,
+                    void *stream);
 
 #ifdef __cplusplus
 }

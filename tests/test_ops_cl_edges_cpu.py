@@ -1,4 +1,5 @@
 """Channels-last layers at the ends of their types' ranges and next to callers' modes (no GPU)."""
+import ctypes as C
 import os
 import re
 import subprocess
@@ -126,3 +127,15 @@ def test_weight_gradients_of_few_rows_take_one_launch(dtype, narrow, wide):
     space = native.lib().tbg_act8_wgrad_workspace_bytes
     for rows, cin, cout in ((narrow, 512, 512), (narrow, 64, 64), (narrow, 512, 1023), (wide, 512, 1024), (wide, 1024, 1024)):
         assert space(rows, cin, cout, dtype) == 0 < space(rows + 1, cin, cout, dtype), (rows, cin, cout)
+
+
+def test_column_sums_entry_checks_its_arguments():
+    lib, p, odd = native.lib(), C.c_void_p(256), C.c_void_p(264)
+    space = lib.tbg_column_sums_workspace_bytes
+    assert space(1, 1, 0) == 0 and space(0, 1, 0) == -1 and space(1, 0, 0) == -1 and space(1, 1, 3) == -1 and space(1, (1 << 30) + 1, 0) == -2
+    need = space(100000, 72, 1)
+    assert need > 0 and need % (72 * 4) == 0
+    call = lambda x, dt, rows, cols, ld, out, ws, n: lib.tbg_column_sums(x, dt, rows, cols, ld, out, ws, n, None)
+    assert call(None, 1, 100000, 72, 72, p, p, need) == -1 and call(p, 1, 100000, 72, 72, None, p, need) == -1
+    assert call(p, 1, 100000, 72, 71, p, p, need) == -1 and call(p, 1, 0, 72, 72, p, p, need) == -1 and call(p, 3, 100000, 72, 72, p, p, need) == -1
+    assert call(p, 1, 100000, 72, 72, p, p, need - 1) == -1 and call(p, 1, 100000, 72, 72, p, None, need) == -1 and call(p, 1, 100000, 72, 72, p, odd, need) == -1

@@ -27,7 +27,7 @@ EXPORTS = [
     "tbg_units_s2_bytes", "tbg_units_pack_s2_f32", "tbg_upfirdn2d_units_s2_f32", "tbg_conv2d_units_s2_blocks", "tbg_conv2d_units_s2_tile_channels", "tbg_conv2d_units_s2_dot_slots", "tbg_conv2d_units_s2", "tbg_conv2d_wgrad_units_s2_workspace_bytes", "tbg_conv2d_wgrad_units_s2", "tbg_conv2d_units_t2_blocks", "tbg_conv2d_units_t2",
     "tbg_slab_epilogue_units_f32", "tbg_conv2d_units_small", "tbg_conv2d_units_small_blocks", "tbg_conv2d_units_small_dot_slots", "tbg_conv2d_units_small_tile_pixels", "tbg_lstm_fused_fwd_f32", "tbg_lstm_fused_bwd_f32", "tbg_lstm_cell_fused_fwd_f32", "tbg_rows_gemv_t_f32", "tbg_dec_sample_fwd_f32", "tbg_dec_sample_bwd_f32",
     "tbg_bias_act_bwd_f32", "tbg_axpby_planes_f32", "tbg_bias_act_bwd2_f32", "tbg_rgb_project_f32", "tbg_rgb_backproject_f32", "tbg_rgb_backproject_chunks", "tbg_adam_tf_f32", "tbg_ema_lerp_f32", "tbg_demod_coefs_f32",
-    "tbg_act8_pack", "tbg_act8_unpack", "tbg_group_norm_workspace_bytes", "tbg_group_norm_fwd", "tbg_group_norm_bwd", "tbg_act8_wgrad_workspace_bytes", "tbg_act8_wgrad",
+    "tbg_act8_pack", "tbg_act8_unpack", "tbg_group_norm_workspace_bytes", "tbg_group_norm_fwd", "tbg_group_norm_bwd", "tbg_act8_wgrad_workspace_bytes", "tbg_act8_wgrad", "tbg_column_sums_workspace_bytes", "tbg_column_sums",
 ]
 
 
@@ -192,6 +192,9 @@ def lib():
         l.tbg_act8_wgrad_workspace_bytes.argtypes = [ll, ci, ci, ci]
         l.tbg_act8_wgrad_workspace_bytes.restype = ll
         l.tbg_act8_wgrad.argtypes = [vp, vp, vp, ci, ll, ci, ci, ll, cf, vp, vp, vp, ll, vp]
+        l.tbg_column_sums_workspace_bytes.argtypes = [ll, ci, ci]
+        l.tbg_column_sums_workspace_bytes.restype = ll
+        l.tbg_column_sums.argtypes = [vp, ci, ll, ci, ll, vp, vp, ll, vp]
         _lib = _LibProxy(l)
     return _lib
 

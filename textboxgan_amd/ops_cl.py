@@ -378,6 +378,22 @@ def _dense_dx(dy, w, coef, shape, dtype):
     return (dy.reshape(-1, w.shape[1]) @ (w * coef).to(dtype).t()).reshape(shape)
 
 
+def _column_sums(dy):
+    """db [cout] = sum of dy's rows, in fp32.  (torch's sum over many rows clears its counters by a memset, which a captured graph does not replay
+    reliably.)"""
+    cout, dev = dy.shape[-1], dy.device
+    db = torch.empty(cout, device=dev, dtype=torch.float32)
+    if not dy.numel():
+        return db.zero_()
+    dy, rows, pitch = _rows(dy)
+    dt = _DTYPES[dy.dtype]
+    nbytes = N.lib().tbg_column_sums_workspace_bytes(rows, cout, dt)
+    N.check(min(nbytes, 0), "tbg_column_sums_workspace_bytes")
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    _call("tbg_column_sums", dy, dy.data_ptr(), dt, rows, cout, pitch, db.data_ptr(), _ptr(ws), nbytes)
+    return db
+
+
 class _DenseAct8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, coef, q, e):
@@ -402,7 +418,7 @@ class _DenseAct8(torch.autograd.Function):
         if need[1]:
             dw, db = act8_wgrad(Act8(q, e, shape, dtype), dy, coef, need[2])
         elif need[2]:
-            db = dy.reshape(-1, w.shape[1]).sum(dim=0, dtype=torch.float32)
+            db = _column_sums(dy)
         return dx, dw, db, None, None, None
 
 
