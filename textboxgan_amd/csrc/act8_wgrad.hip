@@ -83,12 +83,13 @@ __global__ __launch_bounds__(64 * KW * NW, 2) void act8_wgrad_kernel(A8wP p) {
   extern __shared__ __align__(16) char smem[];
   unsigned short *lds = reinterpret_cast<unsigned short *>(smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wk = wave % KW, wn = wave / KW;
-  // 8 neighbouring splits x all tiles of a split: blocks go round the 8 XCDs, so the tiles that share a split's rows share an L2
-  const int tiles = p.tk * p.tn;
-  int b = blockIdx.x;
-  const int z = b / (8 * tiles) * 8 + (b & 7);
-  b = b % (8 * tiles) / 8;
-  if (z >= p.nsplit) return;
+  // (split, tile) pairs, a split's tiles together, in 8 equal runs: blocks go round the 8 XCDs, so that the tiles that share a split's rows share an L2,
+  // and all XCDs have the same work whatever the number of splits
+  const int tiles = p.tk * p.tn, pairs = p.nsplit * tiles;
+  int b = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (b >= pairs) return;
+  const int z = b / tiles;
+  b -= z * tiles;
   const int k0 = (b / p.tn) * TK, n0 = (b % p.tn) * TN;
   const long long r0 = z * p.rsplit, rend = min(p.rows, r0 + p.rsplit);
   const bool do_db = p.want_db && k0 == 0;
@@ -367,7 +368,7 @@ extern "C" long long tbg_act8_wgrad_workspace_bytes(long long rows, int cin, int
 template <class E, int NP, int WM, int WN, int KW, int NW>
 static int a8w_launch(const A8wP &p, bool vec, hipStream_t st) {
   constexpr size_t lds = a8w_lds(32 * WM * KW, 32 * WN * NW, NP);
-  const unsigned blocks = (unsigned)((p.nsplit + 7) / 8 * 8 * p.tk * p.tn);
+  const unsigned blocks = (unsigned)((p.nsplit * p.tk * p.tn + 7) / 8 * 8);
   const auto kern = vec ? act8_wgrad_kernel<E, NP, WM, WN, KW, NW, true> : act8_wgrad_kernel<E, NP, WM, WN, KW, NW, false>;
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
     return TBG_EHIP;
