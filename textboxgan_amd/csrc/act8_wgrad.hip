@@ -306,18 +306,16 @@ __global__ __launch_bounds__(256) void act8_wgrad_join_kernel(const float *ws, c
 // Tile and row splits.  The tile: the largest that the channels fill (fewer re-reads of both operands, fewer operand reads an MFMA), made
 // smaller while splits of 256 rows would leave a quarter of the CUs without a block; the splits then fill the card once: as many blocks a CU as its
 // registers and its 160 KB of LDS hold (the three buffers take 60 KB for 128 x 128 of one term, 120 KB of three).  Calls, us, with the splits of one
-// round of blocks / of two: fp32 65536 x 256 x 256 44 / 50, 262144 x 64 x 64 24 / 30, 262144 x 512 x 512 512 / 520; fp16 36 / 43, 20.6 / 26.6, but
+// round of blocks / of two: fp32 65536 x 256 x 256 44 / 50, 262144 x 64 x 64 24 / 30, 20000 x 1024 x 512 89 / 93; fp16 36 / 43, 21 / 27, 69 / 72, but
 // 262144 x 512 x 512 407 / 391.  Measured, us of kernels:
 // 262144 x 512 x 512 bf16 158 + 12 (join) with 256 x 256 tiles, 200 with 128 x 128; fp32 (three terms: 256 x 256 tiles do not fit the registers)
 // 16384 x 256 x 256 20 + 4 with 128 x 128 tiles.
-// Few rows are not split: a second launch and its partial sums cost the GPU 2-3 us and the host 4 (a call 12.3 / 16.4 us, whichever of the two is
-// longer).  Us of the GPU alone, whole / split:
-//   64 x 64     bf16 384 rows 6.7 / 6.6, 512 8.0 / 6.6, 1024 13.1 / 6.7; fp16 256 6.3 / 7.1, 512 9.5 / 7.1; fp32 256 6.9 / 7.4, 512 10.8 / 7.4
-//   512 x 512   bf16 384 8.1 / 9.0, 512 9.5 / 9.4, 640 10.9 / 10.4; fp16 384 10.5 / 9.9, 512 12.7 / 10.2; fp32 256 9.2 / 9.7, 384 11.7 / 10.4
-//   512 x 1024  bf16 384 11.5 / 13.2, 512 13.5 / 14.6; fp16 256 14.6 / 14.8, 384 18.4 / 15.7; fp32 192 14.0 / 14.7, 256 16.3 / 15.9
-//   1024 x 1024 bf16 384 19.2 / 18.9, 512 22.9 / 20.7; fp16 192 22.2 / 22.7, 256 25.9 / 24.2, 512 40.6 / 31.5; fp32 128 20.9 / 20.7, 256 30.0 / 26.3
-// Products of fewer than 2^19 entries, whose calls are the host's, are whole up to 512 (fp32: 256) rows: what a captured graph loses there, 2.5 us at
-// most, is less than the 4 that a call gains.  Larger ones are whole where the kernels are about even: 384 (fp16 256, fp32 192) rows.
+// Up to 512 rows are not split: a second launch and its partial sums cost the host 4 us (a call 12.3 / 16.4 us, whichever of the two is longer), and the
+// GPU more than the split saves where the product is wide.  Us of the GPU alone, whole / split:
+//   64 x 64      bf16 256 rows 5.5 / 6.5, 512 8.0 / 6.6, 768 10.6 / 6.7; fp16 256 6.4 / 7.0, 512 9.7 / 7.1; fp32 256 7.0 / 7.4, 512 10.9 / 7.5
+//   512 x 512    bf16 256 5.6 / 7.4, 512 8.2 / 8.5, 768 10.7 / 10.3; fp16 256 6.5 / 7.9, 512 9.9 / 9.2; fp32 256 7.2 / 8.4, 512 11.3 / 9.6
+//   1024 x 1024  bf16 256 6.0 / 13.0, 512 8.7 / 20.4, 640 14.2 / 16.7; fp16 512 10.4 / 15.5, 640 18.8 / 18.1; fp32 512 11.5 / 16.6, 640 23.9 / 20.3
+// (narrow products in a captured graph, which has no host, lose up to 3.4 us).
 struct A8wGeo {
   int form, tk, tn, nsplit;
   long long rsplit;
@@ -338,9 +336,7 @@ static A8wGeo a8w_geometry(long long rows, int cin, int cout, int dtype) {
   const A8wForm &f = A8W_FORMS[g.form];
   const long long fits = 160 * 1024 / a8w_lds(f.tk, f.tn, dtype == TBG_DT_F32 ? 3 : dtype == TBG_DT_F16 ? 2 : 1);
   long long want = 256LL * (f.per_cu < fits ? f.per_cu : fits) / ((long long)g.tk * g.tn);
-  const bool wide = (long long)cin * cout >= 1 << 19;
-  const long long whole = dtype == TBG_DT_F32 ? (wide ? 192 : 256) : !wide ? 512 : dtype == TBG_DT_F16 ? 256 : 384;
-  const long long cap = rows <= whole ? 1 : g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
+  const long long cap = rows <= 512 ? 1 : g.form == 4 ? (rows + 4 * A8W_RB - 1) / (4 * A8W_RB) : most;
   if (want > cap) want = cap;
   if (want < 1) want = 1;
   g.rsplit = ((rows + want - 1) / want + A8W_RB - 1) / A8W_RB * A8W_RB;
